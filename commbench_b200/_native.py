@@ -109,6 +109,16 @@ _HOT_ARGTYPES = {
     "cb_moe_router_topk": [_P, _I, _I, _I, _P, _P, _P],
     "cb_moe_slots": [_P, _I, _I, _P, _P, _P],
     "cb_moe_plan": [_P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P],
+    "cb_rms_norm": [_P] * 7 + [_L] * 3 + [_I] * 4 + [_F, _P],
+    "cb_rms_norm_backward_floats": [_P] * 5 + [_L] * 4 + [_I] * 3,
+    "cb_rms_norm_backward": [_P] * 7 + [_L] * 4 + [_I] * 3 + [_F, _P],
+    "cb_rope": ([_P, _P, _L, _L, _L, _I] * 2 + [_I] * 3 + [_P, _P, _I, _I, _I, _P] + [_I] * 4 + [_P, _P]),
+    "cb_kv_append": ([_P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _P, _P] + [_I] * 3 +
+                     [_P, _P]),
+    "cb_kv_read": [_P, _P, _I, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P, _P],
+    "cb_kv_attend_bytes": [_I] * 5,
+    "cb_kv_attend": ([_P, _P, _I, _I, _I, _P, _L, _L, _L, _P, _P, _P, _I, _P, _P] + [_I] * 6 +
+                     [_F, _P, _L, _P, _P]),
 }
 
 
@@ -128,7 +138,8 @@ def load():
                 "(or __graft_entry__.build()) first")
     lib = C.CDLL(str(_LIB_PATH), mode=C.RTLD_GLOBAL)
     lib.cb_last_error.restype = C.c_char_p
-    for name in ("cb_symm_round_size", "cb_attn_split_bytes"):
+    for name in ("cb_symm_round_size", "cb_attn_split_bytes", "cb_rms_norm_backward_floats",
+                 "cb_kv_attend_bytes"):
         getattr(lib, name).restype = C.c_longlong
     for name, args in _HOT_ARGTYPES.items():
         getattr(lib, name).argtypes = args

@@ -1,0 +1,75 @@
+// The paged 8-bit key/value cache: how it lies in memory, and its numbers.
+//
+//   data [pages][kv heads][2: key, value][page tokens][128] e4m3, exps [pages][kv heads][2] int8
+//
+// An element is worth e4m3 * 2^exp: one power-of-two scale for the keys and one for the values of a page and head.
+// e4m3 is itself a floating-point type, so a scale that is not a power of two would buy at most one bit of range
+// and no precision, and a power of two lets the scale of a block grow when a larger token comes: the older tokens
+// of the block are multiplied by 2^(old - new), exact but for the numbers below 2^-6 (e4m3 subnormals).
+//
+// Keys and values of a (page, head) are one piece of 256 x page bytes, so that a few bulk copies bring a tile.  A
+// token's row is eight chunks of 16 bytes; chunk c of token t lies at c ^ (t & 7), which lets ldmatrix read eight
+// rows of one chunk without bank conflicts from a tile that was copied as it is.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+namespace cb {
+
+static constexpr int KV_D = 128;
+static constexpr int KV_EXP_MIN = -120, KV_EXP_MAX = 120;
+
+struct KvCacheView {
+  uint8_t* data;
+  int8_t* exps;
+  int num_pages, hkv, page_log2;
+  __host__ __device__ int page() const { return 1 << page_log2; }
+  __device__ __forceinline__ uint8_t* tile(int pid, int head, int side) const {
+    return data + ((static_cast<long long>(pid) * hkv + head) * 2 + side) * (static_cast<long long>(KV_D) << page_log2);
+  }
+  __device__ __forceinline__ int8_t* exp_of(int pid, int head, int side) const {
+    return exps + (static_cast<long long>(pid) * hkv + head) * 2 + side;
+  }
+};
+
+// The sequences of a call: page ids [B, cols], tokens that were there before, new tokens (null: all S).
+struct KvBatch {
+  const int* pages;
+  const int* start;
+  const int* count;
+  int B, S, cols;
+  __device__ __forceinline__ int new_tokens(int b) const {
+    if (count == nullptr) return S;
+    const int c = count[b];
+    return c < 0 ? 0 : c < S ? c : S;
+  }
+};
+
+// Byte offset of element d (a multiple of 4) of token slot t inside a tile.
+__device__ __forceinline__ int kv_offset(int t, int d) { return t * KV_D + (((d >> 4) ^ (t & 7)) << 4) + (d & 15); }
+
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float kv_pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// The smallest e with amax * 2^-e <= 448 = 1.75 * 2^8.
+__device__ __forceinline__ int kv_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  if (amax == 0.f || e < KV_EXP_MIN) e = KV_EXP_MIN;
+  return e > KV_EXP_MAX ? KV_EXP_MAX : e;
+}
+
+__device__ __forceinline__ uint32_t kv_encode4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+// Two e4m3 numbers (the low 16 bits) as fp16, exactly.
+__device__ __forceinline__ uint32_t kv_to_half2(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
+  return h;
+}
+
+}  // namespace cb

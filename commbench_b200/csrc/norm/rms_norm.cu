@@ -1,0 +1,517 @@
+// Root-mean-square norm of rows with the residual's addition, its 8-bit form and its gradient.
+//
+//   h = x + residual      rstd = 1 / sqrt(mean(h^2) + eps)      y = h * rstd * w
+//   8 bits: per row and 128 columns s = max|y| / 448 (or the next power of two), q = e4m3(y / s)
+//   g = dy * w            dx = rstd * g - h * rstd^3 / D * sum(g h) + dh          dw = sum over rows of dy * h * rstd
+//
+// Bound by memory: every operand is read once and every result written once.  A row stays in the registers of
+// one warp (short rows) or one CTA between the sum of squares and the product, as fp32: h is normalised before
+// it is rounded to its 16-bit copy, and y is rounded once, to its type or to e4m3.
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <string>
+
+#include "../prim/elem.cuh"
+#include "../prim/pdl.cuh"
+
+namespace cb {
+void set_last_error(const std::string& s);
+
+struct NormParams {
+  const void* x;
+  const void* res;    // or null
+  const void* w;
+  void* y;            // type of x, or e4m3
+  void* h;            // x + residual, or null
+  float* scale;       // 8 bits: [rows, D / 128]
+  uint8_t* sf;        // packed exponent bytes, see quant_blockscaled_kernel (gemm/blockscale.cu), or null
+  long long x_stride, res_stride;   // elements between rows; y and h are dense
+  long long rows;
+  int D, w_f32;
+  float eps;
+};
+
+template <class T, int V>
+__device__ __forceinline__ void load_weight(const void* w, int w_f32, int col, float (&x)[V]) {
+  if (w_f32) {
+#pragma unroll
+    for (int i = 0; i < V; i += V >= 4 ? 4 : 1) {
+      if constexpr (V >= 4) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + col + i));
+        x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
+      } else {
+        x[i] = __ldg(static_cast<const float*>(w) + col + i);
+      }
+    }
+  } else {
+    load_vec<T, V>(static_cast<const T*>(w) + col, x);
+  }
+}
+
+// Sum over the threads of a row: a warp, or the whole CTA (`sh` holds two rounds, so that one barrier a call is
+// enough).
+template <bool kWarpRow>
+__device__ __forceinline__ float row_sum(float v, float (*sh)[32], int round) {
+  v = warp_sum(v);
+  if constexpr (kWarpRow) return v;
+  float* s = sh[round & 1];
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum((threadIdx.x & 31) < (blockDim.x >> 5) ? s[threadIdx.x & 31] : 0.f);
+}
+
+enum NormMode : int { NORM_PLAIN = 0, NORM_SCALE = 1, NORM_POW2 = 2 };
+
+// 8-bit output of the V columns from `col` on: 128 / V neighbouring lanes hold a block.
+template <int V, int kMode>
+__device__ __forceinline__ void store_quantised(const NormParams& p, long long row, int col, const float (&y)[V],
+                                                bool active) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) amax = fmaxf(amax, fabsf(y[i]));
+#pragma unroll
+  for (int o = 64 / V; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  float s = amax > 0.f ? amax / 448.f : 1.f;
+  const int kb = col >> 7, kblocks = p.D >> 7;
+  if constexpr (kMode == NORM_POW2) {
+    const uint32_t bits = __float_as_uint(s);
+    uint32_t e = (bits >> 23) & 0xffu;
+    if ((bits & 0x7fffffu) != 0u) ++e;
+    e = min(max(e, 1u), 254u);
+    s = __uint_as_float(e << 23);
+    if (active && (col & 127) == 0 && p.sf != nullptr) {
+      uint8_t* word = p.sf + (static_cast<long long>(kb >> 2) * p.rows + row) * 4;
+      word[kb & 3] = static_cast<uint8_t>(e);
+      if (kb == kblocks - 1)
+        for (int i = (kb & 3) + 1; i < 4; ++i) word[i] = 127;   // missing blocks: 1.0
+    }
+  }
+  if (!active) return;
+  if ((col & 127) == 0) p.scale[row * kblocks + kb] = s;
+  const float inv = 1.f / s;
+  uint32_t q[V / 4];
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[i] * inv, y[i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi =
+        __nv_cvt_float2_to_fp8x2(make_float2(y[i + 2] * inv, y[i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    q[i / 4] = lo | (hi << 16);
+  }
+  uint8_t* dst = static_cast<uint8_t*>(p.y) + row * p.D + col;
+  if constexpr (V == 8)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+  else
+    *reinterpret_cast<uint32_t*>(dst) = q[0];
+}
+
+// VPT vectors of V columns per thread, `threads` threads a row (32 or the CTA).
+template <class T, int V, int VPT, bool kWarpRow, int kMode>
+__global__ void __launch_bounds__(VPT == 4 || VPT == 8 ? 512 : 1024) rms_norm_kernel(const __grid_constant__ NormParams p) {
+  __shared__ float sh[2][32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int threads = kWarpRow ? 32 : blockDim.x;
+  const int t = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
+  const long long row = kWarpRow ? blockIdx.x * static_cast<long long>(blockDim.x >> 5) + (threadIdx.x >> 5)
+                                 : blockIdx.x;
+  if (row >= p.rows) return;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  const T* r = p.res == nullptr ? nullptr : static_cast<const T*>(p.res) + row * p.res_stride;
+  float h[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int col = (i * threads + t) * V;
+    if (col < p.D) load_vec<T, V>(x + col, h[i]);
+    else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[i][j] = 0.f;
+    }
+  }
+  if (r != nullptr) {
+    float a[VPT][V];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int col = (i * threads + t) * V;
+      if (col < p.D) load_vec<T, V>(r + col, a[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int col = (i * threads + t) * V;
+      if (col < p.D) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[i][j] += a[i][j];
+        store_vec<T, V>(static_cast<T*>(p.h) + row * p.D + col, h[i]);
+      }
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) ss += h[i][j] * h[i][j];
+  ss = row_sum<kWarpRow>(ss, sh, 0);
+  const float rstd = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int col = (i * threads + t) * V;
+    const bool active = col < p.D;
+    float w[V];
+    if (active) {
+      load_weight<T, V>(p.w, p.w_f32, col, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rstd * w[j];
+    }
+    if constexpr (kMode == NORM_PLAIN) {
+      if (active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
+    } else {
+      store_quantised<V, kMode>(p, row, col, h[i], active);
+    }
+  }
+}
+
+struct NormBwdParams {
+  const void *dy, *h, *w, *dh;   // dh or null
+  void* dx;
+  float* part;                   // [gridDim.x, D]
+  long long dy_stride, h_stride, dh_stride, rows;
+  int D, w_f32;
+  float eps;
+};
+
+// A CTA takes rows blockIdx.x, blockIdx.x + gridDim.x, ... with the next row's operands on their way while the
+// present one is summed up.  A thread keeps its columns through all of them, and with them its share of dw, which
+// goes to `part` at the end: sums of a fixed order, no atomics.
+// Long rows have no registers left for that and for the weights: they read both when they need them.
+template <class T, int V, int VPT>
+__global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
+  __shared__ float sh[2][2][32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int t = threadIdx.x, threads = blockDim.x, lane = t & 31;
+  using V16 = Vec<T, V>;
+  V16 zero;
+#pragma unroll
+  for (int j = 0; j < V; ++j) zero.e[j] = from_f32<T>(0.f);
+  const T* dy = static_cast<const T*>(p.dy);
+  const T* h = static_cast<const T*>(p.h);
+  const T* dh = static_cast<const T*>(p.dh);
+  constexpr bool kAhead = VPT == 1;
+  float w1[V], dw[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) w1[j] = dw[i][j] = 0.f;
+  if (kAhead && t * V < p.D) load_weight<T, V>(p.w, p.w_f32, t * V, w1);
+  auto weight = [&](int i, float(&w)[V]) {
+    const int col = (i * threads + t) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] = kAhead ? w1[j] : 0.f;
+    if (!kAhead && col < p.D) load_weight<T, V>(p.w, p.w_f32, col, w);
+  };
+  V16 ny[VPT], nh[VPT], nd[VPT];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int col = (i * threads + t) * V;
+      ny[i] = nh[i] = nd[i] = zero;
+      if (col < p.D && row < p.rows) {
+        ny[i] = *reinterpret_cast<const V16*>(dy + row * p.dy_stride + col);
+        nh[i] = *reinterpret_cast<const V16*>(h + row * p.h_stride + col);
+        if (dh != nullptr) nd[i] = *reinterpret_cast<const V16*>(dh + row * p.dh_stride + col);
+      }
+    }
+  };
+  if (kAhead) fetch(blockIdx.x);
+  int round = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, ++round) {
+    if (!kAhead) fetch(row);
+    V16 cy[VPT], ch[VPT], cd[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) cy[i] = ny[i], ch[i] = nh[i], cd[i] = nd[i];
+    if (kAhead) fetch(row + gridDim.x);
+    float ss = 0.f, gh = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float w[V];
+      weight(i, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = to_f32(ch[i].e[j]);
+        ss += a * a;
+        gh += to_f32(cy[i].e[j]) * w[j] * a;
+      }
+    }
+    ss = warp_sum(ss);
+    gh = warp_sum(gh);
+    float(*s)[32] = sh[round & 1];
+    if (lane == 0) s[0][t >> 5] = ss, s[1][t >> 5] = gh;
+    __syncthreads();
+    const bool have = lane < (threads >> 5);
+    ss = warp_sum(have ? s[0][lane] : 0.f);
+    gh = warp_sum(have ? s[1][lane] : 0.f);
+    const float rstd = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
+    const float c = rstd * rstd * rstd * (gh / static_cast<float>(p.D));
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int col = (i * threads + t) * V;
+      float dx[V], w[V];
+      weight(i, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = to_f32(ch[i].e[j]), b = to_f32(cy[i].e[j]);
+        dx[j] = rstd * (b * w[j]) - a * c + to_f32(cd[i].e[j]);
+        dw[i][j] += b * (a * rstd);
+      }
+      if (col < p.D) store_vec<T, V>(static_cast<T*>(p.dx) + row * p.D + col, dx);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int col = (i * threads + t) * V;
+    if (col < p.D) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) p.part[static_cast<long long>(blockIdx.x) * p.D + col + j] = dw[i][j];
+    }
+  }
+}
+
+// dw[col] = sum of `parts` rows, always in the same order.
+__global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, float* dw, int parts, int D) {
+  __shared__ float sh[32][33];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + x;
+  float s = 0.f;
+  if (col < D)
+    for (int i = y; i < parts; i += 32) s += part[static_cast<long long>(i) * D + col];
+  sh[y][x] = s;
+  __syncthreads();
+  s = warp_sum(sh[x][y]);
+  if (x == 0 && blockIdx.x * 32 + y < D) dw[blockIdx.x * 32 + y] = s;
+}
+
+static bool aligned(const void* p, long long stride, int elem, int V) {
+  const uintptr_t bytes = static_cast<uintptr_t>(elem) * V;
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (stride * elem) % bytes == 0);
+}
+
+static int norm_sms() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
+    return 148;
+  return n;
+}
+
+static int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return 0;
+  cudaGetLastError();   // reported here, not by the next call
+  set_last_error(std::string(what) + ": " + cudaGetErrorString(e));
+  return -1;
+}
+
+template <class T, int V, int VPT, int kMode>
+static int launch_norm(const NormParams& p, cudaStream_t st) {
+  const long long vecs = (p.D + V - 1) / V;
+  if (vecs <= 32 * VPT && p.rows > 1) {
+    const int warps = 4;
+    return launched(launch_pdl(rms_norm_kernel<T, V, VPT, true, kMode>,
+                               dim3(static_cast<unsigned>((p.rows + warps - 1) / warps)), dim3(32 * warps), 0, st, p),
+                    "rms_norm launch");
+  }
+  const int threads = static_cast<int>((vecs + VPT - 1) / VPT + 31) / 32 * 32;
+  return launched(launch_pdl(rms_norm_kernel<T, V, VPT, false, kMode>, dim3(static_cast<unsigned>(p.rows)),
+                             dim3(static_cast<unsigned>(threads)), 0, st, p),
+                  "rms_norm launch");
+}
+
+// Vectors per thread: rows that are too few to fill the chip are spread over as many threads as they have vectors.
+template <class T, int V, int kMode>
+static int pick_norm(const NormParams& p, cudaStream_t st) {
+  const long long vecs = (p.D + V - 1) / V;
+  const bool few = p.rows <= 2 * norm_sms();
+  if (few && vecs <= 1024) return launch_norm<T, V, 1, kMode>(p, st);
+  if (few && vecs <= 2048) return launch_norm<T, V, 2, kMode>(p, st);
+  if (vecs <= 2048) return launch_norm<T, V, 4, kMode>(p, st);
+  if (vecs <= 4096) return launch_norm<T, V, 8, kMode>(p, st);
+  if constexpr (V < 4) {
+    if (vecs <= 16384) return launch_norm<T, V, 16, kMode>(p, st);
+  }
+  set_last_error("rms_norm: row too long");
+  return -1;
+}
+
+template <class T, int kMode>
+static int norm_typed(const NormParams& p, cudaStream_t st) {
+  constexpr int kFull = 16 / sizeof(T), E = sizeof(T);
+  auto fits = [&](int V) {
+    return p.D % V == 0 && aligned(p.x, p.x_stride, E, V) && aligned(p.res, p.res_stride, E, V) &&
+           aligned(p.h, p.D, E, V) && aligned(p.w, 0, p.w_f32 ? 4 : E, p.w_f32 && V > 4 ? 4 : V) &&
+           aligned(p.y, p.D, kMode == NORM_PLAIN ? E : 1, V);
+  };
+  if (fits(kFull)) return pick_norm<T, kFull, kMode>(p, st);
+  if constexpr (kMode == NORM_PLAIN) {
+    if (E == 2 && fits(2)) return pick_norm<T, 2, kMode>(p, st);
+    return pick_norm<T, 1, kMode>(p, st);
+  } else {
+    set_last_error("rms_norm: the 8-bit form wants 16-byte aligned rows");
+    return -1;
+  }
+}
+
+template <class T, int V, int VPT>
+static int launch_bwd(const NormBwdParams& p0, float* dw, int grid, int threads, cudaStream_t st) {
+  NormBwdParams p = p0;
+  if (launched(launch_pdl(rms_norm_bwd_kernel<T, V, VPT>, dim3(static_cast<unsigned>(grid)),
+                          dim3(static_cast<unsigned>(threads)), 0, st, p),
+               "rms_norm_backward launch"))
+    return -1;
+  return launched(launch_pdl(rms_norm_dw_kernel, dim3(static_cast<unsigned>((p.D + 31) / 32)), dim3(1024), 0, st,
+                             static_cast<const float*>(p.part), dw, grid, p.D),
+                  "rms_norm_backward launch");
+}
+
+struct BwdShape {
+  int V, VPT, threads, grid;
+};
+static BwdShape bwd_shape(const NormBwdParams& p, int E) {
+  auto fits = [&](int V) {
+    return p.D % V == 0 && aligned(p.dy, p.dy_stride, E, V) && aligned(p.h, p.h_stride, E, V) &&
+           aligned(p.dh, p.dh_stride, E, V) && aligned(p.dx, p.D, E, V) &&
+           aligned(p.w, 0, p.w_f32 ? 4 : E, p.w_f32 && V > 4 ? 4 : V);
+  };
+  BwdShape s;
+  s.V = fits(16 / E) ? 16 / E : (E == 2 && fits(2)) ? 2 : 1;
+  const int vecs = (p.D + s.V - 1) / s.V;
+  s.VPT = vecs <= 1024 ? 1 : vecs <= 2048 ? 4 : vecs <= 4096 ? 8 : vecs <= 8192 && s.V < 4 ? 16 : 0;
+  if (s.VPT == 0) return s;
+  s.threads = ((vecs + s.VPT - 1) / s.VPT + 31) / 32 * 32;
+  int per_sm = 1024 / s.threads;
+  if (per_sm > 8) per_sm = 8;
+  const long long most = static_cast<long long>(norm_sms()) * per_sm;
+  s.grid = static_cast<int>(p.rows < most ? p.rows : most);
+  return s;
+}
+
+template <class T, int V>
+static int bwd_vec(const NormBwdParams& p, float* dw, const BwdShape& s, cudaStream_t st) {
+  switch (s.VPT) {
+    case 1: return launch_bwd<T, V, 1>(p, dw, s.grid, s.threads, st);
+    case 4: return launch_bwd<T, V, 4>(p, dw, s.grid, s.threads, st);
+    case 8: return launch_bwd<T, V, 8>(p, dw, s.grid, s.threads, st);
+    default: break;
+  }
+  if constexpr (V < 4) return launch_bwd<T, V, 16>(p, dw, s.grid, s.threads, st);
+  return -1;
+}
+template <class T>
+static int bwd_typed(const NormBwdParams& p, float* dw, const BwdShape& s, cudaStream_t st) {
+  constexpr int kFull = 16 / sizeof(T);
+  if (s.V == kFull) return bwd_vec<T, kFull>(p, dw, s, st);
+  if constexpr (sizeof(T) == 2) {
+    if (s.V == 2) return bwd_vec<T, 2>(p, dw, s, st);
+  }
+  return bwd_vec<T, 1>(p, dw, s, st);
+}
+
+static NormBwdParams bwd_params(const void* dy, const void* h, const void* w, const void* dh, void* dx,
+                                long long dy_stride, long long h_stride, long long dh_stride, long long rows, int D,
+                                int w_f32, float eps) {
+  NormBwdParams p;
+  p.dy = dy;
+  p.h = h;
+  p.w = w;
+  p.dh = dh;
+  p.dx = dx;
+  p.part = nullptr;
+  p.dy_stride = dy_stride;
+  p.h_stride = h_stride;
+  p.dh_stride = dh_stride;
+  p.rows = rows;
+  p.D = D;
+  p.w_f32 = w_f32;
+  p.eps = eps;
+  return p;
+}
+
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" {
+
+// mode 0: y in the type of x; 1: e4m3 with fp32 scales; 2: e4m3 with power-of-two scales and their packed words.
+// Strides in elements; y, h, scale and sf are dense.  sf: ceil(D / 512) x rows 32-bit words.
+int cb_rms_norm(const void* x, const void* res, const void* w, void* y, void* h, void* scale, void* sf,
+                long long x_stride, long long res_stride, long long rows, int D, int type, int w_f32, int mode,
+                float eps, void* stream) {
+  if (rows < 0 || rows > 0x7fffffffll || D < 1 || type < 0 || type > 2 || mode < 0 || mode > 2 ||
+      (mode != 0 && D % 128 != 0) || (res != nullptr && h == nullptr) || (mode != 0 && scale == nullptr)) {
+    set_last_error("rms_norm: bad shape or type (8 bits: D a multiple of 128)");
+    return -1;
+  }
+  if (rows == 0) return 0;
+  NormParams p;
+  p.x = x;
+  p.res = res;
+  p.w = w;
+  p.y = y;
+  p.h = h;
+  p.scale = static_cast<float*>(scale);
+  p.sf = static_cast<uint8_t*>(sf);
+  p.x_stride = x_stride;
+  p.res_stride = res_stride;
+  p.rows = rows;
+  p.D = D;
+  p.w_f32 = w_f32;
+  p.eps = eps;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (type * 3 + mode) {
+    case 0: return norm_typed<__nv_bfloat16, NORM_PLAIN>(p, st);
+    case 1: return norm_typed<__nv_bfloat16, NORM_SCALE>(p, st);
+    case 2: return norm_typed<__nv_bfloat16, NORM_POW2>(p, st);
+    case 3: return norm_typed<__half, NORM_PLAIN>(p, st);
+    case 4: return norm_typed<__half, NORM_SCALE>(p, st);
+    case 5: return norm_typed<__half, NORM_POW2>(p, st);
+    case 6: return norm_typed<float, NORM_PLAIN>(p, st);
+    case 7: return norm_typed<float, NORM_SCALE>(p, st);
+    default: return norm_typed<float, NORM_POW2>(p, st);
+  }
+}
+
+// Floats of workspace that cb_rms_norm_backward needs, or -1.  Pointers and strides as there.
+long long cb_rms_norm_backward_floats(const void* dy, const void* h, const void* w, const void* dh, const void* dx,
+                                      long long dy_stride, long long h_stride, long long dh_stride, long long rows,
+                                      int D, int type, int w_f32) {
+  if (rows < 1 || rows > 0x7fffffffll || D < 1 || type < 0 || type > 2) {
+    set_last_error("rms_norm_backward: bad shape or type");
+    return -1;
+  }
+  const NormBwdParams p = bwd_params(dy, h, w, dh, const_cast<void*>(dx), dy_stride, h_stride, dh_stride, rows, D,
+                                     w_f32, 0.f);
+  const BwdShape s = bwd_shape(p, type == 2 ? 4 : 2);
+  if (s.VPT == 0) {
+    set_last_error("rms_norm_backward: row too long");
+    return -1;
+  }
+  return static_cast<long long>(s.grid) * D;
+}
+
+int cb_rms_norm_backward(const void* dy, const void* h, const void* w, const void* dh, void* dx, void* dw, void* part,
+                         long long dy_stride, long long h_stride, long long dh_stride, long long rows, int D, int type,
+                         int w_f32, float eps, void* stream) {
+  if (cb_rms_norm_backward_floats(dy, h, w, dh, dx, dy_stride, h_stride, dh_stride, rows, D, type, w_f32) < 0)
+    return -1;
+  NormBwdParams p = bwd_params(dy, h, w, dh, dx, dy_stride, h_stride, dh_stride, rows, D, w_f32, eps);
+  p.part = static_cast<float*>(part);
+  const BwdShape s = bwd_shape(p, type == 2 ? 4 : 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* out = static_cast<float*>(dw);
+  if (type == ELEM_BF16) return bwd_typed<__nv_bfloat16>(p, out, s, st);
+  if (type == ELEM_F16) return bwd_typed<__half>(p, out, s, st);
+  return bwd_typed<float>(p, out, s, st);
+}
+
+}  // extern "C"

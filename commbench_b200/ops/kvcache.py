@@ -1,0 +1,175 @@
+"""A paged key/value cache held in 8 bits, and attention over it.
+
+Tokens live in pages of 16 to 128; a sequence is a row of page ids.  An element is an e4m3 number times a power of
+two that the keys (and the values) of a page and head share.  When a later token of the page is larger than the
+scale allows, the scale grows and the older tokens are multiplied by a power of two, which is exact but for the
+smallest numbers.
+
+    cache = KVCache8(num_pages, kv_heads)
+    q = cache.append(k, v, pages, start, rope=table, q=q)     # rotate, quantise, write: one launch
+    o, lse = cache.attend(q, pages, start)                    # attention of the same tokens over the cache
+
+``pages`` int32 [B, columns], ``start`` int32 [B] (tokens that were there before), ``count`` int32 [B] (how many of
+the S new tokens of a sequence exist; all by default) live on the device: no call waits for the GPU, and each can be
+captured in a graph.  Pages that several sequences share may be read, not written.
+
+A NaN in a token's key or value makes every query that sees the token answer NaN, and no other; infinities become
+the largest number of their block.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from .. import _native as N
+from ..runtime.context import CommError
+from ..utils.tracing import traced
+
+HEAD_DIM = 128
+_L9 = C.c_longlong * 9
+
+
+def _heads(t, name, heads=None, shape=None):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 4
+            and t.shape[3] == HEAD_DIM and t.stride(3) == 1 and t.data_ptr() % 8 == 0
+            and all(s % 4 == 0 for s in t.stride()[:3])):
+        raise CommError(f"{name} must be a bf16 CUDA tensor [B, S, H, 128], rows dense and 8-byte aligned")
+    if heads is not None and t.shape[2] != heads:
+        raise CommError(f"{name} must have {heads} heads")
+    if shape is not None and tuple(t.shape[:2]) != tuple(shape):
+        raise CommError(f"{name} must have {shape[0]} sequences of {shape[1]} tokens")
+
+
+class KVCache8:
+    """``num_pages`` pages of ``page`` tokens (16, 32, 64 or 128) for ``kv_heads`` heads of 128 elements."""
+
+    def __init__(self, num_pages: int, kv_heads: int, page: int = 64, device=None):
+        if page not in (16, 32, 64, 128):
+            raise CommError("a page has 16, 32, 64 or 128 tokens")
+        if num_pages < 1 or kv_heads < 1:
+            raise CommError("a cache has at least one page and one head")
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.num_pages, self.kv_heads, self.page, self.device = num_pages, kv_heads, page, dev
+        # The layout is the kernels' own (csrc/attn/kv_cache.cuh); `read` gives the values.  Zeros: a tile may
+        # hold rows that nobody has written, and what is multiplied by a probability of 0 has to be a number.
+        self.data = torch.zeros(num_pages * kv_heads * 2 * page * HEAD_DIM, dtype=torch.uint8, device=dev)
+        self.exps = torch.zeros(num_pages * kv_heads * 2, dtype=torch.int8, device=dev)
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() + self.exps.numel()
+
+    def _batch(self, pages, B, vectors):
+        if not (pages.is_cuda and pages.dtype == torch.int32 and pages.is_contiguous() and pages.dim() == 2
+                and pages.shape[0] == B and pages.shape[1] > 0 and pages.device == self.device_of()):
+            raise CommError("pages must be a contiguous int32 CUDA tensor [B, columns] on the cache's device")
+        for t, name in vectors:
+            if t is not None and not (t.is_cuda and t.dtype == torch.int32 and t.is_contiguous()
+                                      and tuple(t.shape) == (B,) and t.device == self.device_of()):
+                raise CommError(f"{name} must be a contiguous int32 CUDA tensor [B]")
+
+    def device_of(self):
+        return self.data.device
+
+    @traced("cb200.kv_append")
+    def append(self, k, v, pages, start, count=None, rope=None, q=None, status_ptr: int = 0, stream=None):
+        """Writes tokens ``start[b] .. start[b] + count[b] - 1``: ``k`` / ``v`` [B, S, kv_heads, 128] bf16 (any
+        strides with dense rows; the first ``count[b]`` tokens of each sequence).
+
+        ``rope`` (a :class:`ops.rope.RopeTable`) turns the keys by their positions before they are quantised, from
+        fp32.  ``q`` [B, S, Hq, 128] is turned by the same launch and returned (zeros for tokens that do not
+        exist).  Where a page id is out of range nothing is written; a position beyond the table gives NaN.  With
+        ``status_ptr`` either leaves a status word."""
+        _heads(k, "k", self.kv_heads)
+        _heads(v, "v", self.kv_heads, k.shape[:2])
+        B, S = k.shape[:2]
+        self._batch(pages, B, ((start, "start"), (count, "count")))
+        if k.device != self.device_of() or v.device != k.device:
+            raise CommError("k and v must be on the cache's device")
+        if q is not None:
+            _heads(q, "q", None, (B, S))
+            if rope is None:
+                raise CommError("q is turned with the keys: give the table too")
+        if rope is not None and (rope.rot > HEAD_DIM or rope.rot % 8 or rope.cos.device != k.device):
+            raise CommError("the cache turns a multiple of 8 elements of a head, with a table on its device")
+        out = None
+        if q is not None:
+            out = q.new_empty(q.shape) if stream is None else N.new_empty_on(stream, q, q.shape)
+        st = _L9(*k.stride()[:3], *v.stride()[:3], *(q.stride()[:3] if q is not None else (0, 0, 0)))
+        with torch.cuda.device(k.device):
+            rc = N.load().cb_kv_append(
+                self.data.data_ptr(), self.exps.data_ptr(), self.num_pages, self.kv_heads, self.page, k.data_ptr(),
+                v.data_ptr(), st, pages.data_ptr(), pages.shape[1], start.data_ptr(),
+                count.data_ptr() if count is not None else 0, B, S, q.data_ptr() if q is not None else 0,
+                out.data_ptr() if q is not None else 0, q.shape[2] if q is not None else 0,
+                rope.cos.data_ptr() if rope is not None else 0, rope.sin.data_ptr() if rope is not None else 0,
+                rope.positions if rope is not None else 0, rope.rot if rope is not None else 0,
+                int(rope.interleaved) if rope is not None else 0, status_ptr, N.raw_stream(stream))
+        if rc != 0:
+            raise CommError(f"key/value append failed: {N.last_error()}")
+        return out
+
+    @traced("cb200.kv_read")
+    def read(self, pages, begin, n: int, length=None, status_ptr: int = 0, stream=None):
+        """``(k, v)`` bf16 [B, n, kv_heads, 128]: tokens ``begin[b] .. begin[b] + n - 1`` (``begin`` None: from 0)
+        as the values that the cache holds; zeros before token 0 and from token ``length[b]`` on."""
+        if n < 0:
+            raise CommError("n must not be negative")
+        B = pages.shape[0]
+        self._batch(pages, B, ((begin, "begin"), (length, "length")))
+        shape = (B, n, self.kv_heads, HEAD_DIM)
+        k, v = (self.data.new_empty(shape, dtype=torch.bfloat16) if stream is None else
+                N.new_empty_on(stream, self.data, shape, torch.bfloat16) for _ in range(2))
+        with torch.cuda.device(self.device_of()):
+            rc = N.load().cb_kv_read(
+                self.data.data_ptr(), self.exps.data_ptr(), self.num_pages, self.kv_heads, self.page,
+                pages.data_ptr(), pages.shape[1], begin.data_ptr() if begin is not None else 0,
+                length.data_ptr() if length is not None else 0, B, n, k.data_ptr(), v.data_ptr(), status_ptr,
+                N.raw_stream(stream))
+        if rc != 0:
+            raise CommError(f"key/value read failed: {N.last_error()}")
+        return k, v
+
+    @traced("cb200.kv_attend")
+    def attend(self, q, pages, start, count=None, window: int = 0, sinks: int = 0, scale: float | None = None,
+               max_len: int | None = None, status_ptr: int = 0, stream=None):
+        """``(o [B, S, Hq, 128] bf16, lse [B, Hq, S] fp32)`` of queries at positions ``start[b] + i`` over the
+        sequence's tokens up to each query's own (they have been appended).
+
+        ``window`` > 0: a query at p sees the keys j > p - window, and the first ``sinks`` tokens of the sequence.
+        Rows that see no key, and the rows from ``count[b]`` on, are zeros with lse -inf.  ``max_len``: an upper
+        bound of ``start + count`` that the host knows (default: what the table has room for)."""
+        _heads(q, "q")
+        B, S, Hq, _ = q.shape
+        if Hq % self.kv_heads:
+            raise CommError("query heads must be a multiple of the key/value heads")
+        if window < 0 or sinks < 0:
+            raise CommError("window and sinks must not be negative")
+        self._batch(pages, B, ((start, "start"), (count, "count")))
+        if q.device != self.device_of():
+            raise CommError("q must be on the cache's device")
+        o = q.new_empty(q.shape) if stream is None else N.new_empty_on(stream, q, q.shape)
+        lse = q.new_empty((B, Hq, S), dtype=torch.float32) if stream is None else \
+            N.new_empty_on(stream, q, (B, Hq, S), torch.float32)
+        if B == 0 or S == 0:
+            return o, lse
+        room = pages.shape[1] * self.page
+        max_len = room if max_len is None else max(1, min(int(max_len), room))
+        sc = scale if scale is not None else 1.0 / math.sqrt(HEAD_DIM)
+        lib = N.load()
+        with torch.cuda.device(q.device):
+            n = lib.cb_kv_attend_bytes(B, S, Hq, self.kv_heads, max_len)
+            if n < 0:
+                raise CommError(f"key/value attention failed: {N.last_error()}")
+            ws = q.new_empty((n,), dtype=torch.uint8) if stream is None else \
+                N.new_empty_on(stream, q, (n,), torch.uint8, handed_out=False)
+            rc = lib.cb_kv_attend(
+                self.data.data_ptr(), self.exps.data_ptr(), self.num_pages, self.kv_heads, self.page, q.data_ptr(),
+                q.stride(0), q.stride(1), q.stride(2), o.data_ptr(), lse.data_ptr(), pages.data_ptr(),
+                pages.shape[1], start.data_ptr(), count.data_ptr() if count is not None else 0, B, S, Hq, window,
+                sinks, max_len, sc, ws.data_ptr(), n, status_ptr, N.raw_stream(stream))
+        if rc != 0:
+            raise CommError(f"key/value attention failed: {N.last_error()}")
+        return o, lse

@@ -1,0 +1,120 @@
+"""Rotary positions: pairs of a head's elements turned by an angle that grows with the token's position.
+
+    (a, b) -> (a cos - b sin, b cos + a sin),   angle = position * frequency of the pair
+
+Pairs are the elements ``(i, i + rot / 2)`` or, interleaved, ``(2 i, 2 i + 1)`` of the first ``rot`` elements of a
+head; the others are copied.  The table of cosines and sines is made in 64 bits and kept in fp32.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _native as N
+from ..utils.tracing import traced
+from .gemm import GemmError
+from .norm import _TYPES
+
+
+class RopeError(GemmError):
+    pass
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = None):
+    """(angle per position of each pair in fp64 [rot / 2], factor on the cosines and sines).
+
+    ``scaling``: ``{"kind": "linear", "factor": f}`` divides positions by f; ``{"kind": "ntk", "factor": f}``
+    stretches the base so that the lowest frequency is divided by f; ``{"kind": "yarn", "factor": f,
+    "original_positions": n}`` divides the frequencies that turn less than ``beta_slow`` times (1) in n positions,
+    keeps those that turn more than ``beta_fast`` times (32), blends in between, and multiplies by
+    ``0.1 ln f + 1`` (the published method of that name)."""
+    if rot < 2 or rot % 2:
+        raise RopeError("an even number of elements is turned")
+    i = torch.arange(0, rot, 2, dtype=torch.float64) / rot
+    if scaling is None:
+        return base ** -i, 1.0
+    kind, factor = scaling.get("kind"), float(scaling.get("factor", 1.0))
+    if factor <= 0:
+        raise RopeError("the scaling factor must be positive")
+    if kind == "linear":
+        return base ** -i / factor, 1.0
+    if kind == "ntk":
+        return (base * factor ** (rot / max(rot - 2, 1))) ** -i, 1.0
+    if kind == "yarn":
+        n = scaling["original_positions"]
+
+        def pair_of(turns):
+            return rot * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        lo = max(math.floor(pair_of(scaling.get("beta_fast", 32))), 0)
+        hi = min(math.ceil(pair_of(scaling.get("beta_slow", 1))), rot - 1)
+        slow = ((torch.arange(rot // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        f = base ** -i
+        mscale = scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+        return f * (1 - slow) + f / factor * slow, mscale
+    raise RopeError(f"unknown scaling {kind!r} (linear, ntk or yarn)")
+
+
+class RopeTable:
+    """Cosines and sines of positions ``0 .. positions - 1``, fp32 ``[positions, rot / 2]``, kept by the program."""
+
+    def __init__(self, rot: int, positions: int, base: float = 10000.0, interleaved: bool = False,
+                 scaling: dict | None = None, device=None):
+        if positions < 1:
+            raise RopeError("a table has at least one position")
+        f, m = rope_frequencies(rot, base, scaling)
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        angle = torch.arange(positions, dtype=torch.float64, device=dev)[:, None] * f.to(dev)
+        self.rot, self.positions, self.interleaved = rot, positions, bool(interleaved)
+        self.cos, self.sin = (torch.cos(angle) * m).float(), (torch.sin(angle) * m).float()
+
+
+@traced("cb200.rope")
+def rope(x, positions, table: RopeTable, inverse: bool = False, out=None, status_ptr: int = 0, stream=None):
+    """``x`` [B, S, H, D] (bf16, fp16 or fp32; any strides with dense heads' elements), or a pair of them - queries
+    and keys - in one launch; returns dense tensors of the same shapes.  ``positions`` int32 or int64 [B, S] or
+    [S].  ``inverse`` turns back, which is also the gradient: ``dx = rope(dy, positions, table, inverse=True)``.
+    ``out``: where to write (contiguous; may be a contiguous ``x`` itself).
+
+    A position outside the table gives NaN and, with ``status_ptr``, a status word."""
+    pair = isinstance(x, (tuple, list))
+    xs = list(x) if pair else [x]
+    if not 1 <= len(xs) <= 2:
+        raise RopeError("one tensor or a pair")
+    first = xs[0]
+    for t in xs:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 and t.dtype in _TYPES
+                and (t.stride(3) == 1 or t.shape[3] == 1) and t.shape[2] > 0 and t.dtype == first.dtype
+                and t.shape[:2] == first.shape[:2] and t.shape[3] == first.shape[3] and t.device == first.device):
+            raise RopeError("x must be CUDA [B, S, H, D] tensors of one type, batch, length and head size, "
+                            "elements of a head dense")
+    B, S, _, D = first.shape
+    if table.rot > D:
+        raise RopeError(f"the table turns {table.rot} elements, a head has {D}")
+    if not (positions.is_cuda and positions.is_contiguous() and positions.dtype in (torch.int32, torch.int64)
+            and tuple(positions.shape) in ((B, S), (S,))):
+        raise RopeError("positions must be a contiguous int32 or int64 CUDA tensor [B, S] or [S]")
+    if table.cos.device != first.device or positions.device != first.device:
+        raise RopeError("table, positions and x must be on one device")
+    if out is None:
+        outs = [t.new_empty(t.shape) if stream is None else N.new_empty_on(stream, t, t.shape) for t in xs]
+    else:
+        outs = list(out) if pair else [out]
+        for t, o in zip(xs, outs, strict=True):
+            if not (o.is_cuda and o.is_contiguous() and o.shape == t.shape and o.dtype == t.dtype
+                    and o.device == t.device):
+                raise RopeError("out must be contiguous and have x's shape, type and device")
+    args = []
+    for t, o in zip(xs, outs):
+        args += [t.data_ptr(), o.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2]]
+    if len(xs) == 1:
+        args += [0, 0, 0, 0, 0, 0]
+    with torch.cuda.device(first.device):
+        rc = N.load().cb_rope(*args, B, S, D, table.cos.data_ptr(), table.sin.data_ptr(), table.positions, table.rot,
+                              int(table.interleaved), positions.data_ptr(), int(positions.dtype == torch.int64),
+                              int(positions.dim() == 2), int(inverse), _TYPES[first.dtype], status_ptr,
+                              N.raw_stream(stream))
+    if rc != 0:
+        raise RopeError(f"rope failed: {N.last_error()}")
+    return tuple(outs) if pair else outs[0]

@@ -1,0 +1,331 @@
+"""Root-mean-square norm, its 8-bit form and gradient, and rotary positions, against the formulas in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+# Half a unit in the last place of a result, relative, plus fp32 sums of a row (tree of at most 2^4 terms a thread,
+# 2^10 threads: 14 roundings of 2^-24, and the square root, division and three products).
+ULP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+SUMS = 2.0 ** -19
+
+
+def _randn(*shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def _close(got, want, dtype, extra=0.0):
+    # fp16 has its smallest step at 2^-24
+    tol = (ULP[dtype] + SUMS) * want.abs() + 2.0 ** -25 + extra
+    bad = (got.double() - want).abs() > tol
+    assert not bad.any(), ((got.double() - want).abs() / tol).max()
+
+
+def _norm64(x, w, res, eps):
+    h = x.double() + (res.double() if res is not None else 0)
+    return h, h / torch.sqrt(h.square().mean(dim=1, keepdim=True) + eps) * w.double()
+
+
+SHAPES = [(1, 1), (1, 8), (3, 7), (2, 64), (5, 100), (300, 255), (17, 1024), (4, 1031), (400, 1032), (1, 8192),
+          (333, 8192), (2, 8190), (310, 8191), (2, 12288), (2, 32768), (1000, 256)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,d", SHAPES)
+def test_rms_norm(native_lib, rows, d, dtype):
+    from commbench_b200.ops.norm import rms_norm
+
+    if dtype == torch.float32 and d > 16384:
+        d = 16384
+    x, res = _randn(rows, d, dtype=dtype, seed=1), _randn(rows, d, dtype=dtype, seed=2, scale=3.0)
+    for wt in {dtype, torch.float32}:
+        w = _randn(d, dtype=wt, seed=3)
+        y = rms_norm(x, w, eps=1e-5)
+        assert y.dtype == dtype
+        _close(y, _norm64(x, w, None, 1e-5)[1], dtype)
+        y, h = rms_norm(x, w, residual=res, eps=1e-5)
+        h64, y64 = _norm64(x, w, res, 1e-5)
+        _close(h, h64, dtype)
+        # h in fp32 is the sum rounded once
+        _close(y, y64, dtype, extra=2.0 ** -23 * (x.double().abs() + res.double().abs()).max())
+
+
+@pytest.mark.parametrize("offset,pad", [(0, 8), (8, 24), (1, 3), (2, 6)])
+def test_rms_norm_of_rows_that_lie_apart(native_lib, offset, pad):
+    from commbench_b200.ops.norm import rms_norm, rms_norm_backward
+
+    wide = _randn(37, 512 + offset + pad, dtype=torch.bfloat16, seed=4)
+    x, w = wide[:, offset:offset + 512], _randn(512, dtype=torch.bfloat16, seed=5)
+    y, h = rms_norm(x, w, residual=x)
+    y2, h2 = rms_norm(x.contiguous(), w, residual=x.contiguous())
+    assert torch.equal(h, h2)
+    _close(y, _norm64(x, w, x, 1e-6)[1], torch.bfloat16)
+    dx, dw = rms_norm_backward(x, x, w, dh=x)
+    rx, rw = _backward64(x, x, w, x, 1e-6)
+    _close_grad(dx, dw, rx, rw, x, x, w, x)
+
+
+@pytest.mark.parametrize("value", [0.0, 1e-30, 3e4])
+def test_rms_norm_of_constant_rows(native_lib, value):
+    from commbench_b200.ops.norm import rms_norm, rms_norm_quant
+
+    x = torch.full((3, 256), value, dtype=torch.bfloat16, device="cuda")
+    w = torch.ones(256, dtype=torch.bfloat16, device="cuda")
+    _close(rms_norm(x, w), _norm64(x, w, None, 1e-6)[1], torch.bfloat16)
+    q, s, h = rms_norm_quant(x, w)
+    assert h is None and torch.isfinite(s).all() and torch.isfinite(q.float()).all()
+
+
+def test_rms_norm_keeps_nan_to_its_row(native_lib):
+    from commbench_b200.ops.norm import rms_norm
+
+    x = _randn(9, 512, dtype=torch.bfloat16, seed=6)
+    x[4, 100] = float("nan")
+    w = torch.ones(512, dtype=torch.bfloat16, device="cuda")
+    y = rms_norm(x, w)
+    assert torch.isnan(y[4]).all() and torch.isfinite(y[:4]).all() and torch.isfinite(y[5:]).all()
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,d", [(1, 128), (3, 640), (130, 1024), (7, 8192), (400, 3968)])
+def test_rms_norm_quant(native_lib, rows, d, dtype, residual, pow2):
+    from commbench_b200.ops.gemm import sf_exponents
+    from commbench_b200.ops.norm import rms_norm_quant
+
+    x = _randn(rows, d, dtype=dtype, seed=7)
+    res = _randn(rows, d, dtype=dtype, seed=8) if residual else None
+    w = _randn(d, dtype=dtype, seed=9)
+    x[0, :128] = 0
+    if residual:
+        res[0, :128] = 0
+    out = rms_norm_quant(x, w, residual=res, pow2=pow2)
+    q, s, h = out[0], out[1], out[-1]
+    h64, y64 = _norm64(x, w, res, 1e-6)
+    b = y64.view(rows, -1, 128)
+    amax = b.abs().amax(dim=2)
+    want = torch.where(amax > 0, amax / 448.0, torch.ones_like(amax))
+    if pow2:
+        # a power of two, between the exact scale and twice that
+        m, _ = torch.frexp(s)
+        assert (m == 0.5).all()
+        assert ((s.double() >= want * (1 - SUMS)) & (s.double() < 2 * want * (1 + SUMS))).all()
+        assert torch.equal(torch.exp2(sf_exponents(out[2], d // 128).float() - 127), s)
+        fill = out[2].view(torch.uint8).view(-1, rows, 4).permute(1, 0, 2).reshape(rows, -1)[:, d // 128:]
+        assert (fill == 127).all()
+    else:
+        assert ((s.double() - want).abs() <= SUMS * want).all()
+    # e4m3 rounds to 4 significant bits, with steps of 2^-9 below 2^-6
+    err = (q.double().view(rows, -1, 128) * s.double()[:, :, None] - b).abs()
+    assert (err <= (2.0 ** -4 + SUMS) * b.abs() + 2.0 ** -10 * s.double()[:, :, None] * (1 + SUMS)).all()
+    if residual:
+        _close(h, h64, dtype)
+
+
+def test_rms_norm_quant_feeds_the_scaled_products(native_lib):
+    from commbench_b200.ops.gemm import gemm_fp8_blockscaled, gemm_fp8_mx, quantize_blockscaled
+    from commbench_b200.ops.norm import rms_norm_quant
+    from commbench_b200.ops.tp_fp8 import MxWeight
+
+    x, w = _randn(70, 1024, dtype=torch.bfloat16, seed=10), torch.ones(1024, dtype=torch.bfloat16, device="cuda")
+    wt = _randn(256, 1024, dtype=torch.bfloat16, seed=11, scale=0.05)
+    ref = _norm64(x, w, None, 1e-6)[1] @ wt.double().t()
+    q, s, sf, _ = rms_norm_quant(x, w, pow2=True)
+    mx = MxWeight.from_bf16(wt)
+    a = gemm_fp8_mx(q, sf, mx.q, mx.sf)
+    q, s, _ = rms_norm_quant(x, w)
+    b = gemm_fp8_blockscaled(q, s, *quantize_blockscaled(wt, 128))
+    for y in (a, b):   # two operands of e4m3: 2^-4 / sqrt(3) each at most, in the 2-norm
+        assert (y.double() - ref).norm() / ref.norm() < 2 * 2.0 ** -4 / math.sqrt(3)
+
+
+def _backward64(dy, h, w, dh, eps):
+    h, dy = h.double(), dy.double()
+    rstd = 1 / torch.sqrt(h.square().mean(dim=1, keepdim=True) + eps)
+    g = dy * w.double()
+    dx = rstd * g - h * rstd ** 3 * (g * h).mean(dim=1, keepdim=True)
+    return dx + (dh.double() if dh is not None else 0), (dy * h * rstd).sum(dim=0)
+
+
+def _close_grad(dx, dw, rx, rw, dy, h, w, dh):
+    # dx is a difference of two terms, each of which carries the relative error of a row's sums
+    eps = 1e-6
+    h6, g = h.double(), dy.double() * w.double()
+    rstd = 1 / torch.sqrt(h6.square().mean(dim=1, keepdim=True) + eps)
+    size = rstd * g.abs() + h6.abs() * rstd ** 3 * (g * h6).abs().mean(dim=1, keepdim=True)
+    if dh is not None:
+        size = size + dh.double().abs()
+    tol = ULP[dx.dtype] * rx.abs() + SUMS * size + 2.0 ** -25
+    assert ((dx.double() - rx).abs() <= tol).all(), ((dx.double() - rx).abs() / tol).max()
+    # up to 2^12 rows: at most 2^12 / 148 + 32 + 5 additions one after the other, and SUMS for each term
+    mag = (dy.double() * h6 * rstd).abs().sum(dim=0)
+    assert ((dw.double() - rw).abs() <= (SUMS + 128 * 2.0 ** -24) * mag + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,d", [(1, 1), (3, 7), (1, 64), (200, 100), (1500, 256), (700, 1032), (333, 8192),
+                                    (20, 8190), (20, 8191), (3, 12288), (2, 32768)])
+def test_rms_norm_backward(native_lib, rows, d, dtype):
+    from commbench_b200.ops.norm import rms_norm_backward
+
+    if dtype == torch.float32 and d > 16384:
+        d = 16384
+    h, dy = _randn(rows, d, dtype=dtype, seed=12, scale=2.0), _randn(rows, d, dtype=dtype, seed=13)
+    dh = _randn(rows, d, dtype=dtype, seed=14)
+    for wt in {dtype, torch.float32}:
+        w = _randn(d, dtype=wt, seed=15)
+        for extra in (None, dh):
+            dx, dw = rms_norm_backward(dy, h, w, dh=extra)
+            assert dw.dtype == torch.float32
+            rx, rw = _backward64(dy, h, w, extra, 1e-6)
+            _close_grad(dx, dw, rx, rw, dy, h, w, extra)
+            dx2, dw2 = rms_norm_backward(dy, h, w, dh=extra)
+            assert torch.equal(dx, dx2) and torch.equal(dw, dw2)
+
+
+def test_rms_norm_backward_is_the_forward_s_difference(native_lib):
+    """Along a direction, the change of the loss <y, dy> over a step 2 t: fp32, t = 2^-6, error t^2 and 2^-24 / t."""
+    from commbench_b200.ops.norm import rms_norm, rms_norm_backward
+
+    x, dy = _randn(5, 96, dtype=torch.float32, seed=16), _randn(5, 96, dtype=torch.float32, seed=17)
+    w, t = _randn(96, dtype=torch.float32, seed=18), 2.0 ** -6
+    dx, dw = rms_norm_backward(dy, x, w)
+    v, u = _randn(5, 96, dtype=torch.float32, seed=19), _randn(96, dtype=torch.float32, seed=20)
+    loss = lambda a, b: (rms_norm(a, b).double() * dy.double()).sum()
+    by_x = (loss(x + t * v, w) - loss(x - t * v, w)) / (2 * t)
+    by_w = (loss(x, w + t * u) - loss(x, w - t * u)) / (2 * t)
+    scale = dy.double().norm() * w.double().abs().max()
+    assert abs(by_x - (dx.double() * v.double()).sum()) < 8 * t * t * scale * v.double().norm()
+    assert abs(by_w - (dw.double() * u.double()).sum()) < 2.0 ** -12 * dy.double().norm() * u.double().norm()
+
+
+def test_norm_empty_and_refusals(native_lib):
+    from commbench_b200.ops.norm import NormError, rms_norm, rms_norm_backward, rms_norm_quant
+
+    x, w = _randn(4, 256, dtype=torch.bfloat16, seed=1), torch.ones(256, dtype=torch.bfloat16, device="cuda")
+    assert rms_norm(x[:0], w).shape == (0, 256)
+    dx, dw = rms_norm_backward(x[:0], x[:0], w)
+    assert dx.shape == (0, 256) and (dw == 0).all()
+    for bad in (lambda: rms_norm(x.cpu(), w), lambda: rms_norm(x[0], w), lambda: rms_norm(x.double(), w),
+                lambda: rms_norm(x.t(), w), lambda: rms_norm(x, w[:128]), lambda: rms_norm(x, w.half()),
+                lambda: rms_norm(x, w, residual=x.half()), lambda: rms_norm(x, w, residual=x[:3]),
+                lambda: rms_norm_quant(x[:, :200], w[:200]), lambda: rms_norm_backward(x[:3], x, w),
+                lambda: rms_norm_backward(x, x, w, dh=x.float()),
+                lambda: rms_norm(torch.zeros(1, 40001, device="cuda"), torch.zeros(40001, device="cuda"))):
+        with pytest.raises(NormError):
+            bad()
+
+
+def test_norm_on_another_stream(native_lib):
+    from commbench_b200.ops.norm import rms_norm, rms_norm_backward
+
+    x, w = _randn(64, 4096, dtype=torch.bfloat16, seed=21), torch.ones(4096, dtype=torch.bfloat16, device="cuda")
+    want, (gx, gw) = rms_norm(x, w), rms_norm_backward(x, x, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    got = rms_norm(x, w, stream=s)
+    dx, dw = rms_norm_backward(x, x, w, stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want) and torch.equal(dx, gx) and torch.equal(dw, gw)
+
+
+# ------------------------------------------------------------------------------------------ rotary positions
+def _rope64(x, pos, rot, base, interleaved, inverse, freq=None, factor=1.0):
+    f = base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=x.device) / rot) if freq is None else freq
+    a = pos.double()[..., None, None] * f
+    c, s = torch.cos(a) * factor, torch.sin(a) * factor * (-1 if inverse else 1)
+    y = x.double().clone()
+    one, two = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot))
+    u, v = x.double()[..., one], x.double()[..., two]
+    y[..., one], y[..., two] = u * c - v * s, v * c + u * s
+    return y
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot", [(128, 128), (128, 64), (64, 64), (192, 96), (128, 2), (80, 50), (2, 2), (37, 14),
+                                     (640, 640)])
+def test_rope(native_lib, dim, rot, interleaved, dtype):
+    from commbench_b200.ops.rope import RopeTable, rope
+
+    table = RopeTable(rot, 5000, base=500.0, interleaved=interleaved)
+    qk = _randn(2, 11, 7, dim, dtype=dtype, seed=30)
+    q, k = qk[:, :, :5], qk[:, :, 5:]
+    pos = torch.randint(0, 5000, (2, 11), device="cuda", generator=torch.Generator(device="cuda").manual_seed(31))
+    for p in (pos, pos.int(), pos[0], pos[0].int()):
+        for inverse in (False, True):
+            for x, y in zip((q, k), rope((q, k), p, table, inverse=inverse)):
+                want = _rope64(x, p, rot, 500.0, interleaved, inverse)
+                # two products and a sum in fp32, table entries of half a unit
+                _close(y, want, dtype, extra=2.0 ** -22 * x.double().abs().amax())
+                assert torch.equal(y[..., rot:], x[..., rot:])
+
+
+@pytest.mark.parametrize("tokens", [1, 5000])
+def test_rope_in_place_and_many_tokens(native_lib, tokens):
+    from commbench_b200.ops.rope import RopeTable, rope
+
+    x, pos = _randn(1, tokens, 3, 128, dtype=torch.bfloat16, seed=32), torch.arange(tokens, device="cuda")
+    for il in (False, True):
+        table = RopeTable(128, tokens, interleaved=il)
+        want = rope(x, pos, table)
+        y = x.clone()
+        assert rope(y, pos, table, out=y) is y and torch.equal(y, want)
+        _close(want, _rope64(x, pos, 128, 10000.0, il, False), torch.bfloat16, extra=2.0 ** -20)
+
+
+def test_rope_gradient_is_the_transpose(native_lib):
+    """<rope(x), dy> = <x, rope(dy, inverse)> in fp32, scaled tables too; and it is linear, so the difference
+    quotient along any direction is the operator itself."""
+    from commbench_b200.ops.rope import RopeTable, rope
+
+    x, dy = _randn(2, 9, 4, 128, dtype=torch.float32, seed=33), _randn(2, 9, 4, 128, dtype=torch.float32, seed=34)
+    pos = torch.arange(9, device="cuda") + 3000
+    for scaling in (None, dict(kind="linear", factor=3.0), dict(kind="ntk", factor=8.0),
+                    dict(kind="yarn", factor=4.0, original_positions=2048)):
+        for il in (False, True):
+            t = RopeTable(96, 4096, interleaved=il, scaling=scaling)
+            a = (rope(x, pos, t).double() * dy.double()).sum()
+            b = (x.double() * rope(dy, pos, t, inverse=True).double()).sum()
+            assert abs(a - b) < 2.0 ** -20 * x.double().norm() * dy.double().norm()
+            d = (rope(x + dy, pos, t).double() - rope(x - dy, pos, t).double()) / 2
+            assert (d - rope(dy, pos, t).double()).abs().max() < 2.0 ** -18
+
+
+def test_rope_scaling_and_far_positions(native_lib):
+    from commbench_b200.ops.rope import RopeTable, rope, rope_frequencies
+
+    f, m = rope_frequencies(128, 10000.0, dict(kind="yarn", factor=4.0, original_positions=4096))
+    plain, _ = rope_frequencies(128)
+    assert f[0] == plain[0] and abs(f[-1] - plain[-1] / 4) < 1e-18 and abs(m - (0.1 * math.log(4) + 1)) < 1e-15
+    ntk, _ = rope_frequencies(128, scaling=dict(kind="ntk", factor=4.0))
+    assert ntk[0] == 1.0 and abs(ntk[-1] * 4 / plain[-1] - 1) < 1e-12
+    t = RopeTable(128, 1 << 20, scaling=dict(kind="yarn", factor=4.0, original_positions=4096))
+    x = _randn(1, 4, 2, 128, dtype=torch.float32, seed=35)
+    pos = torch.tensor([0, 4095, 1000003, (1 << 20) - 1], device="cuda")
+    y = rope(x, pos, t)
+    want = _rope64(x, pos, 128, None, False, False, freq=f.cuda(), factor=m)
+    assert (y.double() - want).abs().max() < 2.0 ** -20
+
+
+def test_rope_refusals_and_positions_outside_the_table(native_lib):
+    from commbench_b200.ops.rope import RopeError, RopeTable, rope, rope_frequencies
+
+    t = RopeTable(64, 100)
+    x, pos = _randn(1, 3, 2, 128, dtype=torch.bfloat16, seed=36), torch.tensor([99, 100, -1], device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = rope(x, pos, t, status_ptr=status.data_ptr())
+    assert torch.isfinite(y[:, 0]).all() and torch.isnan(y[:, 1:, :, :64]).all()
+    assert torch.equal(y[..., 64:], x[..., 64:]) and (status.item() >> 24) == 5
+    assert rope(x[:, :0], pos[:0], t).shape == (1, 0, 2, 128)
+    for bad in (lambda: rope(x[0], pos, t), lambda: rope(x.double(), pos, t), lambda: rope(x, pos[:2], t),
+                lambda: rope(x, pos.float(), t), lambda: rope(x[..., :32], pos, t), lambda: rope(x.cpu(), pos, t),
+                lambda: rope((x, x.float()), pos, t), lambda: rope(x, pos, t, out=x[:, :, :1]),
+                lambda: rope_frequencies(7), lambda: rope_frequencies(8, scaling=dict(kind="other")),
+                lambda: RopeTable(64, 0), lambda: rope(x.transpose(2, 3), pos, t)):
+        with pytest.raises(RopeError):
+            bad()
