@@ -241,6 +241,33 @@ struct CpBlockIter {
   }
 };
 
+// The key blocks of a query tile pair over the keys of a cached sequence: those of the first tokens that stay
+// visible, then those from the first that the pair's first query sees to the last.  `i` is the block.
+struct CpCacheIter {
+  int i, sink_blocks, first;
+  __device__ __forceinline__ void start(const FaCpParams& p, int q_first) {
+    const int low = p.window > 0 ? q_first - p.window + 1 : 0;
+    first = low > 0 ? low / CP_BN : 0;
+    sink_blocks = p.window > 0 ? (p.sinks + CP_BN - 1) / CP_BN : 0;
+    if (sink_blocks > first) sink_blocks = first;
+    i = sink_blocks > 0 ? 0 : first;
+  }
+  __device__ __forceinline__ void next() {
+    if (++i == sink_blocks) i = first;
+  }
+  __device__ __forceinline__ int total(const FaCpParams& p, int q_last) const {
+    const int last = min(q_last, p.seg[0].nkeys - 1);
+    return last < 0 ? 0 : max(0, sink_blocks + last / CP_BN - first + 1);
+  }
+};
+
+// Hides the scores from->to-1 of the window's lower edge.
+__device__ __forceinline__ void cp_mask_range(uint32_t (&s)[128], int from, int to) {
+  const uint32_t n = to > from ? static_cast<uint32_t>(to - from) : 0u;
+#pragma unroll
+  for (int i = 0; i < 128; ++i) s[i] = static_cast<uint32_t>(i - from) < n ? 0xff800000u : s[i];
+}
+
 // Communication CTA `c` of `p.num_comm`: its share of every piece, in list order.
 __device__ __forceinline__ void cp_comm_cta(const FaCpParams& p, int c) {
   const int T = blockDim.x;
@@ -301,10 +328,12 @@ __device__ __forceinline__ void cp_reg_inc() {
 
 // One attention item: a pair of query tiles of one head and batch.  Pairs run from the end of a query
 // segment to its start (under a causal mask the late rows are the long items).
+template <bool kCache>
 struct CpItem {
   int qs_i, pair, head, batch;
   int q_first, q_last;   // positions of the pair's first row and last valid row
   int nblk;              // key blocks it visits
+  int rows_there;        // kCache: rows of the sequence that exist
   __device__ __forceinline__ bool decode(const FaCpParams& p, int item) {
     const int per_pair = p.heads * p.B;
     int gp = item / per_pair;
@@ -315,6 +344,19 @@ struct CpItem {
       const int np = (p.qseg[qs_i].nrows + 2 * CP_BM - 1) / (2 * CP_BM);
       if (gp < np) {
         pair = np - 1 - gp;
+        if constexpr (kCache) {
+          // The kernel in front waits before it releases this one, so this may be read before pdl_wait().
+          const int start = p.seq_start[batch];
+          rows_there = p.seq_count == nullptr ? p.qseg[0].nrows : min(max(p.seq_count[batch], 0), p.qseg[0].nrows);
+          if (start < 0) rows_there = 0;
+          q_first = start + pair * 2 * CP_BM;
+          const int rows = min(rows_there - pair * 2 * CP_BM, 2 * CP_BM);
+          q_last = q_first + rows - 1;
+          CpCacheIter it;
+          it.start(p, q_first);
+          nblk = rows > 0 ? it.total(p, q_last) : 0;
+          return true;
+        }
         q_first = p.qseg[qs_i].qpos0 + pair * 2 * CP_BM;
         int rows = p.qseg[qs_i].nrows - pair * 2 * CP_BM;
         if (rows > 2 * CP_BM) rows = 2 * CP_BM;
@@ -333,8 +375,9 @@ struct CpItem {
 // the producer asks for one when it has issued all loads of the item before, and every role reads the
 // answer and says so.  Asking earlier would hand the short items at the end of the list to whoever started
 // first, not to whoever is free first: 2 x 3272 tokens, 8 / 2 heads, 208 items took 77 us so, 60 now.
+template <bool kCache>
 struct CpWalk {
-  CpItem item;
+  CpItem<kCache> item;
   int n = 0;   // items taken
   // For a warp other than the producer's, all lanes converged: the next item, or false at the end (or on
   // an abort).
@@ -365,7 +408,9 @@ struct CpWalk {
 static constexpr int CP_ITEM_READERS = 9;
 
 // kPoly: every kPoly-th pair of keys takes its exponential from the FMA pipe (0: none).
-template <int kPoly>
+// kCache: the sequences of a cache, each with its own positions and length, causal, with a window; one segment of
+// keys and one of queries, no tickets.
+template <int kPoly, bool kCache = false>
 __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_constant__ FaCpParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
@@ -384,7 +429,7 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
     __syncthreads();
     ticket = ctl.ticket;
   }
-  CpItem first;
+  CpItem<kCache> first;
   if (ticket < p.num_comm) {
     cp_comm_cta(p, ticket);
   } else if (first.decode(p, ticket - p.num_comm)) {
@@ -432,8 +477,8 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
     if (warp == 0) {
       if (lane == 0) {
         // ---------------------------------------------------------------- producer
-        CpWalk walk;
-        const CpItem& w = walk.item;
+        CpWalk<kCache> walk;
+        const CpItem<kCache>& w = walk.item;
         bool ok = true;
         int g0 = 0, nq = 0;   // blocks and items before this item
         while (ok && walk.request(p, ctl, ticket)) {
@@ -452,8 +497,14 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
                         &ctl.q_full);
           }
           CpBlockIter ik, iv;
-          ik.start(p, w.q_last);
-          iv.start(p, w.q_last);
+          CpCacheIter ck, cv;
+          if constexpr (kCache) {
+            ck.start(p, w.q_first);
+            cv = ck;
+          } else {
+            ik.start(p, w.q_last);
+            iv.start(p, w.q_last);
+          }
           int jk = 0, jv = 0, ready_seg = -1;
           uint32_t idle = 0;
           uint64_t t0 = 0;
@@ -464,7 +515,7 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
               if (use == 0 || mbar_try_wait(&ctl.k_empty[s], (use - 1) & 1)) {
                 // First block of a segment that is still being pulled: wait for its counter.
                 // K and V of a segment arrive under the same counter.
-                if (ik.seg != ready_seg) {
+                if (!kCache && ik.seg != ready_seg) {
                   const CpSeg& g = p.seg[ik.seg];
                   if (g.flag >= 0) {
                     if (!wait_flag_ge_gpu(p.flags + g.flag, p.flag_target, p.timeout_ns, p.status,
@@ -477,24 +528,26 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
                   }
                   ready_seg = ik.seg;
                 }
-                const int krow = w.batch * p.kv_bstride + p.seg[ik.seg].row0 + ik.i * CP_BN;
+                const int krow = kCache ? w.batch * p.kv_bstride + ck.i * CP_BN
+                                        : w.batch * p.kv_bstride + p.seg[ik.seg].row0 + ik.i * CP_BN;
                 mbar_arrive_expect_tx(&ctl.k_full[s], CP_TILE);
                 tma_load_3d(sK + s * CP_TILE, &p.tm_k, 0, kv_head, krow, &ctl.k_full[s]);
                 tma_load_3d(sK + s * CP_TILE + CP_SUB, &p.tm_k, 64, kv_head, krow, &ctl.k_full[s]);
                 ++jk;
-                ik.next(p, w.q_last);
+                if constexpr (kCache) ck.next(); else ik.next(p, w.q_last);
                 progress = true;
               }
             }
             if (jv < w.nblk && jv < jk) {
               const int s = (g0 + jv) % CP_VST, use = (g0 + jv) / CP_VST;
               if (use == 0 || mbar_try_wait(&ctl.v_empty[s], (use - 1) & 1)) {
-                const int vrow = w.batch * p.kv_bstride + p.seg[iv.seg].row0 + iv.i * CP_BN;
+                const int vrow = kCache ? w.batch * p.kv_bstride + cv.i * CP_BN
+                                        : w.batch * p.kv_bstride + p.seg[iv.seg].row0 + iv.i * CP_BN;
                 mbar_arrive_expect_tx(&ctl.v_full[s], CP_TILE);
                 tma_load_3d(sV + s * CP_TILE, &p.tm_v, 0, kv_head, vrow, &ctl.v_full[s]);
                 tma_load_3d(sV + s * CP_TILE + CP_SUB, &p.tm_v, 64, kv_head, vrow, &ctl.v_full[s]);
                 ++jv;
-                iv.next(p, w.q_last);
+                if constexpr (kCache) cv.next(); else iv.next(p, w.q_last);
                 progress = true;
               }
             }
@@ -584,7 +637,7 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
           __syncwarp();
           return true;
         };
-        CpWalk walk;
+        CpWalk<kCache> walk;
         while (ok && walk.next(p, ctl, ticket)) {
           const int nblk = __shfl_sync(0xffffffffu, walk.item.nblk, 0);
           if (nblk == 0) continue;
@@ -622,8 +675,8 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
       const uint32_t lane_addr = (q * 32u) << 16;
       const uint32_t tS = tmem + 256u * t + lane_addr;
       const uint32_t tO = tS + 128u;
-      CpWalk walk;
-      const CpItem& w = walk.item;
+      CpWalk<kCache> walk;
+      const CpItem<kCache>& w = walk.item;
       bool ok = true;
       int g0 = 0;   // blocks before this item
       while (ok && walk.next(p, ctl, ticket)) {
@@ -633,38 +686,44 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
         const int q_pos = tile_first + static_cast<int>(r);
         float m_ref = -INFINITY, l = 0.f;
         CpBlockIter it;
-        it.start(p, w.q_last);
+        CpCacheIter ci;
+        if constexpr (kCache) ci.start(p, w.q_first); else it.start(p, w.q_last);
         for (int j = 0; ok && j < w.nblk; ++j) {
           if (!mbar_wait(&ctl.s_full[t], (g0 + j) & 1, &ctl.abort_flag, p.status, 0xE30 + t)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const CpSeg& g = p.seg[it.seg];
-          const int key0 = g.kpos0 + it.i * CP_BN;
-          const int kv_left = g.nkeys - it.i * CP_BN;
-          const bool need_mask = kv_left < CP_BN || (p.causal && key0 + CP_BN - 1 > tile_first);
-          it.next(p, w.q_last);
+          const CpSeg& g = p.seg[kCache ? 0 : it.seg];
+          const int key0 = kCache ? ci.i * CP_BN : g.kpos0 + it.i * CP_BN;
+          const int kv_left = g.nkeys - (kCache ? key0 : it.i * CP_BN);
+          const bool need_mask = kv_left < CP_BN || ((kCache || p.causal) && key0 + CP_BN - 1 > tile_first);
+          if constexpr (kCache) ci.next(); else it.next(p, w.q_last);
           uint32_t s[128];
           tmem_ld_32x32_at(tS, &s[0]);
           tmem_ld_32x32_at(tS + 32u, &s[32]);
           tmem_ld_32x32_at(tS + 64u, &s[64]);
           tmem_ld_32x32_at(tS + 96u, &s[96]);
           tmem_wait_ld();
-          if (need_mask) cp_mask_tail(s, p.causal ? min(kv_left, q_pos - key0 + 1) : kv_left);
+          if (need_mask) cp_mask_tail(s, kCache || p.causal ? min(kv_left, q_pos - key0 + 1) : kv_left);
+          bool edge = false;   // the window's lower edge may lie in this block
+          if constexpr (kCache) {
+            edge = p.window > 0 && key0 <= tile_first + CP_BM - 1 - p.window && key0 + CP_BN > p.sinks;
+            if (edge) cp_mask_range(s, max(p.sinks - key0, 0), min(q_pos - p.window + 1 - key0, CP_BN));
+          }
           float mx8[8];
           cp_row_max(s, mx8);
           cp_update_max(mx8, tO, p.scale_log2, j > 0, true, m_ref, l);
           // P_t(j): row r = lane r, keys 2c and 2c+1 in column c.  The product with the first 64 keys runs
           // while the others' exponentials are taken.
           uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull};
-          cp_probabilities<kPoly, 0, 64>(s, p.scale_log2, m_ref, need_mask, sum4);
+          cp_probabilities<kPoly, 0, 64>(s, p.scale_log2, m_ref, need_mask || edge, sum4);
           tmem_st_32x32_at(tS, &s[0]);
           tmem_wait_st();
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl.p_first[t]);
-          cp_probabilities<kPoly, 64, 128>(s, p.scale_log2, m_ref, need_mask, sum4);
+          cp_probabilities<kPoly, 64, 128>(s, p.scale_log2, m_ref, need_mask || edge, sum4);
           tmem_st_32x32_at(tS + 32u, &s[32]);
           tmem_wait_st();
           tc_fence_before_sync();
@@ -680,7 +739,9 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
         if (ok && w.pair * 2 * CP_BM + t * CP_BM < qs.nrows) {
           const bool row_ok = row_in_seg < qs.nrows;
           tc_fence_after_sync();
-          const float inv = l > 0.f ? 1.f / l : 0.f;
+          if (kCache && row_in_seg >= w.rows_there) l = 0.f;   // not a query: zeros
+          // a NaN in a visible key makes the sum NaN, and the row
+          const float inv = kCache ? (l == 0.f ? 0.f : 1.f / l) : l > 0.f ? 1.f / l : 0.f;
           const int orow = qs.row0 + row_in_seg;
           __nv_bfloat16* dst =
               p.o[qs.out] + ((static_cast<size_t>(w.batch) * p.o_rows[qs.out] + orow) * p.o_heads +
@@ -711,7 +772,7 @@ __global__ void __launch_bounds__(CP_THREADS, 1) fa_cp_kernel(const __grid_const
           if (row_ok && p.lse[qs.out] != nullptr)
             p.lse[qs.out][(static_cast<size_t>(w.batch) * p.o_heads + p.o_head0 + w.head) *
                               p.o_rows[qs.out] + orow] =
-                l > 0.f ? (m_ref * 0.6931471805599453f + logf(l)) : -INFINITY;
+                (kCache ? l != 0.f : l > 0.f) ? (m_ref * 0.6931471805599453f + logf(l)) : -INFINITY;
         }
         tc_fence_before_sync();   // O has been read: the hand-over of the next item's first block says so
         g0 += w.nblk;

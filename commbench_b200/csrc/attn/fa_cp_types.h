@@ -70,6 +70,11 @@ struct FaCpParams {
   uint32_t* sched;       // [0] ticket counter, [1] CTAs that left
   uint32_t* status;
   unsigned long long timeout_ns;
+  // Sequences of a cache (kv_prefill.cu): query i of sequence b has position seq_start[b] + i, seq_count[b] (null:
+  // all rows) of them exist; a query at p sees the keys j <= p with j > p - window (0: all) or j < sinks.
+  const int* seq_start;
+  const int* seq_count;
+  int window, sinks;
 };
 
 }  // namespace cb

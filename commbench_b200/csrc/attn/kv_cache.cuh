@@ -12,6 +12,7 @@
 // rows of one chunk without bank conflicts from a tile that was copied as it is.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <stdint.h>
 
@@ -70,6 +71,21 @@ __device__ __forceinline__ uint32_t kv_to_half2(uint32_t two) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
   return h;
+}
+
+// 16 elements as bf16, exactly.
+__device__ __forceinline__ void kv_expand16(uint4 raw, float scale, __nv_bfloat16* dst) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t out[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t h = kv_to_half2(w[i >> 1] >> (16 * (i & 1)));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    const __nv_bfloat162 o = __floats2bfloat162_rn(f.x * scale, f.y * scale);
+    out[i] = *reinterpret_cast<const uint32_t*>(&o);
+  }
+  reinterpret_cast<uint4*>(dst)[0] = make_uint4(out[0], out[1], out[2], out[3]);
+  reinterpret_cast<uint4*>(dst)[1] = make_uint4(out[4], out[5], out[6], out[7]);
 }
 
 }  // namespace cb

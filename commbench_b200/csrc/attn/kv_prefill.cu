@@ -1,0 +1,184 @@
+// Attention of many query tokens per sequence over the paged 8-bit cache: prompts and long chunks.
+//
+// Here the products decide, not the cache's bytes, and they belong on tcgen05 at its bf16 rate: a first kernel
+// expands the keys and values that some query sees into bf16 tiles, and the tile-pair attention kernel (fa_cp.cuh)
+// takes them with every sequence's own positions and length, and the window.  The expansion is exact (an e4m3
+// number times a power of two fits bf16) and costs 5 bytes an element once, where the products cost 512 operations a
+// query head: 7000 tokens, 8 heads: 9 us of the call's.  e4m3 operands for the tensor cores would need the queries and the
+// probabilities in 8 bits too, or split in two terms of 4 bits, at the same rate as bf16.
+#include <cuda_runtime.h>
+
+#include <string>
+
+#include "../gemm/launch.h"
+#include "../symm/driver_api.h"
+#include "fa_cp.cuh"
+#include "kv_cache.cuh"
+
+namespace cb {
+
+struct KvExpandParams {
+  KvCacheView cache;
+  KvBatch batch;
+  __nv_bfloat16 *k, *v;        // [B, room, hkv, 128]
+  int room;                    // a multiple of 128
+  int window, sinks;
+  uint32_t* status;
+};
+
+// A CTA expands one head's keys and values of a block of 128 tokens, if some query sees it; rows past the end are
+// zeros, so that a probability of 0 meets a number.
+__global__ void __launch_bounds__(256) kv_expand_kernel(const __grid_constant__ KvExpandParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int hkv = p.cache.hkv, blocks = p.room / CP_BN;
+  const int head = blockIdx.x % hkv, rest = blockIdx.x / hkv;
+  const int b = rest / blocks, key0 = (rest - b * blocks) * CP_BN;
+  const int start = p.batch.start[b], count = p.batch.new_tokens(b);
+  if (start < 0 || count == 0) return;
+  const long long end = static_cast<long long>(start) + count;
+  if (key0 >= end) return;
+  if (end > p.room && threadIdx.x == 0) report_status(p.status, CB_BAD_ARGUMENT, 3, 0xA05);
+  if (p.window > 0 && key0 >= p.sinks && key0 + CP_BN <= start - p.window + 1) return;
+  const int chunk = threadIdx.x & 7;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = key0 + i * 32 + static_cast<int>(threadIdx.x >> 3);
+    uint4 rk = make_uint4(0, 0, 0, 0), rv = rk;
+    float sk = 0.f, sv = 0.f;
+    if (t < end) {
+      const int col = t >> p.cache.page_log2;
+      const int pid = col < p.batch.cols ? p.batch.pages[static_cast<long long>(b) * p.batch.cols + col] : -1;
+      if (pid >= 0 && pid < p.cache.num_pages) {
+        const int off = kv_offset(t & (p.cache.page() - 1), chunk * 16);
+        rk = *reinterpret_cast<const uint4*>(p.cache.tile(pid, head, 0) + off);
+        rv = *reinterpret_cast<const uint4*>(p.cache.tile(pid, head, 1) + off);
+        sk = kv_pow2(*p.cache.exp_of(pid, head, 0));
+        sv = kv_pow2(*p.cache.exp_of(pid, head, 1));
+      } else {
+        report_status(p.status, CB_BAD_ARGUMENT, 2, 0xA04);
+      }
+    }
+    const long long at = ((static_cast<long long>(b) * p.room + t) * hkv + head) * KV_D + chunk * 16;
+    kv_expand16(rk, sk, p.k + at);
+    kv_expand16(rv, sv, p.v + at);
+  }
+}
+
+static int prefill_tmap(CUtensorMap* out, const void* base, long long rows, int heads, long long row_stride,
+                        long long head_stride) {
+  const DriverApi& d = driver_api();
+  if (!d.ok) {
+    set_last_error("tensor map: " + d.why);
+    return -1;
+  }
+  cuuint64_t dims[3] = {CP_D, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2ull, static_cast<cuuint64_t>(row_stride) * 2ull};
+  cuuint32_t box[3] = {64, 1, CP_BM};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = d.cuTensorMapEncodeTiled(
+      out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error(cu_err("cuTensorMapEncodeTiled(cache attention)", r));
+    return -1;
+  }
+  return 0;
+}
+
+static long long prefill_room(int max_len) { return (static_cast<long long>(max_len) + CP_BN - 1) / CP_BN * CP_BN; }
+
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" {
+
+// Bytes of workspace for cb_kv_prefill, or -1.
+long long cb_kv_prefill_bytes(int B, int S, int Hq, int Hkv, int max_len) {
+  if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || max_len < 1 || prefill_room(max_len) * B > 0x7fffffffll ||
+      static_cast<long long>(B) * S > 0x7fffffffll ||
+      (static_cast<long long>(S) + 2 * CP_BM - 1) / (2 * CP_BM) * B * Hq > 0x7fffffffll) {
+    set_last_error("key/value attention: bad shape, or more than 2^31 rows");
+    return -1;
+  }
+  return 2 * prefill_room(max_len) * B * Hkv * KV_D * 2;
+}
+
+// As cb_kv_attend; q dense, or with strides that are multiples of 8 elements and sequences S tokens apart, 16-byte
+// aligned.  max_len bounds start + count: later keys are not seen (and leave a status word).
+int cb_kv_prefill(void* data, void* exps, int num_pages, int hkv, int page, const void* q, long long q_ss,
+                  long long q_sh, void* o, void* lse, const void* pages, int cols, const void* start,
+                  const void* count, int B, int S, int Hq, int window, int sinks, int max_len, float scale,
+                  void* workspace, long long workspace_bytes, void* status, void* stream) {
+  int lg = 0;
+  while ((1 << lg) < page) ++lg;
+  if (num_pages < 1 || page < 16 || page > 128 || (1 << lg) != page || cols < 1 || window < 0 || sinks < 0 ||
+      (reinterpret_cast<uintptr_t>(q) & 15u) != 0 || q_ss % 8 != 0 || q_sh % 8 != 0) {
+    set_last_error("key/value attention: bad cache, window, sinks or strides");
+    return -1;
+  }
+  const long long need = cb_kv_prefill_bytes(B, S, Hq, hkv, max_len);
+  if (need < 0) return -1;
+  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 127u) != 0) {
+    set_last_error("key/value attention: workspace missing, misaligned or too small");
+    return -1;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  KvExpandParams x;
+  x.cache = {static_cast<uint8_t*>(data), static_cast<int8_t*>(exps), num_pages, hkv, lg};
+  x.batch = {static_cast<const int*>(pages), static_cast<const int*>(start), static_cast<const int*>(count), B, S, cols};
+  x.room = static_cast<int>(prefill_room(max_len));
+  x.k = static_cast<__nv_bfloat16*>(workspace);
+  x.v = x.k + need / 4;
+  x.window = window;
+  x.sinks = sinks;
+  x.status = static_cast<uint32_t*>(status);
+  FaCpParams p = {};
+  const long long rows = static_cast<long long>(B) * x.room;
+  if (prefill_tmap(&p.tm_q_local, q, static_cast<long long>(B) * S, Hq, q_ss, q_sh)) return -1;
+  if (prefill_tmap(&p.tm_k, x.k, rows, hkv, static_cast<long long>(hkv) * KV_D, KV_D)) return -1;
+  if (prefill_tmap(&p.tm_v, x.v, rows, hkv, static_cast<long long>(hkv) * KV_D, KV_D)) return -1;
+  p.nseg = 1;
+  p.seg[0].nkeys = x.room;
+  p.seg[0].flag = -1;
+  p.nqseg = 1;
+  p.qseg[0].map = -1;
+  p.qseg[0].nrows = S;
+  p.o[0] = static_cast<__nv_bfloat16*>(o);
+  p.lse[0] = static_cast<float*>(lse);
+  p.o_rows[0] = S;
+  p.B = B;
+  p.heads = Hq;
+  p.o_heads = Hq;
+  p.kv_group = Hq / hkv;
+  p.q_bstride = S;
+  p.kv_bstride = x.room;
+  p.causal = 1;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = static_cast<uint32_t*>(status);
+  p.timeout_ns = 2000000000ull;
+  p.seq_start = static_cast<const int*>(start);
+  p.seq_count = static_cast<const int*>(count);
+  p.window = window;
+  p.sinks = window > 0 ? sinks : 0;
+
+  const long long blocks = static_cast<long long>(x.room / CP_BN) * B * hkv;
+  const long long items = (static_cast<long long>(S) + 2 * CP_BM - 1) / (2 * CP_BM) * B * Hq;
+  static std::atomic<uint64_t> smem_done{0};
+  auto kernel = fa_cp_kernel<0, true>;
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), CP_SMEM, smem_done);
+  if (e == cudaSuccess)
+    e = launch_pdl(kv_expand_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, x);
+  if (e == cudaSuccess)
+    e = launch_gemm_kernel_pdl(kernel, static_cast<int>(items), CP_THREADS, CP_SMEM, st, 1, false, true, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();   // reported here, not by the next call
+    set_last_error(std::string("key/value attention launch: ") + cudaGetErrorString(e));
+    return -1;
+  }
+  return 0;
+}
+
+}  // extern "C"

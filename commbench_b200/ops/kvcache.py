@@ -29,6 +29,14 @@ from ..utils.tracing import traced
 
 HEAD_DIM = 128
 _L9 = C.c_longlong * 9
+_FEW_ROWS = 64        # query rows per key/value head up to which a call is bound by the cache's bytes
+
+
+def _tileable(q):
+    """Whether the tile loads can read q where it lies: 16-byte rows, sequences S tokens apart."""
+    B, S = q.shape[:2]
+    return (q.data_ptr() % 16 == 0 and q.stride(1) % 8 == 0 and q.stride(2) % 8 == 0 and q.stride(1) > 0
+            and q.stride(2) > 0 and (B == 1 or q.stride(0) == S * q.stride(1)))
 
 
 def _heads(t, name, heads=None, shape=None):
@@ -134,17 +142,24 @@ class KVCache8:
 
     @traced("cb200.kv_attend")
     def attend(self, q, pages, start, count=None, window: int = 0, sinks: int = 0, scale: float | None = None,
-               max_len: int | None = None, status_ptr: int = 0, stream=None):
+               max_len: int | None = None, status_ptr: int = 0, stream=None, impl: str | None = None):
         """``(o [B, S, Hq, 128] bf16, lse [B, Hq, S] fp32)`` of queries at positions ``start[b] + i`` over the
         sequence's tokens up to each query's own (they have been appended).
 
         ``window`` > 0: a query at p sees the keys j > p - window, and the first ``sinks`` tokens of the sequence.
         Rows that see no key, and the rows from ``count[b]`` on, are zeros with lse -inf.  ``max_len``: an upper
-        bound of ``start + count`` that the host knows (default: what the table has room for)."""
+        bound of ``start + count`` that the host knows (default: what the table has room for); workspaces and the
+        cut of the work go by it, and later tokens are not seen.  A page id out of range leaves a status word, is
+        not read, and makes the rows that should see it meaningless.
+
+        ``impl``: "decode" (few query rows, bound by the cache's bytes) or "prefill" (tcgen05 tiles over an expanded
+        copy); by default the number of rows decides."""
         _heads(q, "q")
         B, S, Hq, _ = q.shape
         if Hq % self.kv_heads:
             raise CommError("query heads must be a multiple of the key/value heads")
+        if impl not in (None, "decode", "prefill"):
+            raise CommError(f"unknown attention form {impl!r}")
         if window < 0 or sinks < 0:
             raise CommError("window and sinks must not be negative")
         self._batch(pages, B, ((start, "start"), (count, "count")))
@@ -159,17 +174,22 @@ class KVCache8:
         max_len = room if max_len is None else max(1, min(int(max_len), room))
         sc = scale if scale is not None else 1.0 / math.sqrt(HEAD_DIM)
         lib = N.load()
+        long = S * (Hq // self.kv_heads) > _FEW_ROWS if impl is None else impl == "prefill"
+        if long and not _tileable(q):
+            with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(q.device)):
+                q = q.contiguous()
         with torch.cuda.device(q.device):
-            n = lib.cb_kv_attend_bytes(B, S, Hq, self.kv_heads, max_len)
+            n = (lib.cb_kv_prefill_bytes if long else lib.cb_kv_attend_bytes)(B, S, Hq, self.kv_heads, max_len)
             if n < 0:
                 raise CommError(f"key/value attention failed: {N.last_error()}")
             ws = q.new_empty((n,), dtype=torch.uint8) if stream is None else \
                 N.new_empty_on(stream, q, (n,), torch.uint8, handed_out=False)
-            rc = lib.cb_kv_attend(
+            strides = q.stride()[1:3] if long else q.stride()[:3]
+            rc = (lib.cb_kv_prefill if long else lib.cb_kv_attend)(
                 self.data.data_ptr(), self.exps.data_ptr(), self.num_pages, self.kv_heads, self.page, q.data_ptr(),
-                q.stride(0), q.stride(1), q.stride(2), o.data_ptr(), lse.data_ptr(), pages.data_ptr(),
-                pages.shape[1], start.data_ptr(), count.data_ptr() if count is not None else 0, B, S, Hq, window,
-                sinks, max_len, sc, ws.data_ptr(), n, status_ptr, N.raw_stream(stream))
+                *strides, o.data_ptr(), lse.data_ptr(), pages.data_ptr(), pages.shape[1], start.data_ptr(),
+                count.data_ptr() if count is not None else 0, B, S, Hq, window, sinks, max_len, sc, ws.data_ptr(), n,
+                status_ptr, N.raw_stream(stream))
         if rc != 0:
             raise CommError(f"key/value attention failed: {N.last_error()}")
         return o, lse

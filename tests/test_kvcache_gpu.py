@@ -221,10 +221,11 @@ def _case(lens, S, Hq, H, page, window=0, sinks=0, seed=20, max_len=None, count=
     q = torch.randn(B, S, Hq, D, device="cuda", generator=_gen(seed + 2)).bfloat16()
     cnt = count if count is not None else [S] * B
     start = [n - c for n, c in zip(lens, cnt)]
-    o, lse = cache.attend(q, pages, _ints(*start), count=None if count is None else _ints(*count), window=window,
-                          sinks=sinks, max_len=max_len, scale=scale)
     want = _attend64(q, _quantised(k, page, lens), _quantised(v, page, lens), start, cnt, window, sinks, scale)
-    _check(o, lse, want)
+    for impl in (None, "decode", "prefill"):
+        o, lse = cache.attend(q, pages, _ints(*start), count=None if count is None else _ints(*count), window=window,
+                              sinks=sinks, max_len=max_len, scale=scale, impl=impl)
+        _check(o, lse, want)
     return cache
 
 
@@ -239,7 +240,8 @@ def test_attend_head_groups(native_lib, group):
     _case([300, 77], 1, 2 * group, 2, 64)
 
 
-@pytest.mark.parametrize("S,group", [(2, 1), (3, 4), (4, 8), (5, 7), (8, 4), (33, 4), (100, 1), (64, 8), (130, 2)])
+@pytest.mark.parametrize("S,group", [(2, 1), (3, 4), (4, 8), (5, 7), (8, 4), (33, 4), (100, 1), (64, 8), (130, 2),
+                                     (255, 1), (256, 1), (257, 1)])
 def test_attend_several_tokens(native_lib, S, group):
     _case([S, S + 1, S + 700], S, 2 * group, 2, 32)
 
@@ -257,9 +259,9 @@ def test_attend_long_sequence_is_cut_over_the_chip(native_lib):
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 0), (32, 4), (33, 40), (100, 0), (100, 4), (100, 130),
                                           (257, 64), (1000, 4), (5000, 4)])
-@pytest.mark.parametrize("S", [1, 4, 70])
+@pytest.mark.parametrize("S", [1, 4, 70, 300])
 def test_attend_window_and_sinks(native_lib, S, window, sinks):
-    _case([max(S, 3), 70, 333, 900], S, 4, 2, 16 if S == 4 else 64, window=window, sinks=sinks)
+    _case([max(S, 3), max(S, 70), 333, 900], S, 4, 2, 16 if S == 4 else 64, window=window, sinks=sinks)
 
 
 def test_attend_counts_and_empty_rows(native_lib):
@@ -275,9 +277,10 @@ def test_attend_strides_and_scale(native_lib):
     q = big[:, :, 1:20:2, 4:].transpose(0, 0)[:, :, :8]
     q = q if q.data_ptr() % 8 == 0 else big[:, :, :8, :D]
     start = _ints(87, 87)
-    o, lse = cache.attend(q, pages, start, scale=0.03)
-    o2, lse2 = cache.attend(q.contiguous(), pages, start, scale=0.03)
-    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    for impl in ("prefill", "decode"):
+        o, lse = cache.attend(q, pages, start, scale=0.03, impl=impl)
+        o2, lse2 = cache.attend(q.contiguous(), pages, start, scale=0.03, impl=impl)
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
     _check(o, lse, _attend64(q, _quantised(k, 64, (90, 90)), _quantised(v, 64, (90, 90)), (87, 87), (3, 3), 0, 0, 0.03))
 
 
@@ -343,13 +346,14 @@ def test_attend_repeats_its_bits_and_runs_on_another_stream(native_lib):
     cache, pages = _filled(k, v, 64, (1500, 700, 64), 71)
     q = torch.randn(3, 2, 8, D, device="cuda", generator=_gen(72)).bfloat16()
     start = _ints(1498, 698, 62)
-    o, lse = cache.attend(q, pages, start)
-    s = torch.cuda.Stream()
-    for i in range(4):
-        s.wait_stream(torch.cuda.current_stream())
-        o2, lse2 = cache.attend(q, pages, start, stream=s if i % 2 else None)
-        torch.cuda.current_stream().wait_stream(s)
-        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    for impl in ("decode", "prefill"):
+        o, lse = cache.attend(q, pages, start, impl=impl)
+        s = torch.cuda.Stream()
+        for i in range(4):
+            s.wait_stream(torch.cuda.current_stream())
+            o2, lse2 = cache.attend(q, pages, start, stream=s if i % 2 else None, impl=impl)
+            torch.cuda.current_stream().wait_stream(s)
+            assert torch.equal(o, o2) and torch.equal(lse, lse2)
 
 
 def test_decode_steps_in_a_graph(native_lib):
@@ -429,7 +433,7 @@ def test_cache_refusals(native_lib):
                 lambda: cache.read(pages, start.float(), 3), lambda: cache.attend(q[:, :, :3], pages, start),
                 lambda: cache.attend(q, pages, start, window=-1), lambda: cache.attend(q, pages, start, sinks=-1),
                 lambda: cache.attend(q.half(), pages, start), lambda: cache.attend(q, pages, start, count=_ints(1, 1)),
-                lambda: cache.attend(q, pages.cpu(), start)):
+                lambda: cache.attend(q, pages.cpu(), start), lambda: cache.attend(q, pages, start, impl="other")):
         with pytest.raises(CommError):
             bad()
     assert cache.attend(q[:, :0], pages, start)[0].shape == (1, 0, 4, D)
