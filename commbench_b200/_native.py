@@ -109,9 +109,9 @@ _HOT_ARGTYPES = {
     "cb_moe_router_topk": [_P, _I, _I, _I, _P, _P, _P],
     "cb_moe_slots": [_P, _I, _I, _P, _P, _P],
     "cb_moe_plan": [_P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P],
-    "cb_rms_norm": [_P] * 7 + [_L] * 3 + [_I] * 4 + [_F, _P],
+    "cb_rms_norm": [_P] * 7 + [_L] * 3 + [_I] * 4 + [_F, _P, _P],
     "cb_rms_norm_backward_floats": [_P] * 5 + [_L] * 4 + [_I] * 3,
-    "cb_rms_norm_backward": [_P] * 7 + [_L] * 4 + [_I] * 3 + [_F, _P],
+    "cb_rms_norm_backward": [_P] * 7 + [_L] * 4 + [_I] * 3 + [_F, _P, _P],
     "cb_rope": ([_P, _P, _L, _L, _L, _I] * 2 + [_I] * 3 + [_P, _P, _I, _I, _I, _P] + [_I] * 4 + [_P, _P]),
     "cb_kv_append": ([_P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _I, _P, _P, _I, _P, _P] + [_I] * 3 +
                      [_P, _P]),
@@ -155,7 +155,9 @@ def load():
 
 _FAST_ENTRIES = ("cb_gemm_bf16", "cb_gemm_fp8", "cb_gemm_fp8_blockscaled", "cb_gemm_fp8_mx",
                  "cb_quant_blockscaled", "cb_quant_blockscaled_pow2", "cb_attn_fwd4",
-                 "cb_attn_split_bytes", "cb_attn_split")
+                 "cb_attn_split_bytes", "cb_attn_split", "cb_rms_norm", "cb_rms_norm_backward_floats",
+                 "cb_rms_norm_backward", "cb_rope", "cb_kv_append", "cb_kv_read", "cb_kv_attend_bytes",
+                 "cb_kv_prefill_bytes", "cb_kv_attend", "cb_kv_prefill")
 
 
 class _NoFast:

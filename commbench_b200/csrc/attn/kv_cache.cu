@@ -25,6 +25,8 @@ struct KvAppendParams {
   long long k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, q_sb, q_ss, q_sh;
   RopeTableView rope;                               // rot = 0: none
   int hq, pages_per_seq, kv_blocks;
+  int wide;                                         // queries in vectors of 8 elements, else of 4
+  RopeShare share;                                  // of the queries
   uint32_t* status;
 };
 
@@ -75,39 +77,49 @@ __device__ __forceinline__ void lane_rotate(const RopeTableView& t, const LaneAn
   }
 }
 
-static constexpr int KV_Q_HEADS = 8;   // query heads a warp turns with one token's angles
+static constexpr int KV_THREADS = 512;
+static constexpr int KV_WARPS = KV_THREADS / 32;
+static constexpr int KV_Q_HEADS = 2;   // query heads whose loads a thread has in flight
 
-__device__ __forceinline__ void append_queries(const KvAppendParams& p, long long warp, int lane) {
-  const int groups = (p.hq + KV_Q_HEADS - 1) / KV_Q_HEADS;
-  const long long tok = warp / groups;
-  if (tok >= static_cast<long long>(p.batch.B) * p.batch.S) return;
-  const int h0 = static_cast<int>(warp - tok * groups) * KV_Q_HEADS;
+// The queries of p.share.tokens tokens.
+template <int V, bool kHalf>
+__device__ __forceinline__ void append_queries(const KvAppendParams& p, int block) {
+  const RopeShare& sh = p.share;
+  const int per_token = sh.lanes * sh.head_lanes;
+  const int t = threadIdx.x / per_token, in = threadIdx.x - t * per_token;
+  const long long tok = static_cast<long long>(block) * sh.tokens + t;
+  if (t >= sh.tokens || tok >= static_cast<long long>(p.batch.B) * p.batch.S) return;
+  const int hy = in / sh.lanes, lane = in - hy * sh.lanes;
   const int b = static_cast<int>(tok / p.batch.S), i = static_cast<int>(tok - static_cast<long long>(b) * p.batch.S);
-  const bool there = i < p.batch.new_tokens(b);
-  const __nv_bfloat16* src = p.q + b * p.q_sb + i * p.q_ss + 4 * lane;
-  __nv_bfloat16* dst = p.q_out + tok * p.hq * KV_D + 4 * lane;
-  float x[KV_Q_HEADS][4];
-#pragma unroll
-  for (int h = 0; h < KV_Q_HEADS; ++h)
-    if (there && h0 + h < p.hq) load_vec<__nv_bfloat16, 4>(src + (h0 + h) * p.q_sh, x[h]);
-  const LaneAngles a = lane_angles(p.rope, static_cast<long long>(p.batch.start[b]) + i, lane);
-#pragma unroll
-  for (int h = 0; h < KV_Q_HEADS; ++h) {
-    if (!there) x[h][0] = x[h][1] = x[h][2] = x[h][3] = 0.f;   // padding: zeros
-    if (there) lane_rotate(p.rope, a, x[h]);
-    if (h0 + h < p.hq) store_vec<__nv_bfloat16, 4>(dst + (h0 + h) * KV_D, x[h]);
+  __nv_bfloat16* dst = p.q_out + tok * p.hq * KV_D;
+  if (i >= p.batch.new_tokens(b)) {      // padding: zeros
+    for (int d = in * 4; d < p.hq * KV_D; d += per_token * 4) *reinterpret_cast<uint2*>(dst + d) = make_uint2(0u, 0u);
+    return;
   }
+  RopeRows<__nv_bfloat16> r;
+  r.x0 = r.x1 = p.q + b * p.q_sb + i * p.q_ss;
+  r.y0 = r.y1 = dst;
+  r.sh0 = r.sh1 = p.q_sh;
+  r.heads0 = r.heads = p.hq;
+  r.D = KV_D;
+  const long long pos = static_cast<long long>(p.batch.start[b]) + i;
+  for (int item = lane; item < sh.items; item += sh.lanes)
+    rope_item<__nv_bfloat16, V, kHalf, KV_Q_HEADS>(p.rope, sh, r, pos, 1.f, hy, item);
 }
 
-// kTokens: token slots of a page per warp (8 warps).
+// kTokens: token slots of a page per warp.
 template <int kTokens>
-__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
-  __shared__ float sh_max[2][8];
+__global__ void __launch_bounds__(KV_THREADS, kTokens <= 4 ? 2 : 1) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
+  __shared__ float sh_max[2][KV_WARPS];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (static_cast<int>(blockIdx.x) >= p.kv_blocks) {
-    append_queries(p, static_cast<long long>(blockIdx.x - p.kv_blocks) * 8 + warp, lane);
+    const int block = static_cast<int>(blockIdx.x) - p.kv_blocks;
+    if (p.rope.interleaved)
+      p.wide ? append_queries<8, false>(p, block) : append_queries<4, false>(p, block);
+    else
+      p.wide ? append_queries<8, true>(p, block) : append_queries<4, true>(p, block);
     return;
   }
   const int hkv = p.cache.hkv, page = p.cache.page();
@@ -137,14 +149,14 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     float x[kTokens][4];
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
-      const int t = warp + 8 * i;
+      const int t = warp + KV_WARPS * i;
       x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
       if (t >= lo && t < hi) load_vec<__nv_bfloat16, 4>(src + (t0 + t - start) * ss + 4 * lane, x[i]);
     }
     if (side == 0 && p.rope.rot > 0) {
 #pragma unroll
       for (int i = 0; i < kTokens; ++i) {
-        const int t = warp + 8 * i;
+        const int t = warp + KV_WARPS * i;
         if (t >= lo && t < hi) {
           if (t0 + t >= p.rope.positions && lane == 0) report_status(p.status, CB_BAD_ARGUMENT, 1, 0xA01);
           lane_rotate(p.rope, lane_angles(p.rope, t0 + t, lane), x[i]);
@@ -172,7 +184,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     if (lane == 0) sh_max[side][warp] = amax;
     __syncthreads();
-    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(sh_max[side][lane & 7])));
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(sh_max[side][lane & (KV_WARPS - 1)])));
     int8_t* exp_at = p.cache.exp_of(pid, head, side);
     int e = kv_exponent(amax), e_old = e;
     if (lo > 0) {
@@ -182,7 +194,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     uint8_t* tile = p.cache.tile(pid, head, side);
     if (e != e_old) {
       const float f = kv_pow2(e_old - e < -126 ? -126 : e_old - e);
-      for (int t = warp; t < lo; t += 8) {
+      for (int t = warp; t < lo; t += KV_WARPS) {
         uint32_t* at = reinterpret_cast<uint32_t*>(tile + kv_offset(t, 4 * lane));
         const uint32_t old = *at;
         const uint32_t h0 = kv_to_half2(old), h1 = kv_to_half2(old >> 16);
@@ -194,7 +206,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     const float inv = e == KV_EXP_MIN ? 0.f : kv_pow2(-e);          // the least exponent says: all zero
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
-      const int t = warp + 8 * i;
+      const int t = warp + KV_WARPS * i;
       if (t >= lo && t < hi) {
         if (side == 0 && lane == 0 && ((bad >> i) & 1u)) x[i][0] = __int_as_float(0x7fc00000);
         *reinterpret_cast<uint32_t*>(tile + kv_offset(t, 4 * lane)) =
@@ -291,21 +303,28 @@ int cb_kv_append(void* data, void* exps, int num_pages, int hkv, int page, const
   p.pages_per_seq = (S + page - 2) / page + 1;
   p.status = static_cast<uint32_t*>(status);
   const long long kv_blocks = static_cast<long long>(B) * p.pages_per_seq * hkv;
-  const long long q_warps = q == nullptr ? 0 : static_cast<long long>(B) * S * ((hq + KV_Q_HEADS - 1) / KV_Q_HEADS);
-  const long long blocks = kv_blocks + (q_warps + 7) / 8;
+  p.wide = rot % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0 &&
+           p.q_sb % 8 == 0 && p.q_ss % 8 == 0 && p.q_sh % 8 == 0;
+  p.share = {};
+  long long q_blocks = 0;
+  if (q != nullptr) {
+    p.share.set(KV_THREADS, KV_D, rot, p.wide ? 8 : 4, !interleaved, hq, KV_Q_HEADS);
+    q_blocks = (static_cast<long long>(B) * S + p.share.tokens - 1) / p.share.tokens;
+  }
+  const long long blocks = kv_blocks + q_blocks;
   if (blocks > 0x7fffffffll) {
     set_last_error("key/value cache: too many tokens in one call");
     return -1;
   }
   p.kv_blocks = static_cast<int>(kv_blocks);
-  const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(KV_THREADS);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (page) {
-    case 16: e = launch_pdl(kv_append_kernel<2>, grid, block, 0, st, p); break;
-    case 32: e = launch_pdl(kv_append_kernel<4>, grid, block, 0, st, p); break;
-    case 64: e = launch_pdl(kv_append_kernel<8>, grid, block, 0, st, p); break;
-    default: e = launch_pdl(kv_append_kernel<16>, grid, block, 0, st, p); break;
+    case 16: e = launch_pdl(kv_append_kernel<1>, grid, block, 0, st, p); break;
+    case 32: e = launch_pdl(kv_append_kernel<2>, grid, block, 0, st, p); break;
+    case 64: e = launch_pdl(kv_append_kernel<4>, grid, block, 0, st, p); break;
+    default: e = launch_pdl(kv_append_kernel<8>, grid, block, 0, st, p); break;
   }
   if (e != cudaSuccess) {
     cudaGetLastError();   // reported here, not by the next call

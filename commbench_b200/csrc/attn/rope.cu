@@ -3,7 +3,8 @@
 // the others are copied.  Pairs are (i, i + rot / 2) or (2 i, 2 i + 1).  The transpose (s -> -s) is the gradient.
 //
 // Bound by memory: one read and one write of x.  The table is fp32 made in 64 bits - an angle of 10^5 turns
-// computed in fp32 would be off by a percent of a turn - and a thread keeps its entries for all heads of a token.
+// computed in fp32 would be off by a percent of a turn - and a thread uses its entries for several heads, whose loads
+// are in flight together.
 #include <cuda_runtime.h>
 
 #include <string>
@@ -30,86 +31,49 @@ struct RopeParams {
   const void* pos;                   // [B, S] or, with pos_batched = 0, [S]
   int pos_i64, pos_batched;
   float sign;                        // -1: transpose
-  int pair_items, copy_items;        // work items of a head
+  RopeShare share;
   uint32_t* status;
 };
 
-// A CTA takes tokens in turn; thread = (head of a group of `hy`, item), an item being V elements of both halves
-// (kHalf), V neighbouring elements (V / 2 pairs; a pair for V = 1), or V elements to copy.
+static constexpr int ROPE_THREADS = 256;
+static constexpr int ROPE_HEADS = 3;   // heads whose loads a thread has in flight
+
 template <class T, int V, bool kHalf>
-__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(ROPE_THREADS, 4) rope_kernel(const __grid_constant__ RopeParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  const int items = p.pair_items + p.copy_items;
-  const int per_pass = items < 256 ? items : 256;
-  const int hy_n = 256 / per_pass;
-  const int hy = threadIdx.x / per_pass;
-  if (hy >= hy_n) return;
-  const int half = p.table.rot / 2;
-  const long long tokens = static_cast<long long>(p.B) * p.S;
-  for (long long tok = blockIdx.x; tok < tokens; tok += gridDim.x) {
-    const int b = static_cast<int>(tok / p.S), s = static_cast<int>(tok - static_cast<long long>(b) * p.S);
-    const long long pi = p.pos_batched ? tok : s;
-    const long long pos = p.pos_i64 ? static_cast<const long long*>(p.pos)[pi] : static_cast<const int*>(p.pos)[pi];
-    const bool known = pos >= 0 && pos < p.table.positions;
-    if (!known && threadIdx.x == 0) report_status(p.status, CB_BAD_ARGUMENT, 1, 0xA01);
-    for (int item = threadIdx.x - hy * per_pass; item < items; item += per_pass) {
-      const bool pair = item < p.pair_items;
-      constexpr int P = kHalf || V == 1 ? V : V / 2;   // pairs of an item
-      float c[P], sn[P];
-      const int first = item * P;                      // first pair
-      if (pair) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          // outside the table there is no rotation: the answer is NaN, not some other position's
-          c[i] = known ? __ldg(p.table.cos + pos * half + first + i) : __int_as_float(0x7fc00000);
-          sn[i] = known ? p.sign * __ldg(p.table.sin + pos * half + first + i) : __int_as_float(0x7fc00000);
-        }
-      }
-      for (int k = 0; k < p.tensors; ++k) {
-        const RopeTensor& t = p.t[k];
-        const T* x0 = static_cast<const T*>(t.x) + b * t.sb + s * t.ss;
-        T* y0 = static_cast<T*>(t.y) + tok * t.heads * p.D;
-        for (int h = hy; h < t.heads; h += hy_n) {
-          const T* x = x0 + h * t.sh;
-          T* y = y0 + static_cast<long long>(h) * p.D;
-          if (!pair) {
-            const int d = p.table.rot + (item - p.pair_items) * V;
-            *reinterpret_cast<Vec<T, V>*>(y + d) = *reinterpret_cast<const Vec<T, V>*>(x + d);
-          } else if constexpr (kHalf) {
-            float a[V], e[V], ya[V], ye[V];
-            load_vec<T, V>(x + first, a);
-            load_vec<T, V>(x + half + first, e);
-#pragma unroll
-            for (int i = 0; i < V; ++i) rotate_pair(a[i], e[i], c[i], sn[i], &ya[i], &ye[i]);
-            store_vec<T, V>(y + first, ya);
-            store_vec<T, V>(y + half + first, ye);
-          } else if constexpr (V > 1) {
-            float a[V], ya[V];
-            load_vec<T, V>(x + 2 * first, a);
-#pragma unroll
-            for (int i = 0; i < V; i += 2) rotate_pair(a[i], a[i + 1], c[i / 2], sn[i / 2], &ya[i], &ya[i + 1]);
-            store_vec<T, V>(y + 2 * first, ya);
-          } else {
-            float ya, yb;
-            rotate_pair(to_f32(x[2 * first]), to_f32(x[2 * first + 1]), c[0], sn[0], &ya, &yb);
-            y[2 * first] = from_f32<T>(ya);
-            y[2 * first + 1] = from_f32<T>(yb);
-          }
-        }
-      }
-    }
+  const RopeShare& sh = p.share;
+  const int per_token = sh.lanes * sh.head_lanes;
+  const int t = threadIdx.x / per_token, in = threadIdx.x - t * per_token;
+  const int s = static_cast<int>(blockIdx.x) * sh.tokens + t;
+  if (t >= sh.tokens || s >= p.S) return;
+  const int hy = in / sh.lanes, lane = in - hy * sh.lanes;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+  const long long tok = static_cast<long long>(b) * p.S + s;
+  const long long pi = p.pos_batched ? tok : s;
+  const long long pos = p.pos_i64 ? static_cast<const long long*>(p.pos)[pi] : static_cast<const int*>(p.pos)[pi];
+  if ((pos < 0 || pos >= p.table.positions) && in == 0) report_status(p.status, CB_BAD_ARGUMENT, 1, 0xA01);
+  RopeRows<T> r;
+  r.x0 = static_cast<const T*>(p.t[0].x) + b * p.t[0].sb + s * p.t[0].ss;
+  r.x1 = static_cast<const T*>(p.t[1].x) + b * p.t[1].sb + s * p.t[1].ss;
+  r.y0 = static_cast<T*>(p.t[0].y) + tok * p.t[0].heads * p.D;
+  r.y1 = static_cast<T*>(p.t[1].y) + tok * p.t[1].heads * p.D;
+  r.sh0 = p.t[0].sh;
+  r.sh1 = p.t[1].sh;
+  r.heads0 = p.t[0].heads;
+  r.heads = r.heads0 + (p.tensors > 1 ? p.t[1].heads : 0);
+  r.D = p.D;
+  for (int item = lane; item < sh.items; item += sh.lanes)
+    rope_item<T, V, kHalf, ROPE_HEADS>(p.table, sh, r, pos, p.sign, hy, item);
   }
 }
 
 template <class T, int V, bool kHalf>
 static int rope_go(RopeParams p, cudaStream_t st) {
-  const int rot = p.table.rot;
-  p.pair_items = kHalf ? rot / 2 / V : (V == 1 ? rot / 2 : rot / V);
-  p.copy_items = (p.D - rot) / V;
-  const long long tokens = static_cast<long long>(p.B) * p.S;
-  const unsigned grid = static_cast<unsigned>(tokens < 148 * 32 ? tokens : 148 * 32);
-  const cudaError_t e = launch_pdl(rope_kernel<T, V, kHalf>, dim3(grid), dim3(256), 0, st, p);
+  p.share.set(ROPE_THREADS, p.D, p.table.rot, V, kHalf, p.t[0].heads + (p.tensors > 1 ? p.t[1].heads : 0), ROPE_HEADS);
+  const int blocks = (p.S + p.share.tokens - 1) / p.share.tokens;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.B < 65535 ? p.B : 65535));
+  const cudaError_t e = launch_pdl(rope_kernel<T, V, kHalf>, grid, dim3(ROPE_THREADS), 0, st, p);
   if (e != cudaSuccess) {
     cudaGetLastError();   // reported here, not by the next call
     set_last_error(std::string("rope launch: ") + cudaGetErrorString(e));
@@ -161,7 +125,6 @@ int cb_rope(const void* x0, void* y0, long long sb0, long long ss0, long long sh
   p.pos_i64 = pos_i64;
   p.pos_batched = pos_batched;
   p.sign = inverse ? -1.f : 1.f;
-  p.pair_items = p.copy_items = 0;
   p.status = static_cast<uint32_t*>(status);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (type == ELEM_BF16) return rope_typed<__nv_bfloat16>(p, st);

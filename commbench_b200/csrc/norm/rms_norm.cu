@@ -12,8 +12,10 @@
 
 #include <string>
 
+#include "../gemm/launch.h"
 #include "../prim/elem.cuh"
 #include "../prim/pdl.cuh"
+#include "../prim/tma.cuh"
 
 namespace cb {
 void set_last_error(const std::string& s);
@@ -30,6 +32,7 @@ struct NormParams {
   long long rows;
   int D, w_f32;
   float eps;
+  uint32_t* status;
 };
 
 template <class T, int V>
@@ -170,76 +173,199 @@ __global__ void __launch_bounds__(VPT == 4 || VPT == 8 ? 512 : 1024) rms_norm_ke
   }
 }
 
+// Many long rows: CTAs that stay, each with a ring of rows in shared memory that bulk copies fill ahead, so that the
+// loads of the next rows never wait for the sum of the present one.  A thread keeps its columns' weights.  The barrier
+// of the sum also says that every thread has taken the row out of its slot.
+struct NormRing {
+  int slots, row_bytes;
+};
+// A copy never arrived: the others get time to land before the shared memory goes to another CTA.
+__device__ __forceinline__ void ring_abandon(const volatile int* abort_flag) {
+  if (*abort_flag == 0) return;
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+}
+static constexpr int NORM_SLOTS = 6;
+static constexpr int NORM_RING_BYTES = 200 * 1024;   // of an SM
+
+template <class T, int V, int VPT, int kMode>
+__global__ void __launch_bounds__(512, 2)
+    rms_norm_ring_kernel(const __grid_constant__ NormParams p, const __grid_constant__ NormRing ring) {
+  extern __shared__ __align__(128) uint8_t norm_smem[];
+  __shared__ float sh[2][32];
+  __shared__ uint64_t full[NORM_SLOTS];
+  __shared__ int abort_flag;
+  const int t = threadIdx.x, threads = blockDim.x;
+  const bool two = p.res != nullptr;
+  const uint32_t slot_bytes = ring.row_bytes * (two ? 2 : 1);
+  if (t == 0) {
+    for (int i = 0; i < ring.slots; ++i) mbar_init(&full[i], 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+  auto issue = [&](long long row, int slot) {
+    uint8_t* dst = norm_smem + slot * slot_bytes;
+    mbar_arrive_expect_tx(&full[slot], slot_bytes);
+    bulk_load_1d(dst, static_cast<const T*>(p.x) + row * p.x_stride, ring.row_bytes, &full[slot]);
+    if (two) bulk_load_1d(dst + ring.row_bytes, static_cast<const T*>(p.res) + row * p.res_stride, ring.row_bytes, &full[slot]);
+  };
+  if (t == 0)
+    for (int i = 0; i < ring.slots; ++i) {
+      const long long row = blockIdx.x + static_cast<long long>(i) * gridDim.x;
+      if (row < p.rows) issue(row, i);
+    }
+  float w[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int col = (i * threads + t) * V;
+    if (col < p.D) load_weight<T, V>(p.w, p.w_f32, col, w[i]);
+  }
+  int slot = 0, round = 0;
+  uint32_t phase = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, ++round) {
+    if (!mbar_wait(&full[slot], phase, &abort_flag, p.status, 0xA20)) break;
+    const T* x = reinterpret_cast<const T*>(norm_smem + slot * slot_bytes);
+    const T* r = reinterpret_cast<const T*>(norm_smem + slot * slot_bytes + ring.row_bytes);
+    float h[VPT][V];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int col = (i * threads + t) * V;
+      if (col < p.D) {
+        load_vec<T, V>(x + col, h[i]);
+        if (two) {
+          float a[V];
+          load_vec<T, V>(r + col, a);
+#pragma unroll
+          for (int j = 0; j < V; ++j) h[i][j] += a[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[i][j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) ss += h[i][j] * h[i][j];
+    }
+    ss = row_sum<false>(ss, sh, round);
+    if (t == 0) {
+      const long long next = row + static_cast<long long>(ring.slots) * gridDim.x;
+      if (next < p.rows) issue(next, slot);
+    }
+    const float rstd = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int col = (i * threads + t) * V;
+      const bool active = col < p.D;
+      if (active && two) store_vec<T, V>(static_cast<T*>(p.h) + row * p.D + col, h[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rstd * w[i][j];
+      if constexpr (kMode == NORM_PLAIN) {
+        if (active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
+      } else {
+        store_quantised<V, kMode>(p, row, col, h[i], active);
+      }
+    }
+    if (++slot == ring.slots) slot = 0, phase ^= 1u;
+  }
+  ring_abandon(&abort_flag);
+}
+
 struct NormBwdParams {
+  NormRing ring;                 // slots = 0: none
   const void *dy, *h, *w, *dh;   // dh or null
   void* dx;
   float* part;                   // [gridDim.x, D]
   long long dy_stride, h_stride, dh_stride, rows;
   int D, w_f32;
   float eps;
+  uint32_t* status;
 };
 
-// A CTA takes rows blockIdx.x, blockIdx.x + gridDim.x, ... with the next row's operands on their way while the
-// present one is summed up.  A thread keeps its columns through all of them, and with them its share of dw, which
-// goes to `part` at the end: sums of a fixed order, no atomics.
-// Long rows have no registers left for that and for the weights: they read both when they need them.
-template <class T, int V, int VPT>
+// A CTA takes rows blockIdx.x, blockIdx.x + gridDim.x, ...  A thread keeps its columns through all of them, and with
+// them its share of dw, which goes to `part` at the end: sums of a fixed order, no atomics.
+// kRing: the rows come through a ring in shared memory as above (the operands of a row are dy, h and dh).
+template <class T, int V, int VPT, bool kRing>
 __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p) {
+  extern __shared__ __align__(128) uint8_t norm_smem[];
   __shared__ float sh[2][2][32];
+  __shared__ uint64_t full[NORM_SLOTS];
+  __shared__ int abort_flag;
+  const int t = threadIdx.x, threads = blockDim.x, lane = t & 31;
+  const bool three = p.dh != nullptr;
+  const uint32_t slot_bytes = p.ring.row_bytes * (three ? 3 : 2);
+  if constexpr (kRing) {
+    if (t == 0) {
+      for (int i = 0; i < p.ring.slots; ++i) mbar_init(&full[i], 1);
+      abort_flag = 0;
+      fence_mbar_init();
+    }
+    __syncthreads();
+  }
   pdl_wait();
   pdl_launch_dependents();
-  const int t = threadIdx.x, threads = blockDim.x, lane = t & 31;
-  using V16 = Vec<T, V>;
-  V16 zero;
-#pragma unroll
-  for (int j = 0; j < V; ++j) zero.e[j] = from_f32<T>(0.f);
+  using W = Vec<T, V>;
   const T* dy = static_cast<const T*>(p.dy);
   const T* h = static_cast<const T*>(p.h);
   const T* dh = static_cast<const T*>(p.dh);
-  constexpr bool kAhead = VPT == 1;
+  auto issue = [&](long long row, int slot) {
+    uint8_t* dst = norm_smem + slot * slot_bytes;
+    mbar_arrive_expect_tx(&full[slot], slot_bytes);
+    bulk_load_1d(dst, dy + row * p.dy_stride, p.ring.row_bytes, &full[slot]);
+    bulk_load_1d(dst + p.ring.row_bytes, h + row * p.h_stride, p.ring.row_bytes, &full[slot]);
+    if (three) bulk_load_1d(dst + 2 * p.ring.row_bytes, dh + row * p.dh_stride, p.ring.row_bytes, &full[slot]);
+  };
+  if (kRing && t == 0)
+    for (int i = 0; i < p.ring.slots; ++i) {
+      const long long row = blockIdx.x + static_cast<long long>(i) * gridDim.x;
+      if (row < p.rows) issue(row, i);
+    }
+  // Long rows have no registers for their weights: they read them when they need them.
   float w1[V], dw[VPT][V];
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) w1[j] = dw[i][j] = 0.f;
-  if (kAhead && t * V < p.D) load_weight<T, V>(p.w, p.w_f32, t * V, w1);
+  if (VPT == 1 && t * V < p.D) load_weight<T, V>(p.w, p.w_f32, t * V, w1);
   auto weight = [&](int i, float(&w)[V]) {
     const int col = (i * threads + t) * V;
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[j] = kAhead ? w1[j] : 0.f;
-    if (!kAhead && col < p.D) load_weight<T, V>(p.w, p.w_f32, col, w);
+    for (int j = 0; j < V; ++j) w[j] = VPT == 1 ? w1[j] : 0.f;
+    if (VPT > 1 && col < p.D) load_weight<T, V>(p.w, p.w_f32, col, w);
   };
-  V16 ny[VPT], nh[VPT], nd[VPT];
-  auto fetch = [&](long long row) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int col = (i * threads + t) * V;
-      ny[i] = nh[i] = nd[i] = zero;
-      if (col < p.D && row < p.rows) {
-        ny[i] = *reinterpret_cast<const V16*>(dy + row * p.dy_stride + col);
-        nh[i] = *reinterpret_cast<const V16*>(h + row * p.h_stride + col);
-        if (dh != nullptr) nd[i] = *reinterpret_cast<const V16*>(dh + row * p.dh_stride + col);
-      }
-    }
-  };
-  if (kAhead) fetch(blockIdx.x);
-  int round = 0;
+  int round = 0, slot = 0;
+  uint32_t phase = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, ++round) {
-    if (!kAhead) fetch(row);
-    V16 cy[VPT], ch[VPT], cd[VPT];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) cy[i] = ny[i], ch[i] = nh[i], cd[i] = nd[i];
-    if (kAhead) fetch(row + gridDim.x);
+    const T *ry = dy + row * p.dy_stride, *rh = h + row * p.h_stride, *rd = dh + row * p.dh_stride;
+    if constexpr (kRing) {
+      if (!mbar_wait(&full[slot], phase, &abort_flag, p.status, 0xA20)) break;
+      ry = reinterpret_cast<const T*>(norm_smem + slot * slot_bytes);
+      rh = reinterpret_cast<const T*>(norm_smem + slot * slot_bytes + p.ring.row_bytes);
+      rd = reinterpret_cast<const T*>(norm_smem + slot * slot_bytes + 2 * p.ring.row_bytes);
+    }
+    W cy[VPT], ch[VPT], cd[VPT];
     float ss = 0.f, gh = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float w[V];
+      const int col = (i * threads + t) * V;
+      clear(cy[i]);
+      clear(ch[i]);
+      clear(cd[i]);
+      if (col < p.D) {
+        cy[i] = *reinterpret_cast<const W*>(ry + col);
+        ch[i] = *reinterpret_cast<const W*>(rh + col);
+        if (three) cd[i] = *reinterpret_cast<const W*>(rd + col);
+      }
+      float w[V], a[V], b[V];
       weight(i, w);
+      unpack(ch[i], a);
+      unpack(cy[i], b);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float a = to_f32(ch[i].e[j]);
-        ss += a * a;
-        gh += to_f32(cy[i].e[j]) * w[j] * a;
+        ss += a[j] * a[j];
+        gh += b[j] * w[j] * a[j];
       }
     }
     ss = warp_sum(ss);
@@ -247,6 +373,10 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) rms_norm_bwd_kernel(con
     float(*s)[32] = sh[round & 1];
     if (lane == 0) s[0][t >> 5] = ss, s[1][t >> 5] = gh;
     __syncthreads();
+    if (kRing && t == 0) {
+      const long long next = row + static_cast<long long>(p.ring.slots) * gridDim.x;
+      if (next < p.rows) issue(next, slot);
+    }
     const bool have = lane < (threads >> 5);
     ss = warp_sum(have ? s[0][lane] : 0.f);
     gh = warp_sum(have ? s[1][lane] : 0.f);
@@ -255,17 +385,21 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) rms_norm_bwd_kernel(con
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int col = (i * threads + t) * V;
-      float dx[V], w[V];
+      float dx[V], w[V], a[V], b[V];
       weight(i, w);
+      unpack(ch[i], a);
+      unpack(cy[i], b);
+      unpack(cd[i], dx);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float a = to_f32(ch[i].e[j]), b = to_f32(cy[i].e[j]);
-        dx[j] = rstd * (b * w[j]) - a * c + to_f32(cd[i].e[j]);
-        dw[i][j] += b * (a * rstd);
+        dx[j] += rstd * (b[j] * w[j]) - a[j] * c;
+        dw[i][j] += b[j] * (a[j] * rstd);
       }
       if (col < p.D) store_vec<T, V>(static_cast<T*>(p.dx) + row * p.D + col, dx);
     }
+    if (++slot == p.ring.slots) slot = 0, phase ^= 1u;
   }
+  if constexpr (kRing) ring_abandon(&abort_flag);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int col = (i * threads + t) * V;
@@ -327,6 +461,29 @@ static int launch_norm(const NormParams& p, cudaStream_t st) {
                   "rms_norm launch");
 }
 
+// The ring form, when a ring of at least two rows for each CTA of an SM fits; -2: it does not.
+template <class T, int V, int kMode>
+static int launch_norm_ring(const NormParams& p, cudaStream_t st) {
+  constexpr int VPT = 2;
+  const int vecs = p.D / V, threads = ((vecs + VPT - 1) / VPT + 31) / 32 * 32;
+  if (vecs < 128 || threads > 512) return -2;
+  const int per_sm = 1024 / threads < 4 ? 1024 / threads : 4;
+  NormRing ring;
+  ring.row_bytes = p.D * static_cast<int>(sizeof(T));
+  const int slot = ring.row_bytes * (p.res != nullptr ? 2 : 1);
+  ring.slots = NORM_RING_BYTES / per_sm / slot;
+  if (ring.slots > NORM_SLOTS) ring.slots = NORM_SLOTS;
+  if (ring.slots < 2) return -2;
+  const long long most = static_cast<long long>(norm_sms()) * per_sm;
+  static std::atomic<uint64_t> smem_done{0};
+  auto kernel = rms_norm_ring_kernel<T, V, VPT, kMode>;
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), NORM_RING_BYTES, smem_done);
+  if (e == cudaSuccess)
+    e = launch_pdl(kernel, dim3(static_cast<unsigned>(p.rows < most ? p.rows : most)),
+                   dim3(static_cast<unsigned>(threads)), static_cast<size_t>(slot) * ring.slots, st, p, ring);
+  return launched(e, "rms_norm launch");
+}
+
 // Vectors per thread: rows that are too few to fill the chip are spread over as many threads as they have vectors.
 template <class T, int V, int kMode>
 static int pick_norm(const NormParams& p, cudaStream_t st) {
@@ -334,6 +491,10 @@ static int pick_norm(const NormParams& p, cudaStream_t st) {
   const bool few = p.rows <= 2 * norm_sms();
   if (few && vecs <= 1024) return launch_norm<T, V, 1, kMode>(p, st);
   if (few && vecs <= 2048) return launch_norm<T, V, 2, kMode>(p, st);
+  if constexpr (V * sizeof(T) == 16) {
+    const int rc = few ? -2 : launch_norm_ring<T, V, kMode>(p, st);
+    if (rc != -2) return rc;
+  }
   if (vecs <= 2048) return launch_norm<T, V, 4, kMode>(p, st);
   if (vecs <= 4096) return launch_norm<T, V, 8, kMode>(p, st);
   if constexpr (V < 4) {
@@ -364,10 +525,22 @@ static int norm_typed(const NormParams& p, cudaStream_t st) {
 template <class T, int V, int VPT>
 static int launch_bwd(const NormBwdParams& p0, float* dw, int grid, int threads, cudaStream_t st) {
   NormBwdParams p = p0;
-  if (launched(launch_pdl(rms_norm_bwd_kernel<T, V, VPT>, dim3(static_cast<unsigned>(grid)),
-                          dim3(static_cast<unsigned>(threads)), 0, st, p),
-               "rms_norm_backward launch"))
-    return -1;
+  const dim3 g(static_cast<unsigned>(grid)), b(static_cast<unsigned>(threads));
+  cudaError_t e = cudaErrorUnknown;
+  if constexpr (VPT == 1 && V * sizeof(T) == 16) {
+    const int per_sm = 1024 / threads < 4 ? 1024 / threads : 4;
+    p.ring.row_bytes = p.D * static_cast<int>(sizeof(T));
+    const int slot = p.ring.row_bytes * (p.dh != nullptr ? 3 : 2);
+    p.ring.slots = NORM_RING_BYTES / per_sm / slot;
+    if (p.ring.slots > NORM_SLOTS) p.ring.slots = NORM_SLOTS;
+    static std::atomic<uint64_t> smem_done{0};
+    auto kernel = rms_norm_bwd_kernel<T, V, VPT, true>;
+    e = allow_smem(reinterpret_cast<const void*>(kernel), NORM_RING_BYTES, smem_done);
+    if (e == cudaSuccess) e = launch_pdl(kernel, g, b, static_cast<size_t>(slot) * p.ring.slots, st, p);
+  } else {
+    e = launch_pdl(rms_norm_bwd_kernel<T, V, VPT, false>, g, b, 0, st, p);
+  }
+  if (launched(e, "rms_norm_backward launch")) return -1;
   return launched(launch_pdl(rms_norm_dw_kernel, dim3(static_cast<unsigned>((p.D + 31) / 32)), dim3(1024), 0, st,
                              static_cast<const float*>(p.part), dw, grid, p.D),
                   "rms_norm_backward launch");
@@ -389,7 +562,7 @@ static BwdShape bwd_shape(const NormBwdParams& p, int E) {
   if (s.VPT == 0) return s;
   s.threads = ((vecs + s.VPT - 1) / s.VPT + 31) / 32 * 32;
   int per_sm = 1024 / s.threads;
-  if (per_sm > 8) per_sm = 8;
+  if (per_sm > 4) per_sm = 4;
   const long long most = static_cast<long long>(norm_sms()) * per_sm;
   s.grid = static_cast<int>(p.rows < most ? p.rows : most);
   return s;
@@ -420,6 +593,7 @@ static NormBwdParams bwd_params(const void* dy, const void* h, const void* w, co
                                 long long dy_stride, long long h_stride, long long dh_stride, long long rows, int D,
                                 int w_f32, float eps) {
   NormBwdParams p;
+  p.ring = {0, 0};
   p.dy = dy;
   p.h = h;
   p.w = w;
@@ -433,6 +607,7 @@ static NormBwdParams bwd_params(const void* dy, const void* h, const void* w, co
   p.D = D;
   p.w_f32 = w_f32;
   p.eps = eps;
+  p.status = nullptr;
   return p;
 }
 
@@ -446,7 +621,7 @@ extern "C" {
 // Strides in elements; y, h, scale and sf are dense.  sf: ceil(D / 512) x rows 32-bit words.
 int cb_rms_norm(const void* x, const void* res, const void* w, void* y, void* h, void* scale, void* sf,
                 long long x_stride, long long res_stride, long long rows, int D, int type, int w_f32, int mode,
-                float eps, void* stream) {
+                float eps, void* status, void* stream) {
   if (rows < 0 || rows > 0x7fffffffll || D < 1 || type < 0 || type > 2 || mode < 0 || mode > 2 ||
       (mode != 0 && D % 128 != 0) || (res != nullptr && h == nullptr) || (mode != 0 && scale == nullptr)) {
     set_last_error("rms_norm: bad shape or type (8 bits: D a multiple of 128)");
@@ -467,6 +642,7 @@ int cb_rms_norm(const void* x, const void* res, const void* w, void* y, void* h,
   p.D = D;
   p.w_f32 = w_f32;
   p.eps = eps;
+  p.status = static_cast<uint32_t*>(status);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (type * 3 + mode) {
     case 0: return norm_typed<__nv_bfloat16, NORM_PLAIN>(p, st);
@@ -501,11 +677,12 @@ long long cb_rms_norm_backward_floats(const void* dy, const void* h, const void*
 
 int cb_rms_norm_backward(const void* dy, const void* h, const void* w, const void* dh, void* dx, void* dw, void* part,
                          long long dy_stride, long long h_stride, long long dh_stride, long long rows, int D, int type,
-                         int w_f32, float eps, void* stream) {
+                         int w_f32, float eps, void* status, void* stream) {
   if (cb_rms_norm_backward_floats(dy, h, w, dh, dx, dy_stride, h_stride, dh_stride, rows, D, type, w_f32) < 0)
     return -1;
   NormBwdParams p = bwd_params(dy, h, w, dh, dx, dy_stride, h_stride, dh_stride, rows, D, w_f32, eps);
   p.part = static_cast<float*>(part);
+  p.status = static_cast<uint32_t*>(status);
   const BwdShape s = bwd_shape(p, type == 2 ? 4 : 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* out = static_cast<float*>(dw);

@@ -21,22 +21,84 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 
-// V consecutive elements, aligned to their size together.
+// V consecutive elements, aligned to their size together: as 32-bit words while they wait (an array of 16-bit
+// elements takes a register each), as fp32 for arithmetic.
+template <class T, int V, bool kWords = (sizeof(T) * V >= 4)>
+struct Vec;
 template <class T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T e[V];
+struct alignas(sizeof(T) * V) Vec<T, V, true> {
+  uint32_t w[sizeof(T) * V / 4];
 };
 template <class T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
-  const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p);
+struct alignas(sizeof(T) * V) Vec<T, V, false> {
+  T e[V];
+};
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (__is_same(T, __nv_bfloat16))
+      return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else
+      return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  } else {
+    return make_float2(0.f, 0.f);
+  }
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (__is_same(T, __nv_bfloat16)) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void unpack(const Vec<T, V>& v, float (&x)[V]) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = to_f32(v.e[i]);
+    for (int i = 0; i < V; ++i) x[i] = __uint_as_float(v.w[i]);
+  } else if constexpr (V == 1) {
+    x[0] = to_f32(v.e[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 f = unpack2<T>(v.w[i / 2]);
+      x[i] = f.x;
+      x[i + 1] = f.y;
+    }
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void pack(const float (&x)[V], Vec<T, V>& v) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.w[i] = __float_as_uint(x[i]);
+  } else if constexpr (V == 1) {
+    v.e[0] = from_f32<T>(x[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) v.w[i / 2] = pack2<T>(x[i], x[i + 1]);
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void clear(Vec<T, V>& v) {
+  if constexpr (sizeof(T) * V >= 4) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) * V / 4; ++i) v.w[i] = 0u;
+  } else {
+    v.e[0] = from_f32<T>(0.f);
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
+  unpack(*reinterpret_cast<const Vec<T, V>*>(p), x);
 }
 template <class T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
   Vec<T, V> v;
-#pragma unroll
-  for (int i = 0; i < V; ++i) v.e[i] = from_f32<T>(x[i]);
+  pack(x, v);
   *reinterpret_cast<Vec<T, V>*>(p) = v;
 }
 

@@ -33,6 +33,37 @@ using SplitBytesFn = long long (*)(int, int, int, int, int, int, int, int);
 using SplitFn = int (*)(const void*, const void*, const void*, void*, void*, int, int, int, int, int, int, int,
                         int, float, void*, long long, void*, void*);
 
+using NormFn = int (*)(const void*, const void*, const void*, void*, void*, void*, void*, long long, long long,
+                       long long, int, int, int, int, float, void*, void*);
+using NormBwdFloatsFn = long long (*)(const void*, const void*, const void*, const void*, const void*, long long,
+                                      long long, long long, long long, int, int, int);
+using NormBwdFn = int (*)(const void*, const void*, const void*, const void*, void*, void*, void*, long long,
+                          long long, long long, long long, int, int, int, float, void*, void*);
+using RopeFn = int (*)(const void*, void*, long long, long long, long long, int, const void*, void*, long long,
+                       long long, long long, int, int, int, int, const void*, const void*, int, int, int,
+                       const void*, int, int, int, int, void*, void*);
+using KvAppendFn = int (*)(void*, void*, int, int, int, const void*, const void*, const long long*, const void*, int,
+                           const void*, const void*, int, int, const void*, void*, int, const void*, const void*,
+                           int, int, int, void*, void*);
+using KvReadFn = int (*)(const void*, const void*, int, int, int, const void*, int, const void*, const void*, int, int,
+                         void*, void*, void*, void*);
+using KvBytesFn = long long (*)(int, int, int, int, int);
+using KvAttendFn = int (*)(void*, void*, int, int, int, const void*, long long, long long, long long, void*, void*,
+                           const void*, int, const void*, const void*, int, int, int, int, int, int, float, void*,
+                           long long, void*, void*);
+using KvPrefillFn = int (*)(void*, void*, int, int, int, const void*, long long, long long, void*, void*, const void*,
+                            int, const void*, const void*, int, int, int, int, int, int, float, void*, long long,
+                            void*, void*);
+
+NormFn g_norm;
+NormBwdFloatsFn g_norm_bwd_floats;
+NormBwdFn g_norm_bwd;
+RopeFn g_rope;
+KvAppendFn g_kv_append;
+KvReadFn g_kv_read;
+KvBytesFn g_kv_attend_bytes, g_kv_prefill_bytes;
+KvAttendFn g_kv_attend;
+KvPrefillFn g_kv_prefill;
 GemmFn g_gemm_bf16, g_gemm_fp8;
 ScaledGemmFn g_gemm_bs;
 MxGemmFn g_gemm_mx;
@@ -47,8 +78,8 @@ struct NoGil {
   ~NoGil() { PyEval_RestoreThread(s); }
 };
 
-// A plain CUDA tensor that nothing wraps or intercepts, contiguous and 16-byte aligned.
-const at::Tensor* plain(PyObject* o) {
+// A plain CUDA tensor that nothing wraps or intercepts.
+const at::Tensor* bare(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   const auto* impl = t.unsafeGetTensorImpl();
@@ -58,9 +89,14 @@ const at::Tensor* plain(PyObject* o) {
       ks.has(c10::DispatchKey::Functionalize) || ks.has(c10::DispatchKey::Negative) ||
       ks.has(c10::DispatchKey::Conjugate) || ks.has(c10::DispatchKey::ZeroTensor))
     return nullptr;
-  if (!t.is_contiguous() || !t.has_storage() || (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) != 0)
+  return t.has_storage() ? &t : nullptr;
+}
+// The same, contiguous and 16-byte aligned.
+const at::Tensor* plain(PyObject* o) {
+  const at::Tensor* t = bare(o);
+  if (t == nullptr || !t->is_contiguous() || (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15u) != 0)
     return nullptr;
-  return &t;
+  return t;
 }
 bool modes_off() {
   return !c10::impl::TorchDispatchModeTLS::any_modes_set() && !at::impl::torch_function_mode_enabled();
@@ -292,6 +328,318 @@ PyObject* fast_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
   CB_END
 }
 
+// ------------------------------------------------------------------ norm, rotary positions, the 8-bit cache
+// Their operands may be strided; all of them are on the current device.
+bool here(const at::Tensor* t) { return t != nullptr && t->get_device() == c10::cuda::current_device(); }
+int elem_type(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1; }
+// Rows [rows, D] with dense elements.
+const at::Tensor* rows_of(PyObject* o, const at::Tensor* like) {
+  const at::Tensor* t = bare(o);
+  if (!here(t) || t->dim() != 2 || elem_type(t->scalar_type()) < 0 || t->size(0) < 1 || t->size(1) < 1 ||
+      !fits(t->size(0)) || !fits(t->size(1)) || t->stride(1) != 1)
+    return nullptr;
+  if (like != nullptr && (t->sizes() != like->sizes() || t->scalar_type() != like->scalar_type())) return nullptr;
+  return t;
+}
+const at::Tensor* weight_of(PyObject* o, const at::Tensor& x, int* f32) {
+  const at::Tensor* w = bare(o);
+  if (!here(w) || w->dim() != 1 || w->size(0) != x.size(1) || !w->is_contiguous()) return nullptr;
+  *f32 = w->scalar_type() == at::kFloat ? 1 : 0;
+  return *f32 || w->scalar_type() == x.scalar_type() ? w : nullptr;
+}
+PyObject* tuple_of(std::initializer_list<const at::Tensor*> ts) {
+  PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+  if (t == nullptr) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor* x : ts) {
+    if (x->defined()) {
+      PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(*x));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(t, i++, Py_None);
+    }
+  }
+  return t;
+}
+
+// rms_norm(x, weight, residual | None, eps, mode, status_ptr): (y, scales | None, sf | None, h | None)
+PyObject* fast_rms_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  CB_TRY
+  float eps;
+  int mode, w_f32;
+  void* status;
+  if (n != 6 || !modes_off() || !as_float(v[3], &eps) || !as_int(v[4], &mode) || !as_ptr(v[5], &status))
+    Py_RETURN_NONE;
+  const at::Tensor* x = rows_of(v[0], nullptr);
+  if (x == nullptr) Py_RETURN_NONE;
+  const at::Tensor* w = weight_of(v[1], *x, &w_f32);
+  const at::Tensor* res = v[2] == Py_None ? nullptr : rows_of(v[2], x);
+  const int64_t rows = x->size(0), D = x->size(1);
+  if (w == nullptr || (res == nullptr && v[2] != Py_None) || (mode != 0 && D % 128 != 0)) Py_RETURN_NONE;
+  at::Tensor y, s, sf, h;
+  int rc;
+  {
+    NoGil g;
+    y = empty(*x, {rows, D}, mode != 0 ? at::kFloat8_e4m3fn : x->scalar_type());
+    if (res != nullptr) h = empty(*x, {rows, D}, x->scalar_type());
+    if (mode != 0) s = empty(*x, {rows, D / 128}, at::kFloat);
+    if (mode == 2) sf = empty(*x, {(D / 128 + 3) / 4, rows}, at::kInt);
+    rc = g_norm(x->const_data_ptr(), res != nullptr ? res->const_data_ptr() : nullptr, w->const_data_ptr(),
+                y.mutable_data_ptr(), res != nullptr ? h.mutable_data_ptr() : nullptr,
+                mode != 0 ? s.mutable_data_ptr() : nullptr, mode == 2 ? sf.mutable_data_ptr() : nullptr, x->stride(0),
+                res != nullptr ? res->stride(0) : 0, rows, static_cast<int>(D), elem_type(x->scalar_type()), w_f32,
+                mode, eps, status, current_stream());
+  }
+  if (rc == 0) return tuple_of({&y, &s, &sf, &h});
+  CB_END
+}
+
+// rms_norm_backward(dy, h, weight, dh | None, eps, status_ptr): (dx, dw)
+PyObject* fast_rms_norm_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  CB_TRY
+  float eps;
+  int w_f32;
+  void* status;
+  if (n != 6 || !modes_off() || !as_float(v[4], &eps) || !as_ptr(v[5], &status)) Py_RETURN_NONE;
+  const at::Tensor* h = rows_of(v[1], nullptr);
+  if (h == nullptr) Py_RETURN_NONE;
+  const at::Tensor *dy = rows_of(v[0], h), *w = weight_of(v[2], *h, &w_f32);
+  const at::Tensor* dh = v[3] == Py_None ? nullptr : rows_of(v[3], h);
+  if (dy == nullptr || w == nullptr || (dh == nullptr && v[3] != Py_None)) Py_RETURN_NONE;
+  const int64_t rows = h->size(0), D = h->size(1);
+  const int type = elem_type(h->scalar_type()), d = static_cast<int>(D);
+  const void* dhp = dh != nullptr ? dh->const_data_ptr() : nullptr;
+  const long long dhs = dh != nullptr ? dh->stride(0) : 0;
+  at::Tensor dx, dw;
+  int rc = -1;
+  {
+    NoGil g;
+    dx = empty(*h, {rows, D}, h->scalar_type());
+    dw = empty(*h, {D}, at::kFloat);
+    const long long floats = g_norm_bwd_floats(dy->const_data_ptr(), h->const_data_ptr(), w->const_data_ptr(), dhp,
+                                               dx.const_data_ptr(), dy->stride(0), h->stride(0), dhs, rows, d, type,
+                                               w_f32);
+    if (floats > 0) {
+      at::Tensor part = empty(*h, {floats}, at::kFloat);
+      rc = g_norm_bwd(dy->const_data_ptr(), h->const_data_ptr(), w->const_data_ptr(), dhp, dx.mutable_data_ptr(),
+                      dw.mutable_data_ptr(), part.mutable_data_ptr(), dy->stride(0), h->stride(0), dhs, rows, d, type,
+                      w_f32, eps, status, current_stream());
+    }
+  }
+  if (rc == 0) return tuple_of({&dx, &dw});
+  CB_END
+}
+
+// rope(x0, x1 | None, positions, cos, sin, interleaved, inverse, status_ptr): (y0, y1 | None)
+PyObject* fast_rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  CB_TRY
+  void* status;
+  if (n != 8 || !modes_off() || !PyBool_Check(v[5]) || !PyBool_Check(v[6]) || !as_ptr(v[7], &status)) Py_RETURN_NONE;
+  const at::Tensor *x[2] = {bare(v[0]), v[1] == Py_None ? nullptr : bare(v[1])}, *pos = bare(v[2]);
+  const at::Tensor *cos = bare(v[3]), *sin = bare(v[4]);
+  if (!here(x[0]) || (v[1] != Py_None && !here(x[1])) || !here(pos) || !here(cos) || !here(sin)) Py_RETURN_NONE;
+  if (x[0]->dim() != 4 || cos->dim() != 2 || !cos->is_contiguous() || cos->scalar_type() != at::kFloat ||
+      sin->sizes() != cos->sizes() || !sin->is_contiguous() || sin->scalar_type() != at::kFloat)
+    Py_RETURN_NONE;
+  const int64_t B = x[0]->size(0), S = x[0]->size(1), D = x[0]->size(3), rot = 2 * cos->size(1);
+  const int type = elem_type(x[0]->scalar_type());
+  if (type < 0 || !fits(B) || !fits(S) || !fits(D) || rot < 2 || rot > D || !fits(cos->size(0))) Py_RETURN_NONE;
+  for (const at::Tensor* t : x)
+    if (t != nullptr && (t->dim() != 4 || t->scalar_type() != x[0]->scalar_type() || t->size(0) != B ||
+                         t->size(1) != S || t->size(3) != D || !fits(t->size(2)) || t->stride(3) != 1))
+      Py_RETURN_NONE;
+  const bool i64 = pos->scalar_type() == at::kLong;
+  const bool batched = pos->dim() == 2;
+  if ((!i64 && pos->scalar_type() != at::kInt) || !pos->is_contiguous() ||
+      !(batched ? pos->size(0) == B && pos->size(1) == S : pos->dim() == 1 && pos->size(0) == S))
+    Py_RETURN_NONE;
+  at::Tensor y[2];
+  int rc;
+  {
+    NoGil g;
+    for (int i = 0; i < 2; ++i)
+      if (x[i] != nullptr) y[i] = empty(*x[i], x[i]->sizes(), x[i]->scalar_type());
+    const at::Tensor* b = x[1];
+    rc = g_rope(x[0]->const_data_ptr(), y[0].mutable_data_ptr(), x[0]->stride(0), x[0]->stride(1), x[0]->stride(2),
+                static_cast<int>(x[0]->size(2)), b != nullptr ? b->const_data_ptr() : nullptr,
+                b != nullptr ? y[1].mutable_data_ptr() : nullptr, b != nullptr ? b->stride(0) : 0,
+                b != nullptr ? b->stride(1) : 0, b != nullptr ? b->stride(2) : 0,
+                b != nullptr ? static_cast<int>(b->size(2)) : 0, static_cast<int>(B), static_cast<int>(S),
+                static_cast<int>(D), cos->const_data_ptr(), sin->const_data_ptr(), static_cast<int>(cos->size(0)),
+                static_cast<int>(rot), v[5] == Py_True ? 1 : 0, pos->const_data_ptr(), i64 ? 1 : 0, batched ? 1 : 0,
+                v[6] == Py_True ? 1 : 0, type, status, current_stream());
+  }
+  if (rc == 0) return tuple_of({&y[0], &y[1]});
+  CB_END
+}
+
+// The cache's tensors and shape: (data, exps, num_pages, kv_heads, page) at v[0].
+struct CacheArgs {
+  const at::Tensor *data, *exps;
+  int num_pages, hkv, page;
+};
+bool cache_of(PyObject* const* v, CacheArgs* c) {
+  c->data = plain(v[0]);
+  c->exps = plain(v[1]);
+  return here(c->data) && here(c->exps) && as_int(v[2], &c->num_pages) && as_int(v[3], &c->hkv) &&
+         as_int(v[4], &c->page) && c->page >= 16 && c->page <= 128 && c->data->scalar_type() == at::kByte &&
+         c->exps->scalar_type() == at::kChar &&
+         c->data->numel() == 2ll * c->num_pages * c->hkv * c->page * 128 &&
+         c->exps->numel() == 2ll * c->num_pages * c->hkv;
+}
+const at::Tensor* table_of(PyObject* o) {
+  const at::Tensor* t = bare(o);
+  return here(t) && t->dim() == 2 && t->scalar_type() == at::kInt && t->is_contiguous() && fits(t->size(0)) &&
+                 fits(t->size(1))
+             ? t
+             : nullptr;
+}
+// An int32 vector of B elements, or None where that is allowed.
+bool vector_of(PyObject* o, int64_t B, bool optional, const void** p) {
+  *p = nullptr;
+  if (o == Py_None) return optional;
+  const at::Tensor* t = bare(o);
+  if (!here(t) || t->dim() != 1 || t->size(0) != B || t->scalar_type() != at::kInt || !t->is_contiguous()) return false;
+  *p = t->const_data_ptr();
+  return true;
+}
+// [B, S, heads, 128] bf16 with dense rows of 8-byte alignment.
+const at::Tensor* heads_of(PyObject* o) {
+  const at::Tensor* t = bare(o);
+  if (!here(t) || t->dim() != 4 || t->scalar_type() != at::kBFloat16 || t->size(3) != 128 || t->stride(3) != 1 ||
+      (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 7u) != 0)
+    return nullptr;
+  for (int i = 0; i < 3; ++i)
+    if (t->stride(i) % 4 != 0 || !fits(t->size(i))) return nullptr;
+  return t;
+}
+
+// kv_append(data, exps, num_pages, kv_heads, page, k, v, pages, start, count | None, cos | None, sin | None,
+// interleaved, q | None, status_ptr): (turned q | None,)
+PyObject* fast_kv_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  CB_TRY
+  CacheArgs c;
+  void* status;
+  const void *start, *count;
+  if (n != 15 || !modes_off() || !cache_of(v, &c) || !PyBool_Check(v[12]) || !as_ptr(v[14], &status)) Py_RETURN_NONE;
+  const at::Tensor *k = heads_of(v[5]), *val = heads_of(v[6]), *pages = table_of(v[7]);
+  const at::Tensor *cos = v[10] == Py_None ? nullptr : bare(v[10]), *sin = v[11] == Py_None ? nullptr : bare(v[11]);
+  const at::Tensor* q = v[13] == Py_None ? nullptr : heads_of(v[13]);
+  if (k == nullptr || val == nullptr || pages == nullptr || k->sizes() != val->sizes() || k->size(2) != c.hkv ||
+      pages->size(0) != k->size(0) || (q == nullptr && v[13] != Py_None) || (q != nullptr && cos == nullptr) ||
+      (v[10] == Py_None) != (v[11] == Py_None))
+    Py_RETURN_NONE;
+  const int64_t B = k->size(0), S = k->size(1);
+  if (!vector_of(v[8], B, false, &start) || !vector_of(v[9], B, true, &count)) Py_RETURN_NONE;
+  if (q != nullptr && (q->size(0) != B || q->size(1) != S)) Py_RETURN_NONE;
+  int rot = 0, positions = 0;
+  if (v[10] != Py_None) {
+    if (!here(cos) || !here(sin) || cos->dim() != 2 || cos->scalar_type() != at::kFloat || !cos->is_contiguous() ||
+        sin->sizes() != cos->sizes() || sin->scalar_type() != at::kFloat || !sin->is_contiguous() ||
+        !fits(cos->size(0)) || cos->size(1) > 64 || cos->size(1) % 4 != 0)
+      Py_RETURN_NONE;
+    rot = static_cast<int>(2 * cos->size(1));
+    positions = static_cast<int>(cos->size(0));
+  }
+  long long st[9] = {k->stride(0), k->stride(1), k->stride(2), val->stride(0), val->stride(1), val->stride(2), 0, 0, 0};
+  at::Tensor out;
+  int rc;
+  {
+    NoGil g;
+    if (q != nullptr) {
+      for (int i = 0; i < 3; ++i) st[6 + i] = q->stride(i);
+      out = empty(*q, q->sizes(), at::kBFloat16);
+    }
+    rc = g_kv_append(c.data->mutable_data_ptr(), c.exps->mutable_data_ptr(), c.num_pages, c.hkv, c.page,
+                     k->const_data_ptr(), val->const_data_ptr(), st, pages->const_data_ptr(),
+                     static_cast<int>(pages->size(1)), start, count, static_cast<int>(B), static_cast<int>(S),
+                     q != nullptr ? q->const_data_ptr() : nullptr, q != nullptr ? out.mutable_data_ptr() : nullptr,
+                     q != nullptr ? static_cast<int>(q->size(2)) : 0, rot > 0 ? cos->const_data_ptr() : nullptr,
+                     rot > 0 ? sin->const_data_ptr() : nullptr, positions, rot, v[12] == Py_True ? 1 : 0, status,
+                     current_stream());
+  }
+  if (rc == 0) return tuple_of({&out});
+  CB_END
+}
+
+// kv_read(data, exps, num_pages, kv_heads, page, pages, begin | None, n, length | None, status_ptr): (k, v)
+PyObject* fast_kv_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  CB_TRY
+  CacheArgs c;
+  void* status;
+  int tokens;
+  const void *begin, *length;
+  if (n != 10 || !modes_off() || !cache_of(v, &c) || !as_int(v[7], &tokens) || tokens < 1 || !as_ptr(v[9], &status))
+    Py_RETURN_NONE;
+  const at::Tensor* pages = table_of(v[5]);
+  if (pages == nullptr) Py_RETURN_NONE;
+  const int64_t B = pages->size(0);
+  if (!vector_of(v[6], B, true, &begin) || !vector_of(v[8], B, true, &length)) Py_RETURN_NONE;
+  at::Tensor k, val;
+  int rc;
+  {
+    NoGil g;
+    k = empty(*c.data, {B, tokens, c.hkv, 128}, at::kBFloat16);
+    val = empty(*c.data, {B, tokens, c.hkv, 128}, at::kBFloat16);
+    rc = g_kv_read(c.data->const_data_ptr(), c.exps->const_data_ptr(), c.num_pages, c.hkv, c.page,
+                   pages->const_data_ptr(), static_cast<int>(pages->size(1)), begin, length, static_cast<int>(B),
+                   tokens, k.mutable_data_ptr(), val.mutable_data_ptr(), status, current_stream());
+  }
+  if (rc == 0) return tuple_of({&k, &val});
+  CB_END
+}
+
+// kv_attend(data, exps, num_pages, kv_heads, page, q, pages, start, count | None, window, sinks, scale | None,
+// max_len, long, status_ptr): (o, lse).  long: the form for many query rows, which wants 16-byte rows and sequences
+// that follow each other.
+PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  CB_TRY
+  CacheArgs c;
+  void* status;
+  int window, sinks, max_len;
+  float scale;
+  const void *start, *count;
+  if (n != 15 || !modes_off() || !cache_of(v, &c) || !as_int(v[9], &window) || !as_int(v[10], &sinks) ||
+      window < 0 || sinks < 0 || !as_int(v[12], &max_len) || !PyBool_Check(v[13]) || !as_ptr(v[14], &status))
+    Py_RETURN_NONE;
+  if (v[11] == Py_None) scale = static_cast<float>(1.0 / std::sqrt(128.0));
+  else if (!as_float(v[11], &scale)) Py_RETURN_NONE;
+  const at::Tensor *q = heads_of(v[5]), *pages = table_of(v[6]);
+  if (q == nullptr || pages == nullptr || pages->size(0) != q->size(0) || q->size(2) % c.hkv != 0) Py_RETURN_NONE;
+  const int64_t B = q->size(0), S = q->size(1), Hq = q->size(2);
+  if (!vector_of(v[7], B, false, &start) || !vector_of(v[8], B, true, &count)) Py_RETURN_NONE;
+  const bool tall = v[13] == Py_True;
+  if (tall && ((reinterpret_cast<uintptr_t>(q->const_data_ptr()) & 15u) != 0 || q->stride(1) % 8 != 0 ||
+               q->stride(2) % 8 != 0 || q->stride(1) <= 0 || q->stride(2) <= 0 ||
+               (B > 1 && q->stride(0) != S * q->stride(1))))
+    Py_RETURN_NONE;
+  const int b = static_cast<int>(B), s = static_cast<int>(S), hq = static_cast<int>(Hq),
+            cols = static_cast<int>(pages->size(1));
+  at::Tensor o, lse;
+  int rc = -1;
+  {
+    NoGil g;
+    const long long bytes = (tall ? g_kv_prefill_bytes : g_kv_attend_bytes)(b, s, hq, c.hkv, max_len);
+    if (bytes > 0) {
+      o = empty(*q, q->sizes(), at::kBFloat16);
+      lse = empty(*q, {B, Hq, S}, at::kFloat);
+      at::Tensor ws = empty(*q, {bytes}, at::kByte);
+      if (tall)
+        rc = g_kv_prefill(c.data->mutable_data_ptr(), c.exps->mutable_data_ptr(), c.num_pages, c.hkv, c.page,
+                          q->const_data_ptr(), q->stride(1), q->stride(2), o.mutable_data_ptr(),
+                          lse.mutable_data_ptr(), pages->const_data_ptr(), cols, start, count, b, s, hq, window, sinks,
+                          max_len, scale, ws.mutable_data_ptr(), bytes, status, current_stream());
+      else
+        rc = g_kv_attend(c.data->mutable_data_ptr(), c.exps->mutable_data_ptr(), c.num_pages, c.hkv, c.page,
+                         q->const_data_ptr(), q->stride(0), q->stride(1), q->stride(2), o.mutable_data_ptr(),
+                         lse.mutable_data_ptr(), pages->const_data_ptr(), cols, start, count, b, s, hq, window, sinks,
+                         max_len, scale, ws.mutable_data_ptr(), bytes, status, current_stream());
+    }
+  }
+  if (rc == 0) return tuple_of({&o, &lse});
+  CB_END
+}
+
 // bind({name: address}): the C entry points, from the loaded library.
 PyObject* fast_bind(PyObject*, PyObject* d) {
   const auto get = [&](const char* name) -> void* {
@@ -307,8 +655,19 @@ PyObject* fast_bind(PyObject*, PyObject* d) {
   g_attn = reinterpret_cast<AttnFn>(get("cb_attn_fwd4"));
   g_split_bytes = reinterpret_cast<SplitBytesFn>(get("cb_attn_split_bytes"));
   g_split = reinterpret_cast<SplitFn>(get("cb_attn_split"));
+  g_norm = reinterpret_cast<NormFn>(get("cb_rms_norm"));
+  g_norm_bwd_floats = reinterpret_cast<NormBwdFloatsFn>(get("cb_rms_norm_backward_floats"));
+  g_norm_bwd = reinterpret_cast<NormBwdFn>(get("cb_rms_norm_backward"));
+  g_rope = reinterpret_cast<RopeFn>(get("cb_rope"));
+  g_kv_append = reinterpret_cast<KvAppendFn>(get("cb_kv_append"));
+  g_kv_read = reinterpret_cast<KvReadFn>(get("cb_kv_read"));
+  g_kv_attend_bytes = reinterpret_cast<KvBytesFn>(get("cb_kv_attend_bytes"));
+  g_kv_prefill_bytes = reinterpret_cast<KvBytesFn>(get("cb_kv_prefill_bytes"));
+  g_kv_attend = reinterpret_cast<KvAttendFn>(get("cb_kv_attend"));
+  g_kv_prefill = reinterpret_cast<KvPrefillFn>(get("cb_kv_prefill"));
   if (PyErr_Occurred()) return nullptr;
-  if (!g_gemm_bf16 || !g_gemm_fp8 || !g_gemm_bs || !g_gemm_mx || !g_quant || !g_quant_pow2 || !g_attn ||
+  if (!g_norm || !g_norm_bwd_floats || !g_norm_bwd || !g_rope || !g_kv_append || !g_kv_read || !g_kv_attend_bytes ||
+      !g_kv_prefill_bytes || !g_kv_attend || !g_kv_prefill || !g_gemm_bf16 || !g_gemm_fp8 || !g_gemm_bs || !g_gemm_mx || !g_quant || !g_quant_pow2 || !g_attn ||
       !g_split_bytes || !g_split) {
     PyErr_SetString(PyExc_RuntimeError, "fast_ops.bind: an entry point is missing");
     return nullptr;
@@ -329,6 +688,13 @@ PyMethodDef methods[] = {
     {"quantize_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_quantize_rows)), METH_FASTCALL,
      nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_attention)), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_rms_norm)), METH_FASTCALL, nullptr},
+    {"rms_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_rms_norm_backward)),
+     METH_FASTCALL, nullptr},
+    {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_rope)), METH_FASTCALL, nullptr},
+    {"kv_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_kv_append)), METH_FASTCALL, nullptr},
+    {"kv_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_kv_read)), METH_FASTCALL, nullptr},
+    {"kv_attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fast_kv_attend)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

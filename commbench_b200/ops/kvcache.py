@@ -90,6 +90,12 @@ class KVCache8:
         fp32.  ``q`` [B, S, Hq, 128] is turned by the same launch and returned (zeros for tokens that do not
         exist).  Where a page id is out of range nothing is written; a position beyond the table gives NaN.  With
         ``status_ptr`` either leaves a status word."""
+        if stream is None:
+            r = N.fast().kv_append(self.data, self.exps, self.num_pages, self.kv_heads, self.page, k, v, pages, start,
+                                   count, None if rope is None else rope.cos, None if rope is None else rope.sin,
+                                   rope is not None and rope.interleaved, q, status_ptr)
+            if r is not None:
+                return r[0]
         _heads(k, "k", self.kv_heads)
         _heads(v, "v", self.kv_heads, k.shape[:2])
         B, S = k.shape[:2]
@@ -123,6 +129,11 @@ class KVCache8:
     def read(self, pages, begin, n: int, length=None, status_ptr: int = 0, stream=None):
         """``(k, v)`` bf16 [B, n, kv_heads, 128]: tokens ``begin[b] .. begin[b] + n - 1`` (``begin`` None: from 0)
         as the values that the cache holds; zeros before token 0 and from token ``length[b]`` on."""
+        if stream is None:
+            r = N.fast().kv_read(self.data, self.exps, self.num_pages, self.kv_heads, self.page, pages, begin, n,
+                                 length, status_ptr)
+            if r is not None:
+                return r
         if n < 0:
             raise CommError("n must not be negative")
         B = pages.shape[0]
@@ -154,6 +165,14 @@ class KVCache8:
 
         ``impl``: "decode" (few query rows, bound by the cache's bytes) or "prefill" (tcgen05 tiles over an expanded
         copy); by default the number of rows decides."""
+        if stream is None and impl is None and isinstance(q, torch.Tensor) and q.dim() == 4 and pages.dim() == 2:
+            room = pages.shape[1] * self.page
+            r = N.fast().kv_attend(self.data, self.exps, self.num_pages, self.kv_heads, self.page, q, pages, start,
+                                   count, window, sinks, scale,
+                                   room if max_len is None or max_len > room else max(max_len, 1),
+                                   q.shape[1] * (q.shape[2] // self.kv_heads) > _FEW_ROWS, status_ptr)
+            if r is not None:
+                return r
         _heads(q, "q")
         B, S, Hq, _ = q.shape
         if Hq % self.kv_heads:

@@ -40,7 +40,11 @@ def _new(stream, like, shape, dtype):
     return like.new_empty(shape, dtype=dtype) if stream is None else N.new_empty_on(stream, like, shape, dtype)
 
 
-def _forward(x, weight, residual, eps, mode, stream):
+def _forward(x, weight, residual, eps, mode, status_ptr, stream):
+    if stream is None:
+        r = N.fast().rms_norm(x, weight, residual, eps, mode, status_ptr)
+        if r is not None:
+            return r
     _rows(x, "x")
     w_f32 = _weight(weight, x)
     if residual is not None:
@@ -57,36 +61,41 @@ def _forward(x, weight, residual, eps, mode, stream):
             x.data_ptr(), residual.data_ptr() if residual is not None else 0, weight.data_ptr(), y.data_ptr(),
             h.data_ptr() if h is not None else 0, s.data_ptr() if mode else 0, sf.data_ptr() if mode == 2 else 0,
             x.stride(0), residual.stride(0) if residual is not None else 0, rows, d, _TYPES[x.dtype], w_f32, mode,
-            eps, N.raw_stream(stream))
+            eps, status_ptr, N.raw_stream(stream))
     if rc != 0:
         raise NormError(f"rms_norm failed: {N.last_error()}")
     return y, s, sf, h
 
 
 @traced("cb200.rms_norm")
-def rms_norm(x, weight, residual=None, eps: float = 1e-6, stream=None):
+def rms_norm(x, weight, residual=None, eps: float = 1e-6, status_ptr: int = 0, stream=None):
     """``y`` [rows, D] in x's type; with ``residual`` ``(y, h)``, ``h = x + residual`` rounded to x's type
     (``y`` is computed from the sum before that rounding)."""
-    y, _, _, h = _forward(x, weight, residual, eps, 0, stream)
+    y, _, _, h = _forward(x, weight, residual, eps, 0, status_ptr, stream)
     return y if residual is None else (y, h)
 
 
 @traced("cb200.rms_norm_quant")
-def rms_norm_quant(x, weight, residual=None, eps: float = 1e-6, pow2: bool = False, stream=None):
+def rms_norm_quant(x, weight, residual=None, eps: float = 1e-6, pow2: bool = False, status_ptr: int = 0,
+                   stream=None):
     """The normalised rows as e4m3 with one scale per row and 128 columns, rounded once from fp32.
 
     ``(q, scales, h)`` in the form of :func:`ops.gemm.quantize_blockscaled`, for ``gemm_fp8_blockscaled``; with
     ``pow2`` ``(q, scales, sf, h)`` as :func:`ops.gemm.quantize_blockscaled_pow2` gives them, for ``gemm_fp8_mx``.
     ``h`` is None without a residual."""
-    q, s, sf, h = _forward(x, weight, residual, eps, 2 if pow2 else 1, stream)
+    q, s, sf, h = _forward(x, weight, residual, eps, 2 if pow2 else 1, status_ptr, stream)
     return (q, s, sf, h) if pow2 else (q, s, h)
 
 
 @traced("cb200.rms_norm_backward")
-def rms_norm_backward(dy, h, weight, dh=None, eps: float = 1e-6, stream=None):
+def rms_norm_backward(dy, h, weight, dh=None, eps: float = 1e-6, status_ptr: int = 0, stream=None):
     """``(dx, dw)`` from the gradient ``dy`` of the normalised rows: ``h`` is what was normalised (x, or the sum
     that :func:`rms_norm` returned with it), ``dh`` the gradient that reaches that sum on its other way.  ``dx``
     is the gradient of x and of the residual alike; ``dw`` is fp32, summed in a fixed order."""
+    if stream is None:
+        r = N.fast().rms_norm_backward(dy, h, weight, dh, eps, status_ptr)
+        if r is not None:
+            return r
     _rows(h, "h")
     _rows(dy, "dy", h)
     if dh is not None:
@@ -107,7 +116,8 @@ def rms_norm_backward(dy, h, weight, dh=None, eps: float = 1e-6, stream=None):
             raise NormError(f"rms_norm_backward failed: {N.last_error()}")
         part = h.new_empty((n,), dtype=torch.float32) if stream is None else \
             N.new_empty_on(stream, h, (n,), torch.float32, handed_out=False)
-        rc = lib.cb_rms_norm_backward(*args, dw.data_ptr(), part.data_ptr(), *shape, eps, N.raw_stream(stream))
+        rc = lib.cb_rms_norm_backward(*args, dw.data_ptr(), part.data_ptr(), *shape, eps, status_ptr,
+                                      N.raw_stream(stream))
     if rc != 0:
         raise NormError(f"rms_norm_backward failed: {N.last_error()}")
     return dx, dw

@@ -79,6 +79,11 @@ def rope(x, positions, table: RopeTable, inverse: bool = False, out=None, status
 
     A position outside the table gives NaN and, with ``status_ptr``, a status word."""
     pair = isinstance(x, (tuple, list))
+    if stream is None and out is None and (not pair or len(x) == 2):
+        a, b = x if pair else (x, None)
+        r = N.fast().rope(a, b, positions, table.cos, table.sin, table.interleaved, inverse, status_ptr)
+        if r is not None:
+            return r if pair else r[0]
     xs = list(x) if pair else [x]
     if not 1 <= len(xs) <= 2:
         raise RopeError("one tensor or a pair")
