@@ -5,26 +5,29 @@
 //   j > p_i - window or j < sinks;   o_i = sum_j softmax(s_i)_j v_j;   lse_i = log sum_j exp(s_ij)
 //
 // What it has to read is the visible part of the cache, 256 bytes a token and head; 16 query rows a key/value head
-// want 4096 multiply-adds a token, an eighth of what the tensor cores of an SM do with mma.sync while those bytes
-// arrive.  So the tiles are small and every warp works by itself, without a barrier in the loop:
+// want 4096 multiply-adds a token, a third of what the tensor cores of an SM do with mma.sync (1024 a clock) while
+// those bytes arrive.  e4m3 becomes fp16 in registers, exactly, once for all products; scores and results are fp32,
+// probabilities fp16.  The scales never touch the data: the key scale is a factor on the score, and the value scale
+// 2^e is the term e in the exponent of the probability, which the running maximum covers too; the sum of the softmax
+// takes it out again per block.  (mma.sync with e4m3 operands, the others split into two e4m3 terms, is slower: it
+// converts inside, for each product again.  Decode 57 us where fp16 took 47.)
 //   * the rows of a tile are 16 (query token, head of the group) couples of one key/value head, so keys are read
-//     once for the heads of a group;
-//   * a warp takes units of 32 keys from a ring of its own in shared memory, filled by bulk copies that its own
-//     lanes issue: the memory system sees 8 KB pieces, and a slot is free again when the warp has read it;
-//   * e4m3 becomes fp16 in registers (exactly), scores and products are fp32, probabilities fp16.  With that the
-//     scales never touch the data: the key scale is a factor on the score, and the value scale 2^e is the term e in
-//     the exponent of the probability, which the running maximum covers too - the sum of the softmax takes it out
-//     again per block;
+//     once for the heads of a group; two tiles share a stream of keys;
+//   * a stream takes units of 32 keys from a ring of its own in shared memory, filled by bulk copies that its own
+//     lanes issue: no barrier of the CTA in the loop, and a slot is free again when its warps have read it;
 //   * the running maximum is raised only when a score passes it by 2^8;
 //   * the work is the flat list of (sequence, head, row tile, unit), cut evenly over the CTAs by the lengths that
-//     the device holds: the host needs no lengths, a call can be captured in a graph.  The warps of a CTA merge
-//     in shared memory, items that were cut over CTAs in a second small kernel, in the order of the keys.
+//     the device holds: the host needs no lengths, a call can be captured in a graph.  The next segment's first units
+//     are on their way while a CTA merges its streams; items that were cut over CTAs are merged by a second small
+//     kernel, in the order of the keys;
+//   * a short call gives each item a cluster of CTAs instead, merged through distributed shared memory: one launch.
 #include <cuda_runtime.h>
 #include <math.h>
 
 #include <string>
 
 #include "../gemm/launch.h"
+#include "../prim/cluster.cuh"
 #include "../prim/mbarrier.cuh"
 #include "../prim/pdl.cuh"
 #include "../prim/tma.cuh"
@@ -34,13 +37,27 @@ namespace cb {
 void set_last_error(const std::string& s);
 
 static constexpr int KA_UNIT = 32;                     // keys
-static constexpr int KA_WARPS = 8;
-static constexpr int KA_STAGES = 3;
 static constexpr int KA_SIDE = KA_UNIT * KV_D;         // bytes of a unit's keys (and of its values)
-static constexpr int KA_RING = KA_WARPS * KA_STAGES * 2 * KA_SIDE;
 static constexpr int KA_MAX_B = 1024;
 static constexpr float KA_RAISE = 8.f;
+static constexpr int KA_MAX_PAGES = 1 << 28;
 static constexpr int KA_MERGE_THREADS = 128;
+static constexpr int KA_MAX_CLUSTER = 8;
+
+// kTiles tiles of 16 query rows times kStreams streams of keys, a warp each.  The warps of a stream share its ring
+// of kStages units.  One tile: 8 warps with up to 255 registers, which work on two times 16 keys at once.  Two
+// tiles: 12 warps with 168; 16 warps (128 registers) spill, 32 rows over 16 x 24000 keys, 64 / 8 heads 357 us
+// instead of 222, and one tile after the other takes 246.  Four tiles (three streams) take as long as two passes of
+// two, 446 and 428 us for 64 rows.
+template <int kTiles_>
+struct KaCfg {
+  static constexpr int kTiles = kTiles_, kStreams = kTiles == 1 ? 8 : 6, kWarps = kTiles * kStreams;
+  static constexpr int kStages = 2;
+  static constexpr int kJoint = kTiles == 1 ? 2 : 1;         // times 16 keys
+  static constexpr int kRows = 16 * kTiles;
+  static constexpr int kRing = kStreams * kStages * 2 * KA_SIDE;
+  static constexpr int kBufs = kStreams / 2;                 // of a tile, in the merge of the streams
+};
 
 struct KvAttendParams {
   KvCacheView cache;
@@ -52,19 +69,25 @@ struct KvAttendParams {
   float* part_o;                 // [CTA][taken over / handed on][tile row][128], unnormalised
   float2* part_ml;               // [CTA][taken over / handed on][tile row] {max (log2 units), sum}
   uint32_t* plan;                // [B + 2]: units before each sequence, units per CTA
-  int Hq, group, row_tiles, window, sinks;
+  int Hq, group, row_tiles, window, sinks, cluster;
   float scale_log2;
   uint32_t* status;
 };
 
+template <class Cfg>
 struct KaShared {
-  uint64_t full[KA_WARPS][KA_STAGES];
-  uint32_t base[KA_MAX_B + 1];   // units before each sequence
-  uint32_t sums[KA_WARPS];
-  float2 ml[KA_WARPS][16];
+  float acc[Cfg::kTiles][Cfg::kBufs][16][KV_D];
+  uint4 q[Cfg::kTiles][8][32];   // query fragments: tile, step of 16 dims, lane
+  uint64_t full[Cfg::kStreams][Cfg::kStages];
+  float2 ml[Cfg::kTiles][Cfg::kStreams][16];
+  float2 part_ml[Cfg::kRows];
+  float row_scale[Cfg::kRows];
+  uint32_t sums[Cfg::kWarps];
   int abort_flag;
+  uint32_t base[KA_MAX_B + 1];   // units before each sequence
 };
-static constexpr int KA_SMEM = KA_RING + static_cast<int>(sizeof(KaShared));
+template <class Cfg>
+static constexpr int ka_smem_bytes() { return Cfg::kRing + static_cast<int>(sizeof(KaShared<Cfg>)); }
 
 // The units that some query of a sequence sees: the first `sink_units`, then `first` and on; n in all.
 struct KaSpan {
@@ -119,20 +142,27 @@ __device__ __forceinline__ uint32_t ka_half2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(hi), "f"(lo));
   return h;
 }
+// Four e4m3 numbers as two pairs of fp16.
+__device__ __forceinline__ void ka_expand(uint32_t w, uint32_t* first, uint32_t* second) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(*first), "=r"(*second)
+      : "r"(w));
+}
 
-// The value exponent of a unit's first or second 16 keys.  A block whose values are all zero has the least one; it
-// only counts in the sum of the probabilities, and they would be flushed with it.
-__device__ __forceinline__ int ka_value_exp(int exps, int h) {
-  const int e = static_cast<int8_t>(exps >> (16 * h + 8));
+// The value exponent of 16 keys.  A block whose values are all zero has the least one; it only counts in the sum
+// of the probabilities, and they would be flushed with it.
+__device__ __forceinline__ int ka_value_exp(int exps) {
+  const int e = static_cast<int8_t>(exps >> 8);
   return e == KV_EXP_MIN ? 0 : e;
 }
 
 // Units before each sequence into sh.base, and the units per CTA.  Every CTA does this for itself.
-__device__ __forceinline__ uint32_t ka_plan(const KvAttendParams& p, KaShared& sh) {
+template <class Cfg>
+__device__ __forceinline__ uint32_t ka_plan(const KvAttendParams& p, KaShared<Cfg>& sh) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint32_t items = static_cast<uint32_t>(p.cache.hkv) * p.row_tiles;
   uint32_t before = 0;
-  for (int b0 = 0; b0 < p.batch.B; b0 += KA_WARPS * 32) {
+  for (int b0 = 0; b0 < p.batch.B; b0 += Cfg::kWarps * 32) {
     const int b = b0 + t;
     const uint32_t mine = b < p.batch.B ? static_cast<uint32_t>(ka_span(p, b).n) * items : 0u;
     uint32_t x = mine;
@@ -145,7 +175,7 @@ __device__ __forceinline__ uint32_t ka_plan(const KvAttendParams& p, KaShared& s
     __syncthreads();
     uint32_t off = before, all = 0;
 #pragma unroll
-    for (int w = 0; w < KA_WARPS; ++w) {
+    for (int w = 0; w < Cfg::kWarps; ++w) {
       if (w < warp) off += sh.sums[w];
       all += sh.sums[w];
     }
@@ -156,350 +186,527 @@ __device__ __forceinline__ uint32_t ka_plan(const KvAttendParams& p, KaShared& s
   if (t == 0) sh.base[p.batch.B] = before;
   __syncthreads();
   const uint32_t per = (before + gridDim.x - 1) / gridDim.x;
-  return per < KA_WARPS ? KA_WARPS : per;
+  return per < Cfg::kStreams ? Cfg::kStreams : per;
 }
 
-// What a warp needs to know of one of its units: the page (two pages of 16 tokens), the scales.
-struct KaUnit {
-  int pid[2];
-  int exps;     // key and value exponent bytes of the first and second 16 keys
+__device__ __forceinline__ float4 ka_ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ka_ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// A finished row: four columns of each lane.
+__device__ __forceinline__ void ka_store_row(const KvAttendParams& p, int b, int head, int row, float4 v, float m,
+                                             float sum, int lane) {
+  const int tok = row / p.group, h = head * p.group + row - tok * p.group;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const __nv_bfloat162 o2[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv),
+                                __floats2bfloat162_rn(v.z * inv, v.w * inv)};
+  *reinterpret_cast<uint2*>(p.o + ((static_cast<long long>(b) * p.batch.S + tok) * p.Hq + h) * KV_D + 4 * lane) =
+      *reinterpret_cast<const uint2*>(o2);
+  if (lane == 0)
+    p.lse[(static_cast<long long>(b) * p.Hq + h) * p.batch.S + tok] =
+        sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+}
+
+// The running softmax of a warp's 16 rows: the fragments of rows g and g + 8, results, maximum (log2 units), sum.
+struct KaAcc {
+  float o[8][2][4];
+  float m[2], l[2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 64; ++i) o[i >> 3][(i >> 2) & 1][i & 3] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  __device__ __forceinline__ void scale(int r2, float a) {
+    l[r2] *= a;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      o[i >> 1][i & 1][2 * r2] *= a;
+      o[i >> 1][i & 1][2 * r2 + 1] *= a;
+    }
+  }
+  // x: the largest score of this lane's keys.
+  __device__ __forceinline__ void raise(int r2, float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    x = fmaxf(x, m[r2]);
+    scale(r2, m[r2] == -INFINITY ? 0.f : ka_ex2(m[r2] - x));
+    m[r2] = x;
+  }
+  // Columns 16 k + 4 c .. + 3 of a row.
+  __device__ __forceinline__ float4 four(int r2, int k) const {
+    return make_float4(o[k][0][2 * r2], o[k][1][2 * r2], o[k][0][2 * r2 + 1], o[k][1][2 * r2 + 1]);
+  }
+  __device__ __forceinline__ void add(int r2, int k, float4 v, float f) {
+    o[k][0][2 * r2] += f * v.x;
+    o[k][1][2 * r2] += f * v.y;
+    o[k][0][2 * r2 + 1] += f * v.z;
+    o[k][1][2 * r2 + 1] += f * v.w;
+  }
 };
 
-__global__ void __launch_bounds__(KA_WARPS * 32, 1) kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
+// A range of one item's units.
+struct KaSegment {
+  KaSpan span;
+  int b, head, rt, u0, n;
+  // First key of the i-th unit of a stream.
+  template <class Cfg>
+  __device__ __forceinline__ int key(int stream, int i) const {
+    const int u = u0 + stream + Cfg::kStreams * i;
+    return (u < span.sink_units ? u : span.first + u - span.sink_units) * KA_UNIT;
+  }
+  template <class Cfg>
+  __device__ __forceinline__ int units(int stream) const {
+    return n > stream ? (n - stream + Cfg::kStreams - 1) / Cfg::kStreams : 0;
+  }
+};
+// The segment that begins at unit `pos` of the flat list, in a CTA's range that ends at `range_end`.
+template <class Cfg>
+__device__ __forceinline__ KaSegment ka_locate(const KvAttendParams& p, const KaShared<Cfg>& sh, uint32_t pos,
+                                               uint32_t range_end) {
+  KaSegment s;
+  int lo = 0, hi = p.batch.B;                          // the last sequence with base <= pos
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (sh.base[mid] <= pos) lo = mid; else hi = mid;
+  }
+  s.b = lo;
+  s.span = ka_span(p, lo);
+  const uint32_t in_seq = pos - sh.base[lo], item = in_seq / s.span.n;
+  s.u0 = static_cast<int>(in_seq - item * s.span.n);
+  s.n = s.span.n - s.u0;
+  if (static_cast<uint32_t>(s.n) > range_end - pos) s.n = static_cast<int>(range_end - pos);
+  s.head = static_cast<int>(item) / p.row_tiles;
+  s.rt = static_cast<int>(item) - s.head * p.row_tiles;
+  return s;
+}
+
+// What lane l knows of unit `first + l` of a stream, for its first and second 16 keys: the page (-1: hidden) and the
+// two exponents; `sub` is the unit's place in the page, in units.
+struct KaInfo {
+  int pid, pid2;    // bits 28, 29 of pid: sub
+  int exps;
+};
+template <class Cfg>
+__device__ __forceinline__ KaInfo ka_look_up(const KvAttendParams& p, const KaSegment& s, int stream, int first) {
+  KaInfo k = {-1, -1, 0};
+  const int i = first + static_cast<int>(threadIdx.x & 31u);
+  if (i >= s.units<Cfg>(stream)) return k;
+  const int key = s.key<Cfg>(stream, i);
+  const int* row = p.batch.pages + static_cast<long long>(s.b) * p.batch.cols;
+  const int page = p.cache.page();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = key + 16 * h;
+    if (at >= s.span.end) break;
+    const int col = at >> p.cache.page_log2;
+    const int pid = col < p.batch.cols ? row[col] : -1;
+    if (pid < 0 || pid >= p.cache.num_pages) {
+      report_status(p.status, CB_BAD_ARGUMENT, 2, 0xA04);
+      continue;
+    }
+    const int e = *reinterpret_cast<const uint16_t*>(p.cache.exp_of(pid, s.head, 0));
+    if (h == 0) {
+      k.pid = pid | ((key & (page - 1)) >> 5) << 28;
+      k.exps = e;
+    } else {
+      k.pid2 = pid;
+      k.exps |= e << 16;
+    }
+  }
+  return k;
+}
+
+// Waits for the warps of one stream.
+template <class Cfg>
+__device__ __forceinline__ void ka_stream_sync(int stream) {
+  if constexpr (Cfg::kTiles == 1)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(stream + 1), "n"(32 * Cfg::kTiles) : "memory");
+}
+
+// kCluster: a cluster of CTAs per item, merged through distributed shared memory; else a CTA takes a range of the
+// flat list, and items that are cut leave partial results for the merge kernel.
+template <class Cfg, bool kCluster>
+__global__ void __launch_bounds__(Cfg::kWarps * 32, 1) kv_attend_kernel(const __grid_constant__ KvAttendParams p) {
+  constexpr int kStreams = Cfg::kStreams, kStages = Cfg::kStages, kRows = Cfg::kRows, kBufs = Cfg::kBufs;
   extern __shared__ __align__(1024) uint8_t ka_smem[];
-  KaShared& sh = *reinterpret_cast<KaShared*>(ka_smem + KA_RING);
+  KaShared<Cfg>& sh = *reinterpret_cast<KaShared<Cfg>*>(ka_smem + Cfg::kRing);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  if (lane == 0)
-    for (int i = 0; i < KA_STAGES; ++i) mbar_init(&sh.full[warp][i], 1);
+  const int stream = warp % kStreams, tile = warp / kStreams;
+  if (tile == 0 && lane == 0)
+    for (int i = 0; i < kStages; ++i) mbar_init(&sh.full[stream][i], 1);
   if (threadIdx.x == 0) sh.abort_flag = 0;
   fence_mbar_init();
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t per = ka_plan(p, sh);
-  const uint32_t total = sh.base[p.batch.B];
-  if (blockIdx.x == 0) {
-    for (int b = threadIdx.x; b <= p.batch.B; b += KA_WARPS * 32) p.plan[b] = sh.base[b];
-    if (threadIdx.x == 0) p.plan[p.batch.B + 1] = per;
-  }
-  uint8_t* ring = ka_smem + warp * KA_STAGES * 2 * KA_SIDE;
-  const int page = p.cache.page(), lg = p.cache.page_log2;
-  uint32_t used = 0;                                   // units this warp has taken from its ring
-
-  const unsigned long long end64 = static_cast<unsigned long long>(blockIdx.x + 1) * per;
-  const uint32_t range_end = end64 < total ? static_cast<uint32_t>(end64) : total;
-  uint32_t pos = blockIdx.x * per;
-  int b = 0;
-  bool ok = true;
-  while (pos < range_end) {
-    // ------------------------------------------------------------------ the segment
-    {
-      int lo = b, hi = p.batch.B;                      // the last sequence with base <= pos
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (sh.base[mid] <= pos) lo = mid; else hi = mid;
-      }
-      b = lo;
+  const uint32_t rank = kCluster ? cluster_ctarank() : 0u, ctas = kCluster ? p.cluster : 1u;
+  uint32_t pos = 0, range_end = 1;
+  KaSegment seg;
+  if constexpr (kCluster) {                            // one segment
+    const uint32_t items = static_cast<uint32_t>(p.cache.hkv) * p.row_tiles, it = blockIdx.x / ctas;
+    seg.b = static_cast<int>(it / items);
+    const int item = static_cast<int>(it - seg.b * items);
+    seg.head = item / p.row_tiles;
+    seg.rt = item - seg.head * p.row_tiles;
+    seg.span = ka_span(p, seg.b);
+    const int share = (seg.span.n + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
+    seg.u0 = static_cast<int>(rank) * share;
+    seg.n = max(0, min(share, seg.span.n - seg.u0));
+  } else {
+    const uint32_t per = ka_plan<Cfg>(p, sh);
+    const uint32_t total = sh.base[p.batch.B];
+    if (blockIdx.x == 0) {
+      for (int b = threadIdx.x; b <= p.batch.B; b += Cfg::kWarps * 32) p.plan[b] = sh.base[b];
+      if (threadIdx.x == 0) p.plan[p.batch.B + 1] = per;
     }
-    const KaSpan span = ka_span(p, b);
-    const uint32_t in_seq = pos - sh.base[b];
-    const uint32_t item = in_seq / span.n;
-    const int u0 = static_cast<int>(in_seq - item * span.n);
-    const int head = static_cast<int>(item) / p.row_tiles, rt = static_cast<int>(item) - head * p.row_tiles;
-    int n = span.n - u0;
-    if (static_cast<uint32_t>(n) > range_end - pos) n = static_cast<int>(range_end - pos);
+    const unsigned long long end64 = static_cast<unsigned long long>(blockIdx.x + 1) * per;
+    range_end = end64 < total ? static_cast<uint32_t>(end64) : total;
+    pos = blockIdx.x * per;
+    if (pos < range_end) seg = ka_locate(p, sh, pos, range_end);
+  }
+  uint8_t* ring = ka_smem + stream * kStages * 2 * KA_SIDE;
+  const int rows = p.batch.S * p.group;
+  uint32_t used = 0;                                   // units the stream has taken from its ring
+  // Fills the ring with the `nth` unit from here.  A page that is not there is replaced by any other: its keys are
+  // hidden, its values only have to be numbers.
+  auto issue = [&](uint32_t nth, const KaInfo& info, int from, int head) {
+    if (tile != 0) return;
+    const int first = max(__shfl_sync(0xffffffffu, info.pid, from & 31), 0);
+    const int second = max(__shfl_sync(0xffffffffu, info.pid2, from & 31), 0);
+    const int pid = first & (KA_MAX_PAGES - 1), sub = first >> 28;
+    const uint32_t slot = (used + nth) % kStages;
+    uint64_t* bar = &sh.full[stream][slot];
+    if (lane == 0) mbar_arrive_expect_tx(bar, 2 * KA_SIDE);
+    __syncwarp();
+    if (p.cache.page_log2 == 4) {                      // a unit is two pages
+      if (lane < 4)
+        bulk_load_1d(ring + (2 * slot + (lane & 1)) * KA_SIDE + (lane >> 1) * (KA_SIDE / 2),
+                     p.cache.tile(lane >> 1 ? second : pid, head, lane & 1), KA_SIDE / 2, bar);
+    } else if (lane < 2) {
+      bulk_load_1d(ring + (2 * slot + lane) * KA_SIDE, p.cache.tile(pid, head, lane) + sub * KA_SIDE, KA_SIDE, bar);
+    }
+  };
+  bool ok = true;
+  int mine = 0;                                        // units of the stream in this segment
+  KaInfo info = {-1, -1, 0};
+  if (pos < range_end) {
+    mine = seg.units<Cfg>(stream);
+    info = ka_look_up<Cfg>(p, seg, stream, 0);
+    for (int i = 0; i < kStages && i < mine; ++i) issue(i, info, i, seg.head);
+  }
+  while (pos < range_end) {
+    const KaSpan& span = seg.span;
+    const int b = seg.b, head = seg.head, rt = seg.rt, n = seg.n;
+    KaInfo next = mine > 32 ? ka_look_up<Cfg>(p, seg, stream, 32) : info;
 
-    const int mine = n > warp ? (n - warp + KA_WARPS - 1) / KA_WARPS : 0;   // u0 + warp, + 8, ...
-    auto key_of = [&](int i) {                         // first key of this warp's i-th unit
-      const int u = u0 + warp + KA_WARPS * i;
-      return (u < span.sink_units ? u : span.first + u - span.sink_units) * KA_UNIT;
-    };
-    // Lane l holds what there is to know of unit `base + l`.
-    auto look_up = [&](int base) {
-      KaUnit k;
-      k.pid[0] = k.pid[1] = -1;
-      k.exps = 0;
-      const int i = base + lane;
-      if (i < mine) {
-        const int key = key_of(i);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = key + 16 * h;
-          if (at >= span.end) continue;                // hidden
-          const int col = at >> lg;
-          const int pid = col < p.batch.cols ? p.batch.pages[static_cast<long long>(b) * p.batch.cols + col] : -1;
-          if (pid < 0 || pid >= p.cache.num_pages) {
-            report_status(p.status, CB_BAD_ARGUMENT, 2, 0xA04);
-            continue;
-          }
-          k.pid[h] = pid;
-          const uint32_t e = *reinterpret_cast<const uint16_t*>(p.cache.exp_of(pid, head, 0));
-          k.exps |= static_cast<int>(e << (16 * h));
-        }
-      }
-      return k;
-    };
-    KaUnit info = look_up(0);
-    // Fills the ring with this warp's i-th unit.  A page that is not there is replaced by any other: its keys are
-    // hidden, its values only have to be numbers.
-    auto issue = [&](int i) {
-      const int src = i & 31;
-      const int p0 = __shfl_sync(0xffffffffu, info.pid[0], src), p1 = __shfl_sync(0xffffffffu, info.pid[1], src);
-      const uint32_t slot = (used + i) % KA_STAGES;
-      uint8_t* dst = ring + slot * 2 * KA_SIDE;
-      uint64_t* bar = &sh.full[warp][slot];
-      const int a0 = p0 >= 0 ? p0 : 0, a1 = p1 >= 0 ? p1 : a0;
-      if (lane == 0) mbar_arrive_expect_tx(bar, 2 * KA_SIDE);
-      __syncwarp();
-      if (page == 16) {
-        if (lane < 4)
-          bulk_load_1d(dst + (lane & 1) * KA_SIDE + (lane >> 1) * (KA_SIDE / 2),
-                       p.cache.tile(lane >> 1 ? a1 : a0, head, lane & 1), KA_SIDE / 2, bar);
-      } else if (lane < 2) {
-        const int slot0 = key_of(i) & (page - 1);
-        bulk_load_1d(dst + lane * KA_SIDE, p.cache.tile(a0, head, lane) + slot0 * KV_D, KA_SIDE, bar);
-      }
-    };
-    for (int i = 0; i < KA_STAGES && i < mine; ++i) issue(i);
-
-    // ------------------------------------------------------------------ queries of the tile
-    // Fragments of m16n8k16 with the head dimension in the order in which the keys' bytes arrive: step m takes
-    // dims 16 m + 4 c .. + 3 of lane c.  Rows are brought to [1, 2) by a power of two, so that fp16 holds them.
-    uint32_t qa[8][4];
-    float row_scale[2];
-    int row_pos[2];
-    const int rows = p.batch.S * p.group;
-#pragma unroll
-    for (int r2 = 0; r2 < 2; ++r2) {
-      const int r = rt * 16 + g + 8 * r2;
-      const int tok = r / p.group;
-      const bool there = r < rows && tok < span.count;
-      row_pos[r2] = there ? span.start + tok : -1;
-      uint2 raw[8];
-      float amax = 0.f;
+    // ------------------------------------------------------------------ queries of the tiles
+    // Fragments of m16n8k16 with the head dimension in the order in which the keys' bytes arrive: step m takes dims
+    // 16 m + 4 c .. + 3 of lane c.  Rows are brought to [1, 2) by a power of two, so that fp16 holds them.
+    for (int r = warp; r < kRows; r += Cfg::kWarps) {     // a warp takes a row, a lane four dims
+      const int row = rt * kRows + r, tok = row / p.group;
+      const bool there = row < rows && tok < span.count;
       const __nv_bfloat16* src =
-          p.q + b * p.q_sb + tok * p.q_ss + static_cast<long long>(head * p.group + r - tok * p.group) * p.q_sh + 4 * c;
-#pragma unroll
-      for (int m = 0; m < 8; ++m) {
-        raw[m] = there ? *reinterpret_cast<const uint2*>(src + 16 * m) : make_uint2(0u, 0u);
-        const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[m].x));
-        const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[m].y));
-        amax = fmaxf(amax, fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))));
-      }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+          p.q + b * p.q_sb + tok * p.q_ss + static_cast<long long>(head * p.group + row - tok * p.group) * p.q_sh + 4 * lane;
+      const uint2 raw = there ? *reinterpret_cast<const uint2*>(src) : make_uint2(0u, 0u);
+      const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+      const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+      const float amax = fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y)));
+      int e = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)) >> 23) - 127;
       e = e < -100 ? -100 : e > 100 ? 100 : e;
       const float down = kv_pow2(-e);
-      row_scale[r2] = p.scale_log2 * kv_pow2(e);
+      uint32_t* dst = reinterpret_cast<uint32_t*>(&sh.q[r >> 4][lane >> 2][(r & 7) * 4 + (lane & 3)]) + ((r >> 3) & 1);
+      dst[0] = ka_half2(f0.x * down, f0.y * down);
+      dst[2] = ka_half2(f1.x * down, f1.y * down);
+      if (lane == 0) sh.row_scale[r] = p.scale_log2 * kv_pow2(e);
+    }
+    __syncthreads();
+    float row_scale[2];
+    int row_pos[2];
 #pragma unroll
-      for (int m = 0; m < 8; ++m) {
-        const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[m].x));
-        const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[m].y));
-        qa[m][r2] = ka_half2(f0.x * down, f0.y * down);
-        qa[m][2 + r2] = ka_half2(f1.x * down, f1.y * down);
-      }
+    for (int r2 = 0; r2 < 2; ++r2) {
+      const int r = 16 * tile + 8 * r2 + g, row = rt * kRows + r, tok = row / p.group;
+      row_scale[r2] = sh.row_scale[r];
+      row_pos[r2] = row < rows && tok < span.count ? span.start + tok : -1;
+    }
+    // The next segment's first pages are asked for now and its first units loaded before the merge of this one.
+    KaInfo after = {-1, -1, 0};
+    int after_mine = 0, after_head = 0;
+    if (!kCluster && pos + n < range_end) {
+      const KaSegment s = ka_locate(p, sh, pos + n, range_end);
+      after = ka_look_up<Cfg>(p, s, stream, 0);
+      after_mine = s.units<Cfg>(stream);
+      after_head = s.head;
     }
 
     // ------------------------------------------------------------------ the units
-    float o[8][2][4];
-#pragma unroll
-    for (int m = 0; m < 8; ++m)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[m][x][j] = 0.f;
-    float m_ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    KaAcc acc;
+    acc.clear();
     const int first_pos = span.start, last_pos = span.end - 1;   // of any query of the sequence
-    for (int i = 0; ok && i < mine; ++i) {
-      const uint32_t slot = (used + i) % KA_STAGES;
-      if (!mbar_wait_warp(&sh.full[warp][slot], ((used + i) / KA_STAGES) & 1u, &sh.abort_flag, p.status, 0xA10)) {
-        ok = false;
-        break;
+    for (int i = 0; i < mine; ++i) {
+      const uint32_t slot = (used + i) % kStages;
+      // After a wait that ran out the warps of a stream still meet in every round, without touching the ring.
+      ok = ok && mbar_wait_warp(&sh.full[stream][slot], ((used + i) / kStages) & 1u, &sh.abort_flag, p.status, 0xA10);
+      if (!ok) {
+        ka_stream_sync<Cfg>(stream);
+        continue;
       }
-      const uint32_t keys = smem_u32(ring + slot * 2 * KA_SIDE), values = keys + KA_SIDE;
+      const uint32_t keys = smem_u32(ring + 2 * slot * KA_SIDE), values = keys + KA_SIDE;
+      const int key = seg.key<Cfg>(stream, i);
       const int exps = __shfl_sync(0xffffffffu, info.exps, i & 31);
-      const int seen0 = __shfl_sync(0xffffffffu, info.pid[0], i & 31) >= 0;
-      const int seen1 = __shfl_sync(0xffffffffu, info.pid[1], i & 31) >= 0;
-      const int key = key_of(i);
-      // scores: four tiles of 8 keys
-      float s[4][4];
+      const bool seen[2] = {__shfl_sync(0xffffffffu, info.pid, i & 31) >= 0, __shfl_sync(0xffffffffu, info.pid2, i & 31) >= 0};
+      const bool mask = key + KA_UNIT - 1 > first_pos || !seen[0] || !seen[1] ||
+                        (p.window > 0 && key <= last_pos - p.window && key + KA_UNIT > p.sinks);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int h0 = 0; h0 < 2; h0 += Cfg::kJoint) {    // kJoint times 16 keys at a time
+        // scores: tiles of 8 keys
+        float s[2 * Cfg::kJoint][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[t][j] = 0.f;
+        for (int k = 0; k < 8 * Cfg::kJoint; ++k) s[k >> 2][k & 3] = 0.f;
 #pragma unroll
         for (int mh = 0; mh < 2; ++mh) {
-          uint32_t r[4];
-          const int row = 8 * t + (lane & 7);
-          ka_ldsm(keys + row * KV_D + (((4 * mh + (lane >> 3)) ^ (row & 7)) << 4), r);
+          uint32_t r[2 * Cfg::kJoint][4];
 #pragma unroll
-          for (int m = 0; m < 4; ++m) ka_mma(s[t], qa[4 * mh + m], kv_to_half2(r[m]), kv_to_half2(r[m] >> 16));
-        }
-      }
-      // to log2 units with both scales in, hidden ones to -inf
-      const bool mask = key + KA_UNIT - 1 > first_pos || !seen0 || !seen1 ||
-                        (p.window > 0 && key <= last_pos - p.window && key + KA_UNIT > p.sinks);
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float f = kv_pow2(static_cast<int8_t>(exps >> (16 * (t >> 1))));
-        const float add = static_cast<float>(ka_value_exp(exps, t >> 1));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x = fmaf(s[t][j], row_scale[j >> 1] * f, add);
-          if (mask) {
-            const int at = key + 8 * t + 2 * c + (j & 1), q = row_pos[j >> 1];
-            const bool hidden = at > q || (p.window > 0 && at <= q - p.window && at >= p.sinks) ||
-                                !(t >> 1 ? seen1 : seen0);
-            x = hidden ? -INFINITY : x;
+          for (int k = 0; k < 2 * Cfg::kJoint; ++k) {
+            const int row = 16 * h0 + 8 * k + (lane & 7);
+            ka_ldsm(keys + row * KV_D + (((4 * mh + (lane >> 3)) ^ (row & 7)) << 4), r[k]);
           }
-          s[t][j] = x;
-          mx[j >> 1] = fmaxf(mx[j >> 1], x);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const uint4 q4 = sh.q[tile][4 * mh + m][lane];
+            const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+            for (int k = 0; k < 2 * Cfg::kJoint; ++k) {
+              uint32_t b0, b1;
+              ka_expand(r[k][m], &b0, &b1);
+              ka_mma(s[k], q, b0, b1);
+            }
+          }
         }
-      }
-      const bool grow = mx[0] > m_ref[0] + KA_RAISE || mx[1] > m_ref[1] + KA_RAISE ||
-                        (m_ref[0] == -INFINITY && mx[0] > -INFINITY) || (m_ref[1] == -INFINITY && mx[1] > -INFINITY);
-      if (__any_sync(0xffffffffu, grow)) {
+        // to log2 units with both scales in, less the running maximum; hidden ones to -inf
+        const float off[2] = {acc.m[0] == -INFINITY ? 0.f : acc.m[0], acc.m[1] == -INFINITY ? 0.f : acc.m[1]};
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int r2 = 0; r2 < 2; ++r2) {
-          float x = mx[r2];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          x = fmaxf(x, m_ref[r2]);
-          const float a = m_ref[r2] == -INFINITY ? 0.f : ka_ex2(m_ref[r2] - x);
-          m_ref[r2] = x;
-          l[r2] *= a;
+        for (int h = 0; h < Cfg::kJoint; ++h) {
+          const int e2 = exps >> (16 * (h0 + h));
+          const float f = kv_pow2(static_cast<int8_t>(e2)), add = static_cast<float>(ka_value_exp(e2));
 #pragma unroll
-          for (int m = 0; m < 8; ++m)
+          for (int r2 = 0; r2 < 2; ++r2) {
+            const float mul = row_scale[r2] * f, plus = add - off[r2];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              o[m][y][2 * r2] *= a;
-              o[m][y][2 * r2 + 1] *= a;
+            for (int k = 0; k < 4; ++k) {
+              float& x = s[2 * h + (k >> 1)][2 * r2 + (k & 1)];
+              x = fmaf(x, mul, plus);
+            }
+          }
+        }
+        if (mask) {
+#pragma unroll
+          for (int k = 0; k < 2 * Cfg::kJoint; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int at = key + 16 * h0 + 8 * k + 2 * c + (j & 1), q = row_pos[j >> 1];
+              const bool hidden = at > q || (p.window > 0 && at <= q - p.window && at >= p.sinks) || !seen[h0 + (k >> 1)];
+              s[k][j] = hidden ? -INFINITY : s[k][j];
             }
         }
-      }
-      // probabilities (times the value scale) and their sums (without it)
-      const float off[2] = {m_ref[0] == -INFINITY ? 0.f : m_ref[0], m_ref[1] == -INFINITY ? 0.f : m_ref[1]};
-      uint32_t pa[2][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float sum[2] = {0.f, 0.f};
+        for (int k = 0; k < 2 * Cfg::kJoint; ++k)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float e[4];
+          for (int j = 0; j < 4; ++j) mx[j >> 1] = fmaxf(mx[j >> 1], s[k][j]);
+        const bool grow = mx[0] > KA_RAISE || mx[1] > KA_RAISE || (acc.m[0] == -INFINITY && mx[0] > -INFINITY) ||
+                          (acc.m[1] == -INFINITY && mx[1] > -INFINITY);
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            e[j] = ka_ex2(s[2 * h + t][j] - off[j >> 1]);
-            sum[j >> 1] += e[j];
-          }
-          pa[h][2 * t] = ka_half2(e[0], e[1]);
-          pa[h][2 * t + 1] = ka_half2(e[2], e[3]);
-        }
-        const float out = kv_pow2(-ka_value_exp(exps, h));
-        l[0] = fmaf(sum[0], out, l[0]);
-        l[1] = fmaf(sum[1], out, l[1]);
-      }
-      // products: the transposing load of byte pairs gives {key, dim}, {key, dim + 1}, {key + 1, dim}, {key + 1,
-      // dim + 1}; even and odd dims make a tile of 8 each
+          for (int r2 = 0; r2 < 2; ++r2) {
+            acc.raise(r2, mx[r2] + off[r2]);
+            const float by = (acc.m[r2] == -INFINITY ? 0.f : acc.m[r2]) - off[r2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int m = 0; m < 8; m += 2) {
-          uint32_t r[4];
-          const int row = 16 * h + (lane & 15);
-          ka_ldsm_t(values + row * KV_D + (((m + (lane >> 4)) ^ (row & 7)) << 4), r);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t b0 = __byte_perm(r[2 * x], 0u, 0x3120), b1 = __byte_perm(r[2 * x + 1], 0u, 0x3120);
-            ka_mma(o[m + x][0], pa[h], kv_to_half2(b0), kv_to_half2(b1));
-            ka_mma(o[m + x][1], pa[h], kv_to_half2(b0 >> 16), kv_to_half2(b1 >> 16));
+            for (int k = 0; k < 4 * Cfg::kJoint; ++k) s[k >> 1][2 * r2 + (k & 1)] -= by;
           }
         }
-      __syncwarp();                                    // the slot has been read
-      if (i + 1 < mine && ((i + 1) & 31) == 0) info = look_up(i + 1);
-      // units up to the end of the looked-up batch are issued ahead; the rest after the next look-up
-      const int ahead = i + KA_STAGES;
-      if (ahead < mine && (ahead >> 5) == ((i + 1) >> 5)) issue(ahead);
-      if (((i + 1) & 31) == 0)
-        for (int x = i + 1; x < ahead && x < mine; ++x) issue(x);
+#pragma unroll
+        for (int h = 0; h < Cfg::kJoint; ++h) {
+          // probabilities (times the value scale) and their sums (without it)
+          const float out = kv_pow2(-ka_value_exp(exps >> (16 * (h0 + h))));
+          uint32_t pa[4];
+#pragma unroll
+          for (int r2 = 0; r2 < 2; ++r2) {
+            float e[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e[k] = ka_ex2(s[2 * h + (k >> 1)][2 * r2 + (k & 1)]);
+            acc.l[r2] = fmaf((e[0] + e[1]) + (e[2] + e[3]), out, acc.l[r2]);
+            pa[r2] = ka_half2(e[0], e[1]);
+            pa[2 + r2] = ka_half2(e[2], e[3]);
+          }
+          // products: the transposing load of byte pairs gives {key, dim}, {key, dim + 1}, {key + 1, dim}, {key + 1,
+          // dim + 1}; even and odd dims make a tile of 8 each
+#pragma unroll
+          for (int m = 0; m < 8; m += 2) {
+            uint32_t r[4];
+            const int row = 16 * (h0 + h) + (lane & 15);
+            ka_ldsm_t(values + row * KV_D + (((m + (lane >> 4)) ^ (row & 7)) << 4), r);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              uint32_t b0[2], b1[2];
+              ka_expand(__byte_perm(r[2 * x], 0u, 0x3120), &b0[0], &b0[1]);
+              ka_expand(__byte_perm(r[2 * x + 1], 0u, 0x3120), &b1[0], &b1[1]);
+              ka_mma(acc.o[m + x][0], pa, b0[0], b1[0]);
+              ka_mma(acc.o[m + x][1], pa, b0[1], b1[1]);
+            }
+          }
+        }
+      }
+      ka_stream_sync<Cfg>(stream);                     // the slot has been read
+      if (((i + 1) & 31) == 0) {
+        info = next;
+        next = ka_look_up<Cfg>(p, seg, stream, i + 33);
+      }
+      const int ahead = i + kStages;
+      if (ahead < mine) issue(ahead, (ahead >> 5) == ((i + 1) >> 5) ? info : next, ahead, head);
     }
     used += mine;
-#pragma unroll
-    for (int r2 = 0; r2 < 2; ++r2)
-      if (row_pos[r2] < 0) {                           // not a query: zeros
-        m_ref[r2] = -INFINITY;
-        l[r2] = 0.f;
-#pragma unroll
-        for (int m = 0; m < 8; ++m)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) o[m][y][2 * r2] = o[m][y][2 * r2 + 1] = 0.f;
-      }
+    if constexpr (!kCluster) {
+      for (int i = 0; ok && i < kStages && i < after_mine; ++i) issue(i, after, i, after_head);
+    }
 
-    // ------------------------------------------------------------------ merge of the warps
-    float* acc = reinterpret_cast<float*>(ka_smem);    // [warp][16][128], over the rings
+    // ------------------------------------------------------------------ merge of the streams
+    // The upper half of them hands its results over, the lower half adds them to its own; then rows are summed up.
 #pragma unroll
     for (int r2 = 0; r2 < 2; ++r2) {
-      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 1);
-      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 2);
-      if (c == 0) sh.ml[warp][g + 8 * r2] = make_float2(m_ref[r2], l[r2]);
+      if (row_pos[r2] < 0) {                           // not a query: zeros
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc.o[i >> 1][i & 1][2 * r2] = acc.o[i >> 1][i & 1][2 * r2 + 1] = 0.f;
+        acc.m[r2] = -INFINITY;
+        acc.l[r2] = 0.f;
+      }
+      acc.l[r2] += __shfl_xor_sync(0xffffffffu, acc.l[r2], 1);
+      acc.l[r2] += __shfl_xor_sync(0xffffffffu, acc.l[r2], 2);
+    }
+    const int buf = stream % kBufs;
+    if (stream >= kBufs) {
+#pragma unroll
+      for (int r2 = 0; r2 < 2; ++r2) {
+        if (c == 0) sh.ml[tile][stream][8 * r2 + g] = make_float2(acc.m[r2], acc.l[r2]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<float4*>(&sh.acc[tile][buf][8 * r2 + g][16 * k + 4 * c]) = acc.four(r2, k);
+      }
     }
     __syncthreads();
+    if (stream < kBufs) {
 #pragma unroll
-    for (int r2 = 0; r2 < 2; ++r2)
+      for (int r2 = 0; r2 < 2; ++r2) {
+        const float2 x = sh.ml[tile][stream + kBufs][8 * r2 + g];
+        const float m = fmaxf(acc.m[r2], x.x);
+        const float f = x.x == -INFINITY ? (x.y == x.y ? 0.f : 1.f) : ka_ex2(x.x - m);
+        if (acc.m[r2] != m) acc.scale(r2, acc.m[r2] == -INFINITY ? (acc.l[r2] == acc.l[r2] ? 0.f : 1.f) : ka_ex2(acc.m[r2] - m));
+        acc.m[r2] = m;
+        acc.l[r2] = fmaf(f, x.y, acc.l[r2]);
+        if (c == 0) sh.ml[tile][stream][8 * r2 + g] = make_float2(m, acc.l[r2]);
 #pragma unroll
-      for (int m = 0; m < 8; ++m)
-        *reinterpret_cast<float4*>(acc + (warp * 16 + g + 8 * r2) * KV_D + 16 * m + 4 * c) =
-            make_float4(o[m][0][2 * r2], o[m][1][2 * r2], o[m][0][2 * r2 + 1], o[m][1][2 * r2 + 1]);
+        for (int k = 0; k < 8; ++k) {
+          float4* at = reinterpret_cast<float4*>(&sh.acc[tile][buf][8 * r2 + g][16 * k + 4 * c]);
+          acc.add(r2, k, *at, f);
+          *at = acc.four(r2, k);
+        }
+      }
+    }
     __syncthreads();
-    const bool whole = n == span.n;
-    const uint32_t slot = 2u * blockIdx.x + (u0 == 0 ? 1u : 0u);
+    const bool whole = !kCluster && n == span.n;
+    const uint32_t slot = 2u * blockIdx.x + (seg.u0 == 0 ? 1u : 0u);
 #pragma unroll 1
-    for (int r = warp; r < 16; r += KA_WARPS) {
-      const int row = rt * 16 + r;
+    for (int r = warp; r < kRows; r += Cfg::kWarps) {
+      const int row = rt * kRows + r;
       if (row >= rows) continue;
       float m = -INFINITY, sum = 0.f;
+      float2 x[kBufs];
 #pragma unroll
-      for (int w = 0; w < KA_WARPS; ++w) m = fmaxf(m, sh.ml[w][r].x);
+      for (int w = 0; w < kBufs; ++w) {
+        x[w] = sh.ml[r >> 4][w][r & 15];
+        m = fmaxf(m, x[w].x);
+      }
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < KA_WARPS; ++w) {
-        const float2 x = sh.ml[w][r];
-        const float f = x.x == -INFINITY ? 0.f : ka_ex2(x.x - m);
-        sum += f * x.y;
-        const float4 a = *reinterpret_cast<const float4*>(acc + (w * 16 + r) * KV_D + 4 * lane);
+      for (int w = 0; w < kBufs; ++w) {
+        const float f = x[w].x == -INFINITY ? 0.f : ka_ex2(x[w].x - m);
+        sum += f * x[w].y;
+        const float4 a = *reinterpret_cast<const float4*>(&sh.acc[r >> 4][w][r & 15][4 * lane]);
         v.x += f * a.x, v.y += f * a.y, v.z += f * a.z, v.w += f * a.w;
       }
-      if (whole) {
-        const int tok = row / p.group, h = head * p.group + row - tok * p.group;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const __nv_bfloat162 o2[2] = {__floats2bfloat162_rn(v.x * inv, v.y * inv),
-                                      __floats2bfloat162_rn(v.z * inv, v.w * inv)};
-        *reinterpret_cast<uint2*>(p.o + ((static_cast<long long>(b) * p.batch.S + tok) * p.Hq + h) * KV_D + 4 * lane) =
-            *reinterpret_cast<const uint2*>(o2);
-        if (lane == 0)
-          p.lse[(static_cast<long long>(b) * p.Hq + h) * p.batch.S + tok] =
-              sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+      if (whole || (kCluster && ctas == 1)) {
+        ka_store_row(p, b, head, row, v, m, sum, lane);
+      } else if constexpr (kCluster) {
+        // row r of buffer 0 is this warp's alone now: the CTA's part of the row
+        __syncwarp();
+        *reinterpret_cast<float4*>(&sh.acc[r >> 4][0][r & 15][4 * lane]) = v;
+        if (lane == 0) sh.part_ml[r] = make_float2(m, sum);
       } else {
-        const long long at = static_cast<long long>(slot) * 16 + r;
+        const long long at = static_cast<long long>(slot) * kRows + r;
         *reinterpret_cast<float4*>(p.part_o + at * KV_D + 4 * lane) = v;
         if (lane == 0) p.part_ml[at] = make_float2(m, sum);
       }
     }
-    fence_proxy_async_smem();   // the next segment's bulk copies write where ordinary accesses were
-    __syncthreads();
-    if (*static_cast<volatile int*>(&sh.abort_flag) != 0) {
-      // A copy never arrived: the others get time to land before the shared memory goes to another CTA.
-      const uint64_t t0 = globaltimer_ns();
-      while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    if constexpr (kCluster) {
+      if (ctas == 1) break;
+      cluster_sync_all();
+      // rows in turn; the parts in the order of the keys
+      for (int r = static_cast<int>(rank) + warp * static_cast<int>(ctas); r < kRows; r += Cfg::kWarps * static_cast<int>(ctas)) {
+        const int row = rt * kRows + r;
+        if (row >= rows) continue;
+        float4 v[KA_MAX_CLUSTER];
+        float2 x[KA_MAX_CLUSTER];
+        float m = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < KA_MAX_CLUSTER; ++i)
+          if (i < ctas) {
+            x[i] = ka_ld_cluster2(map_to_cta(smem_u32(&sh.part_ml[r]), i));
+            v[i] = ka_ld_cluster(map_to_cta(smem_u32(&sh.acc[r >> 4][0][r & 15][4 * lane]), i));
+            m = fmaxf(m, x[i].x);
+          }
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t i = 0; i < KA_MAX_CLUSTER; ++i)
+          if (i < ctas) {
+            const float f = x[i].x == -INFINITY ? 0.f : ka_ex2(x[i].x - m);
+            sum += f * x[i].y;
+            a.x += f * v[i].x, a.y += f * v[i].y, a.z += f * v[i].z, a.w += f * v[i].w;
+          }
+        ka_store_row(p, b, head, row, a, m, sum, lane);
+      }
+      cluster_sync_all();                              // nobody leaves while its part is being read
       break;
     }
+    if (__syncthreads_or(*static_cast<volatile int*>(&sh.abort_flag)) != 0) break;
     pos += n;
+    if (pos < range_end) {
+      seg = ka_locate(p, sh, pos, range_end);
+      info = after;
+      mine = after_mine;
+    }
+  }
+  if (*static_cast<volatile int*>(&sh.abort_flag) != 0) {
+    // A copy never arrived: the others get time to land before the shared memory goes to another CTA.
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
   }
 }
 
 // Rows of items that were cut: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i in the order of the keys.  A warp
 // takes a row.
+template <int kRows>
 __global__ void __launch_bounds__(KA_MERGE_THREADS) kv_attend_merge_kernel(const __grid_constant__ KvAttendParams p) {
   pdl_wait();
   pdl_launch_dependents();
@@ -510,7 +717,7 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv_attend_merge_kernel(const
   if (row >= rows * hkv * p.batch.B) return;
   const long long bh = row / rows;
   const int b = static_cast<int>(bh / hkv), head = static_cast<int>(bh - static_cast<long long>(b) * hkv);
-  const int r = static_cast<int>(row - bh * rows), rt = r >> 4;
+  const int r = static_cast<int>(row - bh * rows), rt = r / kRows;
   const uint32_t base = p.plan[b], per = p.plan[p.batch.B + 1];
   const uint32_t n = (p.plan[b + 1] - base) / static_cast<uint32_t>(hkv * p.row_tiles);
   const uint32_t start = base + static_cast<uint32_t>(head * p.row_tiles + rt) * n;
@@ -528,7 +735,7 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv_attend_merge_kernel(const
       const uint32_t i = i0 + u;
       if (i <= cta1) {
         const bool begins = i * per <= start;
-        const long long at = static_cast<long long>(2u * i + (begins ? 1u : 0u)) * 16 + (r & 15);
+        const long long at = static_cast<long long>(2u * i + (begins ? 1u : 0u)) * kRows + (r % kRows);
         x[u] = p.part_ml[at];
         v[u] = reinterpret_cast<const float4*>(p.part_o + at * KV_D)[lane];
       }
@@ -548,43 +755,80 @@ __global__ void __launch_bounds__(KA_MERGE_THREADS) kv_attend_merge_kernel(const
       acc.x += f * v[u].x, acc.y += f * v[u].y, acc.z += f * v[u].z, acc.w += f * v[u].w;
     }
   }
-  const int tok = r / p.group, h = head * p.group + r - tok * p.group;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const __nv_bfloat162 o2[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
-                                __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-  *reinterpret_cast<uint2*>(p.o + ((static_cast<long long>(b) * S + tok) * p.Hq + h) * KV_D + 4 * lane) =
-      *reinterpret_cast<const uint2*>(o2);
-  if (lane == 0)
-    p.lse[(static_cast<long long>(b) * p.Hq + h) * S + tok] =
-        l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+  ka_store_row(p, b, head, r, acc, m, l, lane);
 }
 
+// SMs of the current device, asked for once per device.
 static int ka_sms() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
     return 148;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
 struct KaLaunch {
-  int row_tiles, grid;
+  int tile_rows, row_tiles, grid, cluster;   // cluster 0: the flat list
   long long bytes, o_at, ml_at;
 };
 // False when the flat list of units does not fit 31 bits.
+//
+// A cluster per item or the flat list: a round (one unit for each stream of a CTA) takes kRound, a call 8 us beside its rounds
+// as clusters and 16 as a flat list, which has segments, a plan and a merge.  Measured (sequences x tokens, 32 / 8
+// heads, cluster / flat): 1 x 1000 12.7 / 15.4, 4 x 4000 14.1 / 18.2, 1 x 16000 17.5 / 18.3, 8 x 4000 18.0 / 22.9, 16 x 6001
+// 40.6 / 45.8; 8 / 1 heads, 1 x 32000 27.7 / 19.0; 16 x 24000 134 / 129.  The host knows a bound of the lengths only,
+// and the longest item of a cluster call decides: the flat list counts as if lengths were nine tenths of the bound.
 static bool ka_shape(KaLaunch* s, int B, int S, int Hq, int Hkv, long long max_len) {
   const long long rows = static_cast<long long>(S) * (Hq / Hkv);
-  const long long tiles = (rows + 15) / 16;
-  const long long units = static_cast<long long>(B) * Hkv * tiles * ((max_len + KA_UNIT - 1) / KA_UNIT + 1);
-  if (units > 0x7fffffffll || B > KA_MAX_B) return false;
+  s->tile_rows = rows <= 16 ? 16 : 32;
+  const int streams = rows <= 16 ? KaCfg<1>::kStreams : KaCfg<2>::kStreams;
+  const float kRound = rows <= 16 ? 1.35f : 1.9f;
+  const long long tiles = (rows + s->tile_rows - 1) / s->tile_rows;
+  const long long items = static_cast<long long>(B) * Hkv * tiles, per_item = (max_len + KA_UNIT - 1) / KA_UNIT + 1;
+  if (items * per_item > 0x7fffffffll || B > KA_MAX_B) return false;
   s->row_tiles = static_cast<int>(tiles);
-  const long long want = (units + KA_WARPS - 1) / KA_WARPS;
   const int sms = ka_sms();
+  int c = 1;
+  while (2 * c <= KA_MAX_CLUSTER && 2 * c * items <= sms && c * streams < per_item) c *= 2;
+  const float chain = static_cast<float>((per_item + c * streams - 1) / (c * streams));
+  const float rounds = static_cast<float>(items * per_item) / static_cast<float>(sms * streams);
+  s->cluster = 0;
+  s->bytes = s->o_at = s->ml_at = 0;
+  if (items * c <= sms && 8.f + kRound * chain <= 16.f + kRound * 0.9f * rounds) {
+    s->cluster = c;
+    s->grid = static_cast<int>(items) * c;
+    return true;
+  }
+  const long long want = (items * per_item + streams - 1) / streams;
   s->grid = static_cast<int>(want < sms ? want : sms);
   s->o_at = (static_cast<long long>(B + 2) * 4 + 127) / 128 * 128;
-  s->ml_at = s->o_at + 2ll * s->grid * 16 * KV_D * 4;
-  s->bytes = s->ml_at + 2ll * s->grid * 16 * 8;
+  s->ml_at = s->o_at + 2ll * s->grid * s->tile_rows * KV_D * 4;
+  s->bytes = s->ml_at + 2ll * s->grid * s->tile_rows * 8;
   return true;
+}
+
+template <class Cfg>
+static cudaError_t ka_launch(const KvAttendParams& p, const KaLaunch& s, cudaStream_t st) {
+  constexpr int kSmem = ka_smem_bytes<Cfg>();
+  static_assert(kSmem <= 232448, "over the 227 KB shared-memory limit");
+  static std::atomic<uint64_t> flat_done{0}, cluster_done{0};
+  if (s.cluster > 0) {
+    auto kernel = kv_attend_kernel<Cfg, true>;
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), kSmem, cluster_done);
+    return e != cudaSuccess ? e
+                            : launch_gemm_kernel_pdl(kernel, s.grid, Cfg::kWarps * 32, kSmem, st, s.cluster, false, true, p);
+  }
+  auto kernel = kv_attend_kernel<Cfg, false>;
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), kSmem, flat_done);
+  if (e == cudaSuccess) e = launch_gemm_kernel_pdl(kernel, s.grid, Cfg::kWarps * 32, kSmem, st, 1, false, true, p);
+  if (e != cudaSuccess) return e;
+  const long long rows = static_cast<long long>(p.batch.B) * p.batch.S * p.Hq;
+  const int per = KA_MERGE_THREADS / 32;
+  return launch_pdl(kv_attend_merge_kernel<Cfg::kRows>, dim3(static_cast<unsigned>((rows + per - 1) / per)),
+                    dim3(KA_MERGE_THREADS), 0, st, p);
 }
 
 }  // namespace cb
@@ -593,7 +837,7 @@ using namespace cb;
 
 extern "C" {
 
-// Bytes of workspace for cb_kv_attend, or -1: the call is too large for one launch.
+// Bytes of workspace for cb_kv_attend (0: none), or -1: the call is too large for one launch.
 long long cb_kv_attend_bytes(int B, int S, int Hq, int Hkv, int max_len) {
   KaLaunch s;
   if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || max_len < 1 || !ka_shape(&s, B, S, Hq, Hkv, max_len)) {
@@ -613,13 +857,14 @@ int cb_kv_attend(void* data, void* exps, int num_pages, int hkv, int page, const
   KvAttendParams p;
   int lg = 0;
   while ((1 << lg) < page) ++lg;
-  if (num_pages < 1 || page < 16 || page > 128 || (1 << lg) != page || cols < 1 || window < 0 || sinks < 0) {
+  if (num_pages < 1 || num_pages > KA_MAX_PAGES || page < 16 || page > 128 || (1 << lg) != page || cols < 1 || window < 0 || sinks < 0) {
     set_last_error("key/value attention: bad cache, window or sinks");
     return -1;
   }
   const long long need = cb_kv_attend_bytes(B, S, Hq, hkv, max_len);
   if (need < 0) return -1;
-  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) {
+  if (need > 0 &&
+      (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)) {
     set_last_error("key/value attention: workspace missing, misaligned or too small");
     return -1;
   }
@@ -643,16 +888,8 @@ int cb_kv_attend(void* data, void* exps, int num_pages, int hkv, int page, const
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = static_cast<uint32_t*>(status);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  static std::atomic<uint64_t> smem_done{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv_attend_kernel), KA_SMEM, smem_done);
-  if (e == cudaSuccess)
-    e = launch_pdl(kv_attend_kernel, dim3(static_cast<unsigned>(s.grid)), dim3(KA_WARPS * 32), KA_SMEM, st, p);
-  if (e == cudaSuccess) {
-    const long long rows = static_cast<long long>(B) * S * Hq;
-    const int per = KA_MERGE_THREADS / 32;
-    e = launch_pdl(kv_attend_merge_kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(KA_MERGE_THREADS), 0,
-                   st, p);
-  }
+  p.cluster = s.cluster;
+  const cudaError_t e = s.tile_rows == 16 ? ka_launch<KaCfg<1>>(p, s, st) : ka_launch<KaCfg<2>>(p, s, st);
   if (e != cudaSuccess) {
     cudaGetLastError();   // reported here, not by the next call
     set_last_error(std::string("key/value attention launch: ") + cudaGetErrorString(e));

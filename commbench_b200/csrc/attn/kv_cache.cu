@@ -25,60 +25,11 @@ struct KvAppendParams {
   long long k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, q_sb, q_ss, q_sh;
   RopeTableView rope;                               // rot = 0: none
   int hq, pages_per_seq, kv_blocks;
-  int wide;                                         // queries in vectors of 8 elements, else of 4
   RopeShare share;                                  // of the queries
   uint32_t* status;
 };
 
-// The lane's four elements d = 4 lane .. 4 lane + 3 of a head at `pos`, turned.  Warp-collective.
-struct LaneAngles {
-  float c[4], s[4];
-  bool low;          // elements of the first half (half layout)
-  int partner;       // lane that holds the other elements of the pairs
-  bool on;
-};
-__device__ __forceinline__ LaneAngles lane_angles(const RopeTableView& t, long long pos, int lane) {
-  LaneAngles a;
-  const int d = 4 * lane, half = t.rot / 2;
-  a.on = d < t.rot;
-  a.low = d < half;
-  a.partner = t.interleaved || !a.on ? lane : a.low ? lane + half / 4 : lane - half / 4;
-  const bool known = pos >= 0 && pos < t.positions;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a.c[i] = a.s[i] = __int_as_float(0x7fc00000);
-    if (a.on && known) {
-      const long long at = pos * half + (t.interleaved ? (d + i) / 2 : (a.low ? d : d - half) + i);
-      a.c[i] = __ldg(t.cos + at);
-      a.s[i] = __ldg(t.sin + at);
-    }
-  }
-  return a;
-}
-__device__ __forceinline__ void lane_rotate(const RopeTableView& t, const LaneAngles& a, float (&x)[4]) {
-  float y[4];
-  if (t.interleaved) {
-    rotate_pair(x[0], x[1], a.c[0], a.s[0], &y[0], &y[1]);
-    rotate_pair(x[2], x[3], a.c[2], a.s[2], &y[2], &y[3]);
-  } else {
-    float o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], a.partner);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float lo, hi;
-      rotate_pair(a.low ? x[i] : o[i], a.low ? o[i] : x[i], a.c[i], a.s[i], &lo, &hi);
-      y[i] = a.low ? lo : hi;
-    }
-  }
-  if (a.on) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = y[i];
-  }
-}
-
-static constexpr int KV_THREADS = 512;
-static constexpr int KV_WARPS = KV_THREADS / 32;
+static constexpr int KV_THREADS = 256;
 static constexpr int KV_Q_HEADS = 2;   // query heads whose loads a thread has in flight
 
 // The queries of p.share.tokens tokens.
@@ -107,19 +58,68 @@ __device__ __forceinline__ void append_queries(const KvAppendParams& p, int bloc
     rope_item<__nv_bfloat16, V, kHalf, KV_Q_HEADS>(p.rope, sh, r, pos, 1.f, hy, item);
 }
 
-// kTokens: token slots of a page per warp.
-template <int kTokens>
-__global__ void __launch_bounds__(KV_THREADS, kTokens <= 4 ? 2 : 1) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
-  __shared__ float sh_max[2][KV_WARPS];
+// A thread's share of a token's row: two pieces of V elements.  Half layout: a piece of the first half and its
+// partner, then pairs of pieces that are copied; interleaved: neighbours.
+template <int V>
+struct KvItem {
+  int d0, d1;
+  bool turn0, turn1;
+  __device__ __forceinline__ KvItem(const RopeTableView& t, int i) {
+    const int half = t.rot / 2;
+    if (t.interleaved || i * V >= half) {
+      d0 = t.interleaved ? 2 * i * V : t.rot + 2 * (i * V - half);
+      d1 = d0 + V;
+      turn0 = t.interleaved && d0 < t.rot;
+      turn1 = t.interleaved && d1 < t.rot;
+    } else {
+      d0 = i * V;
+      d1 = half + d0;
+      turn0 = turn1 = true;
+    }
+  }
+  __device__ __forceinline__ void turn(const RopeTableView& t, long long pos, float (&x)[2][V]) const {
+    if (!turn0) return;
+    const int half = t.rot / 2;
+    const bool known = pos >= 0 && pos < t.positions;
+    float c[V], s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);   // outside the table: NaN
+    if (known) {
+      const long long at = pos * half + (t.interleaved ? d0 / 2 : d0);
+#pragma unroll
+      for (int i = 0; i < V; i += V / 2)
+        if (!t.interleaved || i == 0 || turn1) {
+          load_vec<float, V / 2>(t.cos + at + i, reinterpret_cast<float(&)[V / 2]>(c[i]));
+          load_vec<float, V / 2>(t.sin + at + i, reinterpret_cast<float(&)[V / 2]>(s[i]));
+        }
+    }
+    if (t.interleaved) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (k == 0 || turn1) {
+#pragma unroll
+          for (int i = 0; i < V; i += 2)
+            rotate_pair(x[k][i], x[k][i + 1], c[(k * V + i) / 2], s[(k * V + i) / 2], &x[k][i], &x[k][i + 1]);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) rotate_pair(x[0][i], x[1][i], c[i], s[i], &x[0][i], &x[1][i]);
+    }
+  }
+};
+
+// V elements to a piece, kTokens token slots of the page per thread: 64 / V lanes share a row.
+template <int V, int kTokens>
+__global__ void __launch_bounds__(KV_THREADS, kTokens * V <= 16 ? 4 : 2)
+    kv_append_kernel(const __grid_constant__ KvAppendParams p) {
+  constexpr int kLanes = 64 / V, kRows = KV_THREADS / kLanes;
+  __shared__ uint32_t sh_max[2][KV_THREADS / 32];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (static_cast<int>(blockIdx.x) >= p.kv_blocks) {
     const int block = static_cast<int>(blockIdx.x) - p.kv_blocks;
-    if (p.rope.interleaved)
-      p.wide ? append_queries<8, false>(p, block) : append_queries<4, false>(p, block);
-    else
-      p.wide ? append_queries<8, true>(p, block) : append_queries<4, true>(p, block);
+    p.rope.interleaved ? append_queries<V, false>(p, block) : append_queries<V, true>(p, block);
     return;
   }
   const int hkv = p.cache.hkv, page = p.cache.page();
@@ -138,55 +138,75 @@ __global__ void __launch_bounds__(KV_THREADS, kTokens <= 4 ? 2 : 1) kv_append_ke
   const int lo = start > t0 ? static_cast<int>(start - t0) : 0;     // slots lo .. hi - 1 are new
   const long long left = static_cast<long long>(start) + count - t0;
   const int hi = left < page ? static_cast<int>(left) : page;
+  if (p.rope.rot > 0 && t0 + hi > p.rope.positions && threadIdx.x == 0)
+    report_status(p.status, CB_BAD_ARGUMENT, 1, 0xA01);
+  const KvItem<V> it(p.rope, threadIdx.x % kLanes);
+  const int row = threadIdx.x / kLanes;
 
   // Values first: a NaN among them is stored as 0 and put into the token's key instead, so that a query that
   // does not see the token has nothing to multiply by zero, and one that does answers NaN.
-  uint32_t bad = 0;                                                 // bit per token of the warp
+  uint32_t bad = 0;                                                 // bit per token of the thread
 #pragma unroll 1
   for (int side = 1; side >= 0; --side) {
     const __nv_bfloat16* src = side ? p.v + b * p.v_sb + head * p.v_sh : p.k + b * p.k_sb + head * p.k_sh;
     const long long ss = side ? p.v_ss : p.k_ss;
-    float x[kTokens][4];
+    Vec<__nv_bfloat16, V> raw[kTokens][2];
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
-      const int t = warp + KV_WARPS * i;
-      x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
-      if (t >= lo && t < hi) load_vec<__nv_bfloat16, 4>(src + (t0 + t - start) * ss + 4 * lane, x[i]);
+      const int t = row + kRows * i;
+      clear(raw[i][0]);
+      clear(raw[i][1]);
+      if (t >= lo && t < hi) {
+        const __nv_bfloat16* at = src + (t0 + t - start) * ss;
+        raw[i][0] = *reinterpret_cast<const Vec<__nv_bfloat16, V>*>(at + it.d0);
+        raw[i][1] = *reinterpret_cast<const Vec<__nv_bfloat16, V>*>(at + it.d1);
+      }
     }
-    if (side == 0 && p.rope.rot > 0) {
+    float x[kTokens][2][V];
+    uint32_t top = 0;                                               // bits of the largest |x|; NaN above all
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) {
+      const int t = row + kRows * i;
+      unpack(raw[i][0], x[i][0]);
+      unpack(raw[i][1], x[i][1]);
+      if (side == 0 && p.rope.rot > 0 && t >= lo && t < hi) it.turn(p.rope, t0 + t, x[i]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(x[i][k][j]) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) sh_max[side][warp] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, sh_max[side][lane % (KV_THREADS / 32)]);
+    if (top >= 0x7f800000u) {
+      // Infinities and NaN, seldom: the scale is that of the finite numbers, and infinities become the largest.
+      top = 0;
 #pragma unroll
       for (int i = 0; i < kTokens; ++i) {
-        const int t = warp + KV_WARPS * i;
-        if (t >= lo && t < hi) {
-          if (t0 + t >= p.rope.positions && lane == 0) report_status(p.status, CB_BAD_ARGUMENT, 1, 0xA01);
-          lane_rotate(p.rope, lane_angles(p.rope, t0 + t, lane), x[i]);
-        }
-      }
-    }
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTokens; ++i) {
-      if (side == 1) {
         bool nan = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          nan = nan || x[i][j] != x[i][j];
-          if (x[i][j] != x[i][j]) x[i][j] = 0.f;
-        }
-        if (__any_sync(0xffffffffu, nan)) bad |= 1u << i;
-      }
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = fabsf(x[i][j]);
-        amax = fmaxf(amax, a <= 3.4028234e38f ? a : 0.f);           // infinities become the largest number
+          for (int j = 0; j < V; ++j) {
+            const uint32_t a = __float_as_uint(x[i][k][j]) & 0x7fffffffu;
+            if (a < 0x7f800000u) top = max(top, a);
+            if (side == 1 && a > 0x7f800000u) {
+              nan = true;
+              x[i][k][j] = 0.f;
+            }
+          }
+        const uint32_t row_lanes = (kLanes == 32 ? 0xffffffffu : (1u << (kLanes & 31)) - 1u) << (lane / kLanes * kLanes);
+        if ((__ballot_sync(0xffffffffu, nan) & row_lanes) != 0u) bad |= 1u << i;
       }
+      top = __reduce_max_sync(0xffffffffu, top);
+      __syncthreads();
+      if (lane == 0) sh_max[side][warp] = top;
+      __syncthreads();
+      top = __reduce_max_sync(0xffffffffu, sh_max[side][lane % (KV_THREADS / 32)]);
     }
-    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-    if (lane == 0) sh_max[side][warp] = amax;
-    __syncthreads();
-    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(sh_max[side][lane & (KV_WARPS - 1)])));
     int8_t* exp_at = p.cache.exp_of(pid, head, side);
-    int e = kv_exponent(amax), e_old = e;
+    int e = kv_exponent(__uint_as_float(top)), e_old = e;
     if (lo > 0) {
       e_old = *exp_at;
       e = e > e_old ? e : e_old;
@@ -194,8 +214,8 @@ __global__ void __launch_bounds__(KV_THREADS, kTokens <= 4 ? 2 : 1) kv_append_ke
     uint8_t* tile = p.cache.tile(pid, head, side);
     if (e != e_old) {
       const float f = kv_pow2(e_old - e < -126 ? -126 : e_old - e);
-      for (int t = warp; t < lo; t += KV_WARPS) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(tile + kv_offset(t, 4 * lane));
+      for (int i = threadIdx.x; i < lo * (KV_D / 4); i += KV_THREADS) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(tile) + i;       // whole rows: where an element lies does not matter
         const uint32_t old = *at;
         const uint32_t h0 = kv_to_half2(old), h1 = kv_to_half2(old >> 16);
         const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
@@ -206,16 +226,34 @@ __global__ void __launch_bounds__(KV_THREADS, kTokens <= 4 ? 2 : 1) kv_append_ke
     const float inv = e == KV_EXP_MIN ? 0.f : kv_pow2(-e);          // the least exponent says: all zero
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
-      const int t = warp + KV_WARPS * i;
-      if (t >= lo && t < hi) {
-        if (side == 0 && lane == 0 && ((bad >> i) & 1u)) x[i][0] = __int_as_float(0x7fc00000);
-        *reinterpret_cast<uint32_t*>(tile + kv_offset(t, 4 * lane)) =
-            kv_encode4(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv);
+      const int t = row + kRows * i;
+      if (t < lo || t >= hi) continue;
+      if (side == 0 && it.d0 == 0 && ((bad >> i) & 1u)) x[i][0][0] = __int_as_float(0x7fc00000);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        Vec<uint32_t, V / 4> q;
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          q.w[j / 4] = kv_encode4(x[i][k][j] * inv, x[i][k][j + 1] * inv, x[i][k][j + 2] * inv, x[i][k][j + 3] * inv);
+        *reinterpret_cast<Vec<uint32_t, V / 4>*>(tile + kv_offset(t, k ? it.d1 : it.d0)) = q;
       }
     }
     if (lo > 0) __syncthreads();   // every warp has read the old exponent
     if (threadIdx.x == 0) *exp_at = static_cast<int8_t>(e);
   }
+}
+
+template <int V>
+static cudaError_t launch_append(const KvAppendParams& p, unsigned blocks, cudaStream_t st) {
+  constexpr int kRows = KV_THREADS * V / 64;
+  const dim3 grid(blocks), block(KV_THREADS);
+  const int tokens = p.cache.page() / kRows;
+  if (tokens <= 1) return launch_pdl(kv_append_kernel<V, 1>, grid, block, 0, st, p);
+  if (tokens == 2) return launch_pdl(kv_append_kernel<V, 2>, grid, block, 0, st, p);
+  if constexpr (V == 4) {
+    if (tokens == 8) return launch_pdl(kv_append_kernel<V, 8>, grid, block, 0, st, p);
+  }
+  return launch_pdl(kv_append_kernel<V, 4>, grid, block, 0, st, p);
 }
 
 struct KvReadParams {
@@ -303,12 +341,14 @@ int cb_kv_append(void* data, void* exps, int num_pages, int hkv, int page, const
   p.pages_per_seq = (S + page - 2) / page + 1;
   p.status = static_cast<uint32_t*>(status);
   const long long kv_blocks = static_cast<long long>(B) * p.pages_per_seq * hkv;
-  p.wide = rot % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0 &&
-           p.q_sb % 8 == 0 && p.q_ss % 8 == 0 && p.q_sh % 8 == 0;
+  // pieces of 8 elements where the layout of the pairs and the operands allow it, else of 4
+  bool wide = interleaved ? rot % 8 == 0 : rot % 16 == 0;
+  for (const void* x : {k, v, q, static_cast<const void*>(q_out)}) wide = wide && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  for (int i = 0; i < 9; ++i) wide = wide && strides[i] % 8 == 0;
   p.share = {};
   long long q_blocks = 0;
   if (q != nullptr) {
-    p.share.set(KV_THREADS, KV_D, rot, p.wide ? 8 : 4, !interleaved, hq, KV_Q_HEADS);
+    p.share.set(KV_THREADS, KV_D, rot, wide ? 8 : 4, !interleaved, hq, KV_Q_HEADS);
     q_blocks = (static_cast<long long>(B) * S + p.share.tokens - 1) / p.share.tokens;
   }
   const long long blocks = kv_blocks + q_blocks;
@@ -317,15 +357,9 @@ int cb_kv_append(void* data, void* exps, int num_pages, int hkv, int page, const
     return -1;
   }
   p.kv_blocks = static_cast<int>(kv_blocks);
-  const dim3 grid(static_cast<unsigned>(blocks)), block(KV_THREADS);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e;
-  switch (page) {
-    case 16: e = launch_pdl(kv_append_kernel<1>, grid, block, 0, st, p); break;
-    case 32: e = launch_pdl(kv_append_kernel<2>, grid, block, 0, st, p); break;
-    case 64: e = launch_pdl(kv_append_kernel<4>, grid, block, 0, st, p); break;
-    default: e = launch_pdl(kv_append_kernel<8>, grid, block, 0, st, p); break;
-  }
+  const cudaError_t e = wide ? launch_append<8>(p, static_cast<unsigned>(blocks), st)
+                             : launch_append<4>(p, static_cast<unsigned>(blocks), st);
   if (e != cudaSuccess) {
     cudaGetLastError();   // reported here, not by the next call
     set_last_error(std::string("key/value append launch: ") + cudaGetErrorString(e));

@@ -66,46 +66,72 @@ __device__ __forceinline__ float row_sum(float v, float (*sh)[32], int round) {
 
 enum NormMode : int { NORM_PLAIN = 0, NORM_SCALE = 1, NORM_POW2 = 2 };
 
-// 8-bit output of the V columns from `col` on: 128 / V neighbouring lanes hold a block.
-template <int V, int kMode>
-__device__ __forceinline__ void store_quantised(const NormParams& p, long long row, int col, const float (&y)[V],
-                                                bool active) {
-  float amax = 0.f;
+// 8-bit output of a thread's VPT vectors, `step` columns apart from `col0` on: 128 / V neighbouring lanes hold a block.
+// The power of two is read off the maximum's bits, max <= 1.75 * 2^8 * scale; the other scale costs two divisions,
+// of which each lane makes those of one vector (8192 x 8192: both in every lane 64 us instead of the copy's 44).
+template <int V, int VPT, int kMode>
+__device__ __forceinline__ void store_quantised(const NormParams& p, long long row, int col0, int step,
+                                                const float (&y)[VPT][V]) {
+  const int kblocks = p.D >> 7, lane = threadIdx.x & 31;
+  float scale[VPT], inv[VPT];
+  float mine = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) amax = fmaxf(amax, fabsf(y[i]));
+  for (int i = 0; i < VPT; ++i) {
+    float amax = 0.f;
 #pragma unroll
-  for (int o = 64 / V; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  float s = amax > 0.f ? amax / 448.f : 1.f;
-  const int kb = col >> 7, kblocks = p.D >> 7;
-  if constexpr (kMode == NORM_POW2) {
-    const uint32_t bits = __float_as_uint(s);
-    uint32_t e = (bits >> 23) & 0xffu;
-    if ((bits & 0x7fffffu) != 0u) ++e;
-    e = min(max(e, 1u), 254u);
-    s = __uint_as_float(e << 23);
-    if (active && (col & 127) == 0 && p.sf != nullptr) {
-      uint8_t* word = p.sf + (static_cast<long long>(kb >> 2) * p.rows + row) * 4;
-      word[kb & 3] = static_cast<uint8_t>(e);
-      if (kb == kblocks - 1)
-        for (int i = (kb & 3) + 1; i < 4; ++i) word[i] = 127;   // missing blocks: 1.0
+    for (int j = 0; j < V; ++j) amax = fmaxf(amax, fabsf(y[i][j]));
+#pragma unroll
+    for (int o = 64 / V; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if constexpr (kMode == NORM_POW2) {
+      const uint32_t bits = __float_as_uint(amax);
+      int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+      e = amax > 0.f ? min(max(e, 1), 253) : 127;
+      scale[i] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+      inv[i] = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+    } else {
+      if (lane % VPT == i) mine = amax;
     }
   }
-  if (!active) return;
-  if ((col & 127) == 0) p.scale[row * kblocks + kb] = s;
-  const float inv = 1.f / s;
-  uint32_t q[V / 4];
+  if constexpr (kMode == NORM_SCALE) {
+    const float s = mine > 0.f ? mine / 448.f : 1.f;
+    const float r = 1.f / s;
 #pragma unroll
-  for (int i = 0; i < V; i += 4) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[i] * inv, y[i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi =
-        __nv_cvt_float2_to_fp8x2(make_float2(y[i + 2] * inv, y[i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-    q[i / 4] = lo | (hi << 16);
+    for (int i = 0; i < VPT; ++i) {
+      const int from = (lane & ~(128 / V - 1)) + i;
+      scale[i] = __shfl_sync(0xffffffffu, s, from);
+      inv[i] = __shfl_sync(0xffffffffu, r, from);
+    }
   }
-  uint8_t* dst = static_cast<uint8_t*>(p.y) + row * p.D + col;
-  if constexpr (V == 8)
-    *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
-  else
-    *reinterpret_cast<uint32_t*>(dst) = q[0];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int col = col0 + i * step;
+    if (col >= p.D) continue;
+    if ((col & 127) == 0) {
+      const int kb = col >> 7;
+      p.scale[row * kblocks + kb] = scale[i];
+      if (kMode == NORM_POW2 && p.sf != nullptr) {
+        uint8_t* word = p.sf + (static_cast<long long>(kb >> 2) * p.rows + row) * 4;
+        word[kb & 3] = static_cast<uint8_t>(__float_as_uint(scale[i]) >> 23);
+        if (kb == kblocks - 1)
+          for (int k = (kb & 3) + 1; k < 4; ++k) word[k] = 127;   // missing blocks: 1.0
+      }
+    }
+    uint32_t q[V / 4];
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float f = inv[i];
+      const uint32_t lo =
+          __nv_cvt_float2_to_fp8x2(make_float2(y[i][j] * f, y[i][j + 1] * f), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi =
+          __nv_cvt_float2_to_fp8x2(make_float2(y[i][j + 2] * f, y[i][j + 3] * f), __NV_SATFINITE, __NV_E4M3);
+      q[j / 4] = lo | (hi << 16);
+    }
+    uint8_t* dst = static_cast<uint8_t*>(p.y) + row * p.D + col;
+    if constexpr (V == 8)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
+    else
+      *reinterpret_cast<uint32_t*>(dst) = q[0];
+  }
 }
 
 // VPT vectors of V columns per thread, `threads` threads a row (32 or the CTA).
@@ -165,12 +191,9 @@ __global__ void __launch_bounds__(VPT == 4 || VPT == 8 ? 512 : 1024) rms_norm_ke
 #pragma unroll
       for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rstd * w[j];
     }
-    if constexpr (kMode == NORM_PLAIN) {
-      if (active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
-    } else {
-      store_quantised<V, kMode>(p, row, col, h[i], active);
-    }
+    if (kMode == NORM_PLAIN && active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
   }
+  if constexpr (kMode != NORM_PLAIN) store_quantised<V, VPT, kMode>(p, row, t * V, threads * V, h);
 }
 
 // Many long rows: CTAs that stay, each with a ring of rows in shared memory that bulk copies fill ahead, so that the
@@ -186,7 +209,8 @@ __device__ __forceinline__ void ring_abandon(const volatile int* abort_flag) {
   while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
 }
 static constexpr int NORM_SLOTS = 6;
-static constexpr int NORM_RING_BYTES = 200 * 1024;   // of an SM
+// Of an SM.  Forward: 128 KB are as good as 200; gradient: two rows of three operands and two CTAs' worth ahead.
+static constexpr int NORM_RING_BYTES = 128 * 1024, NORM_BWD_RING_BYTES = 200 * 1024;
 
 template <class T, int V, int VPT, int kMode>
 __global__ void __launch_bounds__(512, 2)
@@ -262,12 +286,9 @@ __global__ void __launch_bounds__(512, 2)
       if (active && two) store_vec<T, V>(static_cast<T*>(p.h) + row * p.D + col, h[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rstd * w[i][j];
-      if constexpr (kMode == NORM_PLAIN) {
-        if (active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
-      } else {
-        store_quantised<V, kMode>(p, row, col, h[i], active);
-      }
+      if (kMode == NORM_PLAIN && active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
     }
+    if constexpr (kMode != NORM_PLAIN) store_quantised<V, VPT, kMode>(p, row, t * V, threads * V, h);
     if (++slot == ring.slots) slot = 0, phase ^= 1u;
   }
   ring_abandon(&abort_flag);
@@ -531,11 +552,11 @@ static int launch_bwd(const NormBwdParams& p0, float* dw, int grid, int threads,
     const int per_sm = 1024 / threads < 4 ? 1024 / threads : 4;
     p.ring.row_bytes = p.D * static_cast<int>(sizeof(T));
     const int slot = p.ring.row_bytes * (p.dh != nullptr ? 3 : 2);
-    p.ring.slots = NORM_RING_BYTES / per_sm / slot;
+    p.ring.slots = NORM_BWD_RING_BYTES / per_sm / slot;
     if (p.ring.slots > NORM_SLOTS) p.ring.slots = NORM_SLOTS;
     static std::atomic<uint64_t> smem_done{0};
     auto kernel = rms_norm_bwd_kernel<T, V, VPT, true>;
-    e = allow_smem(reinterpret_cast<const void*>(kernel), NORM_RING_BYTES, smem_done);
+    e = allow_smem(reinterpret_cast<const void*>(kernel), NORM_BWD_RING_BYTES, smem_done);
     if (e == cudaSuccess) e = launch_pdl(kernel, g, b, static_cast<size_t>(slot) * p.ring.slots, st, p);
   } else {
     e = launch_pdl(rms_norm_bwd_kernel<T, V, VPT, false>, g, b, 0, st, p);

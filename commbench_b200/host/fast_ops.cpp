@@ -620,20 +620,22 @@ PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   {
     NoGil g;
     const long long bytes = (tall ? g_kv_prefill_bytes : g_kv_attend_bytes)(b, s, hq, c.hkv, max_len);
-    if (bytes > 0) {
+    if (bytes >= 0) {
       o = empty(*q, q->sizes(), at::kBFloat16);
       lse = empty(*q, {B, Hq, S}, at::kFloat);
-      at::Tensor ws = empty(*q, {bytes}, at::kByte);
+      at::Tensor ws;
+      if (bytes > 0) ws = empty(*q, {bytes}, at::kByte);
+      void* work = bytes > 0 ? ws.mutable_data_ptr() : nullptr;
       if (tall)
         rc = g_kv_prefill(c.data->mutable_data_ptr(), c.exps->mutable_data_ptr(), c.num_pages, c.hkv, c.page,
                           q->const_data_ptr(), q->stride(1), q->stride(2), o.mutable_data_ptr(),
                           lse.mutable_data_ptr(), pages->const_data_ptr(), cols, start, count, b, s, hq, window, sinks,
-                          max_len, scale, ws.mutable_data_ptr(), bytes, status, current_stream());
+                          max_len, scale, work, bytes, status, current_stream());
       else
         rc = g_kv_attend(c.data->mutable_data_ptr(), c.exps->mutable_data_ptr(), c.num_pages, c.hkv, c.page,
                          q->const_data_ptr(), q->stride(0), q->stride(1), q->stride(2), o.mutable_data_ptr(),
                          lse.mutable_data_ptr(), pages->const_data_ptr(), cols, start, count, b, s, hq, window, sinks,
-                         max_len, scale, ws.mutable_data_ptr(), bytes, status, current_stream());
+                         max_len, scale, work, bytes, status, current_stream());
     }
   }
   if (rc == 0) return tuple_of({&o, &lse});

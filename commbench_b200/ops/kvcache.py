@@ -201,14 +201,16 @@ class KVCache8:
             n = (lib.cb_kv_prefill_bytes if long else lib.cb_kv_attend_bytes)(B, S, Hq, self.kv_heads, max_len)
             if n < 0:
                 raise CommError(f"key/value attention failed: {N.last_error()}")
-            ws = q.new_empty((n,), dtype=torch.uint8) if stream is None else \
-                N.new_empty_on(stream, q, (n,), torch.uint8, handed_out=False)
+            ws = None
+            if n > 0:
+                ws = q.new_empty((n,), dtype=torch.uint8) if stream is None else \
+                    N.new_empty_on(stream, q, (n,), torch.uint8, handed_out=False)
             strides = q.stride()[1:3] if long else q.stride()[:3]
             rc = (lib.cb_kv_prefill if long else lib.cb_kv_attend)(
                 self.data.data_ptr(), self.exps.data_ptr(), self.num_pages, self.kv_heads, self.page, q.data_ptr(),
                 *strides, o.data_ptr(), lse.data_ptr(), pages.data_ptr(), pages.shape[1], start.data_ptr(),
-                count.data_ptr() if count is not None else 0, B, S, Hq, window, sinks, max_len, sc, ws.data_ptr(), n,
-                status_ptr, N.raw_stream(stream))
+                count.data_ptr() if count is not None else 0, B, S, Hq, window, sinks, max_len, sc,
+                0 if ws is None else ws.data_ptr(), n, status_ptr, N.raw_stream(stream))
         if rc != 0:
             raise CommError(f"key/value attention failed: {N.last_error()}")
         return o, lse
