@@ -118,6 +118,7 @@ _HOT_ARGTYPES = {
     "cb_kv_read": [_P, _P, _I, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P, _P],
     "cb_kv_attend_bytes": [_I] * 5,
     "cb_kv_prefill_bytes": [_I] * 5,
+    "cb_kv_attend_form": [_I] * 6,
     "cb_kv_prefill": ([_P, _P, _I, _I, _I, _P, _L, _L, _P, _P, _P, _I, _P, _P] + [_I] * 6 +
                       [_F, _P, _L, _P, _P]),
     "cb_kv_attend": ([_P, _P, _I, _I, _I, _P, _L, _L, _L, _P, _P, _P, _I, _P, _P] + [_I] * 6 +
@@ -157,7 +158,7 @@ _FAST_ENTRIES = ("cb_gemm_bf16", "cb_gemm_fp8", "cb_gemm_fp8_blockscaled", "cb_g
                  "cb_quant_blockscaled", "cb_quant_blockscaled_pow2", "cb_attn_fwd4",
                  "cb_attn_split_bytes", "cb_attn_split", "cb_rms_norm", "cb_rms_norm_backward_floats",
                  "cb_rms_norm_backward", "cb_rope", "cb_kv_append", "cb_kv_read", "cb_kv_attend_bytes",
-                 "cb_kv_prefill_bytes", "cb_kv_attend", "cb_kv_prefill")
+                 "cb_kv_prefill_bytes", "cb_kv_attend_form", "cb_kv_attend", "cb_kv_prefill")
 
 
 class _NoFast:

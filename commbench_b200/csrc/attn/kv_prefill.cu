@@ -7,6 +7,7 @@
 // query head: 7000 tokens, 8 heads: 9 us of the call's.  e4m3 operands for the tensor cores would need the queries and the
 // probabilities in 8 bits too, or split in two terms of 4 bits, at the same rate as bf16.
 #include <cuda_runtime.h>
+#include <math.h>
 
 #include <string>
 
@@ -94,6 +95,25 @@ static long long prefill_room(int max_len) { return (static_cast<long long>(max_
 using namespace cb;
 
 extern "C" {
+
+// Which form takes a call: 1 this one, 0 cb_kv_attend, from a model of both in microseconds.
+//   Few rows: a key of a head costs 37 ps of the whole chip with a tile of 16 rows and 73 with two (16 sequences of
+// 24000 keys, 64 / 8 heads: 129 us with one tile, 222 with two), however the rows are spread over sequences.
+//   Many: a key of a head is expanded in 150 ps, and a pair of 128-row tiles of one query head visits 128 keys in 1.3 us on one SM.
+// 4 x 16 queries over 6000 keys, 64 / 8 heads, take 196 us here (256 items, 16 of 256 rows each) and 74 there.
+int cb_kv_attend_form(int B, int S, int Hq, int Hkv, int window, int max_len) {
+  if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || max_len < 1) return 0;
+  const float group = static_cast<float>(Hq / Hkv), rows = static_cast<float>(S) * group;
+  float keys = static_cast<float>(max_len);
+  if (window > 0 && static_cast<float>(window) + S < keys) keys = static_cast<float>(window) + S;
+  const float heads = static_cast<float>(B) * Hkv;
+  const float few = 14.f + heads * keys * (rows <= 16.f ? 37e-6f : 73e-6f * ceilf(rows / 32.f));
+  const float waves = ceilf(ceilf(static_cast<float>(S) / (2 * CP_BM)) * B * Hq / 148.f);
+  // a query in the middle of a chunk sees the chunk's first half
+  const float seen = window > 0 ? keys : keys - 0.5f * S;
+  const float many = 14.f + heads * keys * 150e-6f + waves * 1.3f * seen / CP_BN;
+  return many < few ? 1 : 0;
+}
 
 // Bytes of workspace for cb_kv_prefill, or -1.
 long long cb_kv_prefill_bytes(int B, int S, int Hq, int Hkv, int max_len) {

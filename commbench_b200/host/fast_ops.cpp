@@ -48,6 +48,7 @@ using KvAppendFn = int (*)(void*, void*, int, int, int, const void*, const void*
 using KvReadFn = int (*)(const void*, const void*, int, int, int, const void*, int, const void*, const void*, int, int,
                          void*, void*, void*, void*);
 using KvBytesFn = long long (*)(int, int, int, int, int);
+using KvFormFn = int (*)(int, int, int, int, int, int);
 using KvAttendFn = int (*)(void*, void*, int, int, int, const void*, long long, long long, long long, void*, void*,
                            const void*, int, const void*, const void*, int, int, int, int, int, int, float, void*,
                            long long, void*, void*);
@@ -62,6 +63,7 @@ RopeFn g_rope;
 KvAppendFn g_kv_append;
 KvReadFn g_kv_read;
 KvBytesFn g_kv_attend_bytes, g_kv_prefill_bytes;
+KvFormFn g_kv_form;
 KvAttendFn g_kv_attend;
 KvPrefillFn g_kv_prefill;
 GemmFn g_gemm_bf16, g_gemm_fp8;
@@ -590,8 +592,8 @@ PyObject* fast_kv_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
 }
 
 // kv_attend(data, exps, num_pages, kv_heads, page, q, pages, start, count | None, window, sinks, scale | None,
-// max_len, long, status_ptr): (o, lse).  long: the form for many query rows, which wants 16-byte rows and sequences
-// that follow each other.
+// max_len, status_ptr): (o, lse).  The form for many query rows wants 16-byte rows and sequences that follow each
+// other.
 PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   CB_TRY
   CacheArgs c;
@@ -599,8 +601,8 @@ PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   int window, sinks, max_len;
   float scale;
   const void *start, *count;
-  if (n != 15 || !modes_off() || !cache_of(v, &c) || !as_int(v[9], &window) || !as_int(v[10], &sinks) ||
-      window < 0 || sinks < 0 || !as_int(v[12], &max_len) || !PyBool_Check(v[13]) || !as_ptr(v[14], &status))
+  if (n != 14 || !modes_off() || !cache_of(v, &c) || !as_int(v[9], &window) || !as_int(v[10], &sinks) ||
+      window < 0 || sinks < 0 || !as_int(v[12], &max_len) || !as_ptr(v[13], &status))
     Py_RETURN_NONE;
   if (v[11] == Py_None) scale = static_cast<float>(1.0 / std::sqrt(128.0));
   else if (!as_float(v[11], &scale)) Py_RETURN_NONE;
@@ -608,7 +610,7 @@ PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (q == nullptr || pages == nullptr || pages->size(0) != q->size(0) || q->size(2) % c.hkv != 0) Py_RETURN_NONE;
   const int64_t B = q->size(0), S = q->size(1), Hq = q->size(2);
   if (!vector_of(v[7], B, false, &start) || !vector_of(v[8], B, true, &count)) Py_RETURN_NONE;
-  const bool tall = v[13] == Py_True;
+  const bool tall = g_kv_form(static_cast<int>(B), static_cast<int>(S), static_cast<int>(Hq), c.hkv, window, max_len) != 0;
   if (tall && ((reinterpret_cast<uintptr_t>(q->const_data_ptr()) & 15u) != 0 || q->stride(1) % 8 != 0 ||
                q->stride(2) % 8 != 0 || q->stride(1) <= 0 || q->stride(2) <= 0 ||
                (B > 1 && q->stride(0) != S * q->stride(1))))
@@ -665,11 +667,12 @@ PyObject* fast_bind(PyObject*, PyObject* d) {
   g_kv_read = reinterpret_cast<KvReadFn>(get("cb_kv_read"));
   g_kv_attend_bytes = reinterpret_cast<KvBytesFn>(get("cb_kv_attend_bytes"));
   g_kv_prefill_bytes = reinterpret_cast<KvBytesFn>(get("cb_kv_prefill_bytes"));
+  g_kv_form = reinterpret_cast<KvFormFn>(get("cb_kv_attend_form"));
   g_kv_attend = reinterpret_cast<KvAttendFn>(get("cb_kv_attend"));
   g_kv_prefill = reinterpret_cast<KvPrefillFn>(get("cb_kv_prefill"));
   if (PyErr_Occurred()) return nullptr;
   if (!g_norm || !g_norm_bwd_floats || !g_norm_bwd || !g_rope || !g_kv_append || !g_kv_read || !g_kv_attend_bytes ||
-      !g_kv_prefill_bytes || !g_kv_attend || !g_kv_prefill || !g_gemm_bf16 || !g_gemm_fp8 || !g_gemm_bs || !g_gemm_mx || !g_quant || !g_quant_pow2 || !g_attn ||
+      !g_kv_prefill_bytes || !g_kv_form || !g_kv_attend || !g_kv_prefill || !g_gemm_bf16 || !g_gemm_fp8 || !g_gemm_bs || !g_gemm_mx || !g_quant || !g_quant_pow2 || !g_attn ||
       !g_split_bytes || !g_split) {
     PyErr_SetString(PyExc_RuntimeError, "fast_ops.bind: an entry point is missing");
     return nullptr;

@@ -29,7 +29,6 @@ from ..utils.tracing import traced
 
 HEAD_DIM = 128
 _L9 = C.c_longlong * 9
-_FEW_ROWS = 64        # query rows per key/value head up to which a call is bound by the cache's bytes
 
 
 def _tileable(q):
@@ -164,13 +163,12 @@ class KVCache8:
         not read, and makes the rows that should see it meaningless.
 
         ``impl``: "decode" (few query rows, bound by the cache's bytes) or "prefill" (tcgen05 tiles over an expanded
-        copy); by default the number of rows decides."""
+        copy); by default a model of both decides."""
         if stream is None and impl is None and isinstance(q, torch.Tensor) and q.dim() == 4 and pages.dim() == 2:
             room = pages.shape[1] * self.page
             r = N.fast().kv_attend(self.data, self.exps, self.num_pages, self.kv_heads, self.page, q, pages, start,
                                    count, window, sinks, scale,
-                                   room if max_len is None or max_len > room else max(max_len, 1),
-                                   q.shape[1] * (q.shape[2] // self.kv_heads) > _FEW_ROWS, status_ptr)
+                                   room if max_len is None or max_len > room else max(max_len, 1), status_ptr)
             if r is not None:
                 return r
         _heads(q, "q")
@@ -193,7 +191,8 @@ class KVCache8:
         max_len = room if max_len is None else max(1, min(int(max_len), room))
         sc = scale if scale is not None else 1.0 / math.sqrt(HEAD_DIM)
         lib = N.load()
-        long = S * (Hq // self.kv_heads) > _FEW_ROWS if impl is None else impl == "prefill"
+        long = bool(lib.cb_kv_attend_form(B, S, Hq, self.kv_heads, window, max_len)) if impl is None else \
+            impl == "prefill"
         if long and not _tileable(q):
             with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(q.device)):
                 q = q.contiguous()
