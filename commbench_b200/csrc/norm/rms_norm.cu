@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(512, 2)
     const T* x = reinterpret_cast<const T*>(norm_smem + slot * slot_bytes);
     const T* r = reinterpret_cast<const T*>(norm_smem + slot * slot_bytes + ring.row_bytes);
     float h[VPT][V];
-    float ss = 0.f;
+    uint64_t ss2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int col = (i * threads + t) * V;
@@ -264,28 +264,41 @@ __global__ void __launch_bounds__(512, 2)
           float a[V];
           load_vec<T, V>(r + col, a);
 #pragma unroll
-          for (int j = 0; j < V; ++j) h[i][j] += a[j];
+          for (int j = 0; j < V; j += 2) {
+            const float2 f = f2_parts(f2_add(f2_pack(h[i][j], h[i][j + 1]), f2_pack(a[j], a[j + 1])));
+            h[i][j] = f.x;
+            h[i][j + 1] = f.y;
+          }
         }
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) h[i][j] = 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) ss += h[i][j] * h[i][j];
+      for (int j = 0; j < V; j += 2) {
+        const uint64_t h2 = f2_pack(h[i][j], h[i][j + 1]);
+        ss2 = f2_fma(h2, h2, ss2);
+      }
     }
-    ss = row_sum<false>(ss, sh, round);
+    const float2 parts = f2_parts(ss2);
+    const float ss = row_sum<false>(parts.x + parts.y, sh, round);
     if (t == 0) {
       const long long next = row + static_cast<long long>(ring.slots) * gridDim.x;
       if (next < p.rows) issue(next, slot);
     }
     const float rstd = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
+    const uint64_t r2 = f2_pack(rstd, rstd);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int col = (i * threads + t) * V;
       const bool active = col < p.D;
       if (active && two) store_vec<T, V>(static_cast<T*>(p.h) + row * p.D + col, h[i]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rstd * w[i][j];
+      for (int j = 0; j < V; j += 2) {
+        const float2 f = f2_parts(f2_mul(f2_mul(f2_pack(h[i][j], h[i][j + 1]), r2), f2_pack(w[i][j], w[i][j + 1])));
+        h[i][j] = f.x;
+        h[i][j + 1] = f.y;
+      }
       if (kMode == NORM_PLAIN && active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
     }
     if constexpr (kMode != NORM_PLAIN) store_quantised<V, VPT, kMode>(p, row, t * V, threads * V, h);
@@ -368,6 +381,7 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) rms_norm_bwd_kernel(con
     }
     W cy[VPT], ch[VPT], cd[VPT];
     float ss = 0.f, gh = 0.f;
+    uint64_t ss2 = 0, gh2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int col = (i * threads + t) * V;
@@ -383,26 +397,38 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) rms_norm_bwd_kernel(con
       weight(i, w);
       unpack(ch[i], a);
       unpack(cy[i], b);
+      if constexpr (V % 2 == 0) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        ss += a[j] * a[j];
-        gh += b[j] * w[j] * a[j];
+        for (int j = 0; j < V; j += 2) {
+          const uint64_t a2 = f2_pack(a[j], a[j + 1]);
+          ss2 = f2_fma(a2, a2, ss2);
+          gh2 = f2_fma(f2_mul(f2_pack(b[j], b[j + 1]), f2_pack(w[j], w[j + 1])), a2, gh2);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          ss += a[j] * a[j];
+          gh += b[j] * w[j] * a[j];
+        }
       }
     }
-    ss = warp_sum(ss);
-    gh = warp_sum(gh);
+    if constexpr (V % 2 == 0) {
+      const float2 x = f2_parts(ss2), y = f2_parts(gh2);
+      ss = x.x + x.y;
+      gh = y.x + y.y;
+    }
+    float2 both = warp_sum2(ss, gh);
     float(*s)[32] = sh[round & 1];
-    if (lane == 0) s[0][t >> 5] = ss, s[1][t >> 5] = gh;
+    if (lane == 0) s[0][t >> 5] = both.x, s[1][t >> 5] = both.y;
     __syncthreads();
     if (kRing && t == 0) {
       const long long next = row + static_cast<long long>(p.ring.slots) * gridDim.x;
       if (next < p.rows) issue(next, slot);
     }
     const bool have = lane < (threads >> 5);
-    ss = warp_sum(have ? s[0][lane] : 0.f);
-    gh = warp_sum(have ? s[1][lane] : 0.f);
-    const float rstd = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
-    const float c = rstd * rstd * rstd * (gh / static_cast<float>(p.D));
+    both = warp_sum2(have ? s[0][lane] : 0.f, have ? s[1][lane] : 0.f);
+    const float rstd = 1.f / sqrtf(both.x / static_cast<float>(p.D) + p.eps);
+    const float c = rstd * rstd * rstd * (both.y / static_cast<float>(p.D));
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int col = (i * threads + t) * V;
@@ -411,10 +437,25 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) rms_norm_bwd_kernel(con
       unpack(ch[i], a);
       unpack(cy[i], b);
       unpack(cd[i], dx);
+      if constexpr (V % 2 == 0) {
+        const uint64_t r2 = f2_pack(rstd, rstd), c2 = f2_pack(-c, -c);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        dx[j] += rstd * (b[j] * w[j]) - a[j] * c;
-        dw[i][j] += b[j] * (a[j] * rstd);
+        for (int j = 0; j < V; j += 2) {
+          const uint64_t a2 = f2_pack(a[j], a[j + 1]), b2 = f2_pack(b[j], b[j + 1]);
+          const uint64_t g2 = f2_mul(b2, f2_pack(w[j], w[j + 1]));
+          const float2 d = f2_parts(f2_fma(a2, c2, f2_fma(g2, r2, f2_pack(dx[j], dx[j + 1]))));
+          dx[j] = d.x;
+          dx[j + 1] = d.y;
+          const float2 e = f2_parts(f2_fma(b2, f2_mul(a2, r2), f2_pack(dw[i][j], dw[i][j + 1])));
+          dw[i][j] = e.x;
+          dw[i][j + 1] = e.y;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          dx[j] += rstd * (b[j] * w[j]) - a[j] * c;
+          dw[i][j] += b[j] * (a[j] * rstd);
+        }
       }
       if (col < p.D) store_vec<T, V>(static_cast<T*>(p.dx) + row * p.D + col, dx);
     }
