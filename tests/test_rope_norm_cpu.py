@@ -1,0 +1,45 @@
+"""Rotary frequencies, and the checks of the norm, rotary and cache operators that need no GPU."""
+import math
+
+import pytest
+import torch
+
+
+def test_frequencies():
+    from commbench_b200.ops.rope import RopeError, rope_frequencies
+
+    f, m = rope_frequencies(8, 10000.0)
+    assert m == 1.0 and torch.allclose(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-14)
+    f2, _ = rope_frequencies(8, 10000.0, dict(kind="linear", factor=2.0))
+    assert torch.equal(f2 * 2, f)
+    f3, _ = rope_frequencies(8, 10000.0, dict(kind="ntk", factor=2.0))
+    assert f3[0] == 1.0 and math.isclose(f3[-1] * 2, f[-1], rel_tol=1e-12)
+    f4, m4 = rope_frequencies(128, 10000.0, dict(kind="yarn", factor=8.0, original_positions=4096))
+    plain, _ = rope_frequencies(128)
+    ratio = f4 / plain
+    assert ratio[0] == 1.0 and math.isclose(ratio[-1], 1 / 8, rel_tol=1e-12) and (ratio.diff() <= 0).all()
+    assert math.isclose(m4, 0.1 * math.log(8) + 1)
+    for bad in (dict(kind="linear", factor=0.0), dict(kind="x"), dict()):
+        with pytest.raises(RopeError):
+            rope_frequencies(8, scaling=bad)
+    with pytest.raises(RopeError):
+        rope_frequencies(3)
+
+
+def test_tables_on_the_cpu():
+    from commbench_b200.ops.rope import RopeTable
+
+    t = RopeTable(64, 2000, device="cpu")
+    a = 1999.0 * 10000.0 ** (-2 / 64)
+    assert abs(t.cos[1999, 1].item() - math.cos(a)) < 1e-7 and t.cos.shape == (2000, 32)
+
+
+def test_sf_and_cache_shapes():
+    from commbench_b200.ops.kvcache import KVCache8
+    from commbench_b200.runtime.context import CommError
+
+    c = KVCache8(3, 2, page=16, device="cpu")
+    assert c.nbytes == 3 * 2 * 2 * 16 * 128 + 3 * 2 * 2
+    for bad in ((3, 2, 17), (0, 2, 16), (3, 0, 16), (3, 2, 256)):
+        with pytest.raises(CommError):
+            KVCache8(bad[0], bad[1], page=bad[2], device="cpu")
