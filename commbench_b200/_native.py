@@ -118,6 +118,9 @@ _HOT_ARGTYPES = {
     "cb_kv_read": [_P, _P, _I, _I, _I, _P, _I, _P, _P, _I, _I, _P, _P, _P, _P],
     "cb_kv_attend_bytes": [_I] * 5,
     "cb_kv_prefill_bytes": [_I] * 5,
+    "cb_kv_tiles_bytes": [_I] * 5,
+    "cb_kv_tiles": ([_P, _P, _I, _I, _I, _P, _L, _L, _L, _P, _P, _P, _I, _P, _P] + [_I] * 6 +
+                    [_F, _P, _L, _P, _P]),
     "cb_kv_attend_form": [_I] * 6,
     "cb_kv_prefill": ([_P, _P, _I, _I, _I, _P, _L, _L, _P, _P, _P, _I, _P, _P] + [_I] * 6 +
                       [_F, _P, _L, _P, _P]),
@@ -143,7 +146,7 @@ def load():
     lib = C.CDLL(str(_LIB_PATH), mode=C.RTLD_GLOBAL)
     lib.cb_last_error.restype = C.c_char_p
     for name in ("cb_symm_round_size", "cb_attn_split_bytes", "cb_rms_norm_backward_floats",
-                 "cb_kv_attend_bytes", "cb_kv_prefill_bytes"):
+                 "cb_kv_attend_bytes", "cb_kv_prefill_bytes", "cb_kv_tiles_bytes"):
         getattr(lib, name).restype = C.c_longlong
     for name, args in _HOT_ARGTYPES.items():
         getattr(lib, name).argtypes = args

@@ -1,0 +1,805 @@
+// Attention of a middling number of query rows over the paged 8-bit cache (kv_cache.cuh): drafts of several tokens with
+// many heads to a group, short chunks.
+//
+// Between the two other forms: too many rows for mma.sync, whose rate a tile of 32 rows uses up before the cache's
+// bytes have arrived, and too few query tiles to pay for an expanded copy of the keys and to fill the chip with them.
+// Here the products are tcgen05's and the expansion happens on the way to them:
+//   * the rows of a 128-row tile are (query token, head of the group) couples of one key/value head;
+//   * bulk copies bring 128 keys and values, 32 KB, as they lie in their pages into a ring of two; four warps expand
+//     them to fp16, exactly, into the swizzled tiles that the tensor cores read (a copy through memory would cost 5
+//     bytes an element instead of 1).  The scales of a block's pages are brought to the largest of them, so that one
+//     factor for the scores and one exponent for the probabilities serve the whole block; a value 2^24 below the
+//     largest of its block is lost;
+//   * two softmax streams take alternate blocks, each with its scores, probabilities (fp16) and results in tensor
+//     memory, as in fa_split.cu, and the flat list of (sequence, query tile, head, block) is cut evenly over the
+//     CTAs as there - by the lengths that the device holds.
+// Every mbarrier wait is bounded (see mbarrier.cuh).
+#include <math.h>
+
+#include <string>
+
+#include "../gemm/launch.h"
+#include "fa_cp.cuh"
+#include "kv_cache.cuh"
+
+namespace cb {
+void set_last_error(const std::string& s);
+
+static constexpr int KT_THREADS = 512;    // producer, MMA and two idle warps; 4 that expand; 2 x 4 of softmax
+static constexpr int KT_BN = 128;         // keys of a block
+static constexpr int KT_RING = 2;         // raw blocks, and tiles of keys and of values
+static constexpr int KT_RAW = 2 * KT_BN * KV_D;
+static constexpr int KT_TILES = CP_TILE + KT_RING * (2 * CP_TILE + KT_RAW);
+static constexpr int KT_MAX_ENTRIES = 96;
+static constexpr int KT_MIN_BLOCKS = 2;   // of a CTA
+static constexpr int KT_MERGE_THREADS = 128;
+
+struct KvTilesParams {
+  KvCacheView cache;
+  KvBatch batch;
+  const __nv_bfloat16* q;
+  long long q_sb, q_ss, q_sh;
+  __nv_bfloat16* o;              // [B, S, Hq, 128]
+  float* lse;                    // [B, Hq, S]
+  float* part_o;                 // [CTA][taken over / handed on][tile row][128] unnormalised
+  float2* part_ml;               // [CTA][taken over / handed on][tile row] {max (log2 units), sum}
+  uint32_t* plan;                // [entries + 2]: blocks before each (sequence, query tile), blocks per CTA
+  int Hq, group, qrows, nqt, window, sinks;
+  float scale_log2;
+  uint32_t* status;
+};
+
+struct KtCtl {
+  uint64_t raw_full[KT_RING], raw_empty[KT_RING], q_full, q_empty;
+  uint64_t k_full[KT_RING], k_empty[KT_RING], v_full[KT_RING], v_empty[KT_RING];
+  uint64_t sc_full[4];
+  uint64_t s_full[2], p_first[2], p_rest[2], pv_done[2], seg_full, seg_done;
+  float2 sc[4];                    // of a block: factor of the scores, exponent of the values
+  alignas(16) uint16_t exps[KT_RING][8];   // of a raw block's pages: key, value << 8
+  int8_t row_exp[2][CP_BM];        // rows were multiplied by 2^-e; of a segment and the next
+  float2 ml[2][CP_BM];             // (max, sum) of the segment per stream and row
+  uint32_t tmem_base;
+  int abort_flag;
+  uint32_t base[KT_MAX_ENTRIES + 1];
+};
+static constexpr int KT_SMEM = KT_TILES + static_cast<int>(sizeof(KtCtl));
+static_assert(KT_SMEM <= 232448, "over the 227 KB shared-memory limit");
+
+// The blocks that the queries of a (sequence, query tile) see: the first `sink`, then `first` and on; n in all.
+struct KtSpan {
+  int start, count, q_first, sink, first, n;
+};
+__device__ __forceinline__ KtSpan kt_span(const KvTilesParams& p, int entry) {
+  KtSpan s;
+  const int b = entry / p.nqt, qt = entry - b * p.nqt;
+  s.start = p.batch.start[b];
+  s.count = p.batch.new_tokens(b);
+  if (s.start < 0) s.start = 0, s.count = 0;
+  const int t0 = qt * p.qrows, last = min(s.count, t0 + p.qrows) - 1;
+  s.q_first = s.start + t0;
+  s.sink = s.first = 0;
+  if (p.window > 0) {
+    const int low = s.q_first - p.window + 1;
+    s.first = low > 0 ? low / KT_BN : 0;
+    s.sink = min((p.sinks + KT_BN - 1) / KT_BN, s.first);
+  }
+  s.n = last >= t0 ? s.sink + (s.start + last) / KT_BN - s.first + 1 : 1;   // without a query: one, all hidden
+  return s;
+}
+
+// The segments of one CTA's range of the flat list; every role walks its own copy.
+struct KtWalk {
+  KtSpan span;
+  uint32_t pos, end;
+  int entry, head, k0, n;   // blocks k0 .. k0 + n - 1 of the item
+  __device__ __forceinline__ bool locate(const KvTilesParams& p, const KtCtl& ctl) {
+    if (pos >= end) return false;
+    while (pos >= ctl.base[entry + 1]) ++entry;
+    span = kt_span(p, entry);
+    const uint32_t in = pos - ctl.base[entry];
+    head = static_cast<int>(in / span.n);
+    k0 = static_cast<int>(in) - head * span.n;
+    n = span.n - k0;
+    if (static_cast<uint32_t>(n) > end - pos) n = static_cast<int>(end - pos);
+    return true;
+  }
+  __device__ __forceinline__ bool start(const KvTilesParams& p, const KtCtl& ctl, uint32_t per, uint32_t total) {
+    const unsigned long long e = static_cast<unsigned long long>(blockIdx.x + 1) * per;
+    pos = blockIdx.x * per;
+    end = e < total ? static_cast<uint32_t>(e) : total;
+    entry = 0;
+    return locate(p, ctl);
+  }
+  __device__ __forceinline__ bool next(const KvTilesParams& p, const KtCtl& ctl) {
+    pos += n;
+    return locate(p, ctl);
+  }
+  __device__ __forceinline__ int key0(int j) const {   // first key of the segment's j-th block
+    const int i = k0 + j;
+    return (i < span.sink ? i : span.first + i - span.sink) * KT_BN;
+  }
+};
+
+// 16 e4m3 numbers of a row, times a power of two, as fp16 into a swizzled tile: its row, its chunk of 16 columns.
+__device__ __forceinline__ void kt_expand(const uint8_t* raw, uint8_t* tile, int row, int chunk, __half2 f, bool scaled) {
+  const uint4 x = *reinterpret_cast<const uint4*>(raw + row * KV_D + ((chunk ^ (row & 7)) << 4));
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(h[2 * i]), "=r"(h[2 * i + 1])
+        : "r"(w[i]));
+  }
+  if (scaled) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), f);
+      h[i] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+  }
+  uint8_t* dst = tile + (chunk >> 2) * CP_SUB + row * 128;
+  const int c0 = 2 * (chunk & 3);
+  *reinterpret_cast<uint4*>(dst + ((c0 ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+__device__ __forceinline__ void kt_store8(float* dst, const float* v) {   // a whole sector
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+// The scores FROM ... TO-1 become fp16 probabilities, two to a word, in s[FROM / 2 ...], their sums go to sum4.
+template <int FROM, int TO>
+__device__ __forceinline__ void kt_probabilities(uint32_t (&s)[128], float scale, float plus, uint64_t (&sum4)[4]) {
+  const uint64_t scale2 = cp_pack(scale, scale), plus2 = cp_pack(plus, plus);
+#pragma unroll
+  for (int i = FROM; i < TO; i += 2) {
+    const uint64_t y = cp_fma2(cp_pack_u(s[i], s[i + 1]), scale2, plus2);
+    const float p0 = cp_ex2(__uint_as_float(static_cast<uint32_t>(y)));
+    const float p1 = cp_ex2(__uint_as_float(static_cast<uint32_t>(y >> 32)));
+    sum4[(i >> 1) & 3] = cp_add2(sum4[(i >> 1) & 3], cp_pack(p0, p1));
+    const __half2 h = __floats2half2_rn(p0, p1);
+    s[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+__global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_constant__ KvTilesParams p) {
+  extern __shared__ __align__(1024) uint8_t kt_smem[];
+  uint8_t* sQ = kt_smem;
+  if ((smem_u32(sQ) & 1023u) != 0u) {
+    if (threadIdx.x == 0) report_status(p.status, CB_BAD_ARGUMENT, 0, 0xA3F);
+    return;
+  }
+  uint8_t* sK = sQ + CP_TILE;
+  uint8_t* sV = sK + KT_RING * CP_TILE;
+  uint8_t* sR = sV + KT_RING * CP_TILE;
+  KtCtl& ctl = *reinterpret_cast<KtCtl*>(kt_smem + KT_TILES);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const int tile_rows = p.qrows * p.group;
+  const uint32_t active = static_cast<uint32_t>(tile_rows + 31) / 32;   // softmax warps per stream
+  const int entries = p.batch.B * p.nqt;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < KT_RING; ++i) {
+      mbar_init(&ctl.raw_full[i], 1);
+      mbar_init(&ctl.raw_empty[i], 4);
+      mbar_init(&ctl.k_full[i], 4);
+      mbar_init(&ctl.k_empty[i], 1);
+      mbar_init(&ctl.v_full[i], 4);
+      mbar_init(&ctl.v_empty[i], 1);
+    }
+    mbar_init(&ctl.q_full, 4);
+    mbar_init(&ctl.q_empty, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&ctl.sc_full[i], 4);
+    mbar_init(&ctl.seg_full, 2 * active);
+    mbar_init(&ctl.seg_done, 2 * active);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl.s_full[i], 1);
+      mbar_init(&ctl.p_first[i], active);
+      mbar_init(&ctl.p_rest[i], active);
+      mbar_init(&ctl.pv_done[i], 1);
+    }
+    ctl.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl.tmem_base, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  if (warp == 0) {                                          // blocks before each entry
+    uint32_t before = 0;
+    for (int e0 = 0; e0 < entries; e0 += 32) {
+      const int e = e0 + static_cast<int>(lane);
+      const uint32_t mine = e < entries ? static_cast<uint32_t>(kt_span(p, e).n) * p.cache.hkv : 0u;
+      uint32_t x = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= static_cast<uint32_t>(o)) x += y;
+      }
+      if (e < entries) ctl.base[e] = before + x - mine;
+      before += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) ctl.base[entries] = before;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t total = ctl.base[entries];
+  const uint32_t even = (total + gridDim.x - 1) / gridDim.x;
+  const uint32_t per = even < KT_MIN_BLOCKS ? KT_MIN_BLOCKS : even;
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= entries + 1; e += KT_THREADS) p.plan[e] = e <= entries ? ctl.base[e] : per;
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl.tmem_base);
+  // stream t: S (fp32, 128 columns; the first 64 hold P as fp16 pairs after the softmax) at column 256 t, O at column
+  // 256 t + 128.
+
+  // 128 x (64 + 80 + 184 + 184) registers = 65,536, what 512 threads x 128 were launched with.
+  if (warp < 4) {
+    cp_reg_dec<64>();
+    if (warp == 0) {
+      // ---------------------------------------------------------------- producer: raw blocks
+      const int lg = p.cache.page_log2, pages = KT_BN >> lg;
+      const uint32_t bytes = static_cast<uint32_t>(KV_D) << lg;
+      KtWalk w;
+      bool ok = true;
+      uint32_t g = 0;
+      for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl)) {
+        const int b = w.entry / p.nqt, end = w.span.start + w.span.count;
+        const int* row = p.batch.pages + static_cast<long long>(b) * p.batch.cols;
+        // lane l looks page l of a block up, a block ahead
+        int pid = 0;
+        uint32_t ex = 0;
+        auto look_up = [&](int j) {
+          pid = 0;
+          ex = 0;
+          const int at = w.key0(j) + (static_cast<int>(lane) << lg);
+          if (j >= w.n || static_cast<int>(lane) >= pages || at >= end) return;
+          const int col = at >> lg;
+          pid = col < p.batch.cols ? row[col] : -1;
+          if (pid < 0 || pid >= p.cache.num_pages) {
+            report_status(p.status, CB_BAD_ARGUMENT, 2, 0xA04);
+            pid = 0;
+          }
+          ex = *reinterpret_cast<const uint16_t*>(p.cache.exp_of(pid, w.head, 0));
+        };
+        look_up(0);
+        for (int j = 0; ok && j < w.n; ++j, ++g) {
+          const uint32_t s = g % KT_RING;
+          if (g >= KT_RING)
+            ok = mbar_wait_warp(&ctl.raw_empty[s], (g / KT_RING - 1) & 1u, &ctl.abort_flag, p.status, 0xA30);
+          if (!ok) break;
+          if (lane < 8) ctl.exps[s][lane] = static_cast<uint16_t>(ex);   // pages that are not there: 0
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(&ctl.raw_full[s], KT_RAW);
+          __syncwarp();
+          const int src = __shfl_sync(0xffffffffu, pid, lane >> 1);
+          if (static_cast<int>(lane) < 2 * pages)
+            bulk_load_1d(sR + s * KT_RAW + (lane & 1u) * (KT_BN * KV_D) + (lane >> 1) * bytes,
+                         p.cache.tile(src, w.head, lane & 1u), bytes, &ctl.raw_full[s]);
+          look_up(j + 1);
+        }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------- MMA
+      // The whole warp walks the schedule and waits; one elected lane issues.
+      constexpr uint32_t idesc_s = make_idesc(128, 128, 0u);
+      constexpr uint32_t idesc_pv = make_idesc(128, 128, 0u) | (1u << 16);  // V is MN-major
+      const uint64_t q_desc = make_sw128_kmajor_desc(smem_u32(sQ));
+      const uint64_t k_desc0 = make_sw128_kmajor_desc(smem_u32(sK));
+      const uint64_t v_desc0 = cp_mnmajor_desc(smem_u32(sV));
+      constexpr uint64_t kTileStep = static_cast<uint64_t>(CP_TILE >> 4);
+      constexpr uint64_t kSubStep = static_cast<uint64_t>(CP_SUB >> 4);
+      auto wait_all = [&](uint64_t* bar, uint32_t parity, uint32_t detail) -> bool {
+        return mbar_wait_warp(bar, parity, &ctl.abort_flag, p.status, detail);
+      };
+      uint32_t g0 = 0;                 // blocks before this segment
+      uint32_t pv_count[2] = {0u, 0u};
+      auto issue_qk = [&](int j, bool last) -> bool {
+        const uint32_t g = g0 + j, s = g % KT_RING, t = j & 1;
+        if (!wait_all(&ctl.k_full[s], (g / KT_RING) & 1u, 0xA31)) return false;
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint64_t ka = k_desc0 + s * kTileStep;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t off = (kk >> 2) * kSubStep + 2u * (kk & 3);
+            mma_bf16_ss(tmem + 256u * t, q_desc + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&ctl.s_full[t]);
+          mma_commit(&ctl.k_empty[s]);
+          if (last) mma_commit(&ctl.q_empty);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_pv = [&](int j) -> bool {
+        const uint32_t g = g0 + j, s = g % KT_RING, t = j & 1;
+        const uint32_t par = pv_count[t] & 1u;
+        if (!wait_all(&ctl.p_first[t], par, 0xA32)) return false;
+        if (!wait_all(&ctl.v_full[s], (g / KT_RING) & 1u, 0xA33)) return false;
+        ++pv_count[t];
+        tc_fence_after_sync();
+        const uint64_t va = v_desc0 + s * kTileStep;
+        const uint32_t d = tmem + 256u * t + 128u;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_bf16_ts(d, tmem + 256u * t + 8u * kk, va + kk * (2048u >> 4), idesc_pv, (j > 1 || kk > 0) ? 1u : 0u);
+        }
+        __syncwarp();
+        if (!wait_all(&ctl.p_rest[t], par, 0xA34)) return false;
+        tc_fence_after_sync();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 4; kk < 8; ++kk)
+            mma_bf16_ts(d, tmem + 256u * t + 8u * kk, va + kk * (2048u >> 4), idesc_pv, 1u);
+          mma_commit(&ctl.pv_done[t]);
+          mma_commit(&ctl.v_empty[s]);
+        }
+        __syncwarp();
+        return true;
+      };
+      KtWalk w;
+      bool ok = true;
+      uint32_t seg = 0;
+      for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
+        ok = wait_all(&ctl.q_full, seg & 1u, 0xA35);
+        for (int j = 0; ok && j < 2 && j < w.n; ++j) ok = issue_qk(j, j + 1 == w.n);
+        for (int j = 0; ok && j < w.n; ++j) {
+          // A stream's first product of a segment overwrites the O of its last one: that was read before its softmax
+          // warps hand over (p_first) the first block of this segment.
+          ok = issue_pv(j);
+          if (ok && j + 2 < w.n) ok = issue_qk(j + 2, j + 3 == w.n);
+        }
+        g0 += w.n;
+      }
+    }
+  } else if (warp < 8) {
+    cp_reg_dec<80>();
+    // ------------------------------------------------------------------- expansion
+    const int tid = static_cast<int>(threadIdx.x) - 128;
+    const int lg = p.cache.page_log2;
+    auto arrive = [&](uint64_t* bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto wait_all = [&](uint64_t* bar, uint32_t parity, uint32_t detail) -> bool {
+      return mbar_wait_warp(bar, parity, &ctl.abort_flag, p.status, detail);
+    };
+    KtWalk w;
+    bool ok = true;
+    uint32_t seg = 0, g = 0;
+    for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
+      if (seg > 0) ok = wait_all(&ctl.q_empty, (seg - 1) & 1u, 0xA36);
+      if (!ok) break;
+      // Queries: eight lanes take a row, brought to [1, 2) by a power of two so that fp16 holds it.
+      {
+        const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, chunk = tid & 7;
+#pragma unroll 1
+        for (int r = tid >> 3; r < CP_BM; r += 16) {
+          const int in = r / p.group, tok = qt * p.qrows + in;
+          const bool there = r < tile_rows && tok < w.span.count;
+          const __nv_bfloat16* src = p.q + b * p.q_sb + tok * p.q_ss +
+                                     static_cast<long long>(w.head * p.group + r - in * p.group) * p.q_sh + 16 * chunk;
+          float x[16];
+          float amax = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint2 raw = there ? *reinterpret_cast<const uint2*>(src + 4 * i) : make_uint2(0u, 0u);
+            const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+            const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+            x[4 * i] = f0.x, x[4 * i + 1] = f0.y, x[4 * i + 2] = f1.x, x[4 * i + 3] = f1.y;
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))));
+          }
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+          e = e < -60 ? -60 : e > 100 ? 100 : e;
+          const float down = kv_pow2(-e);
+          uint32_t h[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __half2 y = __floats2half2_rn(x[2 * i] * down, x[2 * i + 1] * down);
+            h[i] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          uint8_t* dst = sQ + (chunk >> 2) * CP_SUB + r * 128;
+          const int c0 = 2 * (chunk & 3);
+          *reinterpret_cast<uint4*>(dst + ((c0 ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+          if (chunk == 0) ctl.row_exp[seg & 1u][r] = static_cast<int8_t>(e);
+        }
+      }
+      fence_proxy_async_smem();
+      arrive(&ctl.q_full);
+      // A thread: rows (tid & 7) + 8 (tid >> 6) + 16 i, one chunk of 16 columns; eight lanes write eight rows.
+      const int row0 = (tid & 7) + 8 * (tid >> 6), chunk = (tid >> 3) & 7;
+      for (int j = 0; ok && j < w.n; ++j, ++g) {
+        const uint32_t s = g % KT_RING, par = (g / KT_RING) & 1u;
+        ok = wait_all(&ctl.raw_full[s], par, 0xA37);
+        if (ok && g >= KT_RING) ok = wait_all(&ctl.k_empty[s], par ^ 1u, 0xA38);
+        if (!ok) break;
+        const uint4 e4 = *reinterpret_cast<const uint4*>(ctl.exps[s]);
+        const uint32_t ew[4] = {e4.x, e4.y, e4.z, e4.w};
+        int ek[8], ev[8], top_k = KV_EXP_MIN, top_v = KV_EXP_MIN;
+        const int pages = KT_BN >> lg;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t x = ew[i >> 1] >> (16 * (i & 1));
+          ek[i] = static_cast<int8_t>(x);
+          ev[i] = static_cast<int8_t>(x >> 8);
+          // only pages with keys that exist
+          if (i < pages && w.key0(j) + (i << lg) < w.span.start + w.span.count) {
+            top_k = max(top_k, ek[i]);
+            top_v = max(top_v, ev[i]);
+          }
+        }
+        if (top_k == KV_EXP_MIN) top_k = 0;   // all zero
+        if (top_v == KV_EXP_MIN) top_v = 0;
+        if (tid == 0) ctl.sc[g & 3u] = make_float2(kv_pow2(top_k), static_cast<float>(top_v));
+        arrive(&ctl.sc_full[g & 3u]);
+        bool same_k = true, same_v = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          same_k = same_k && (i >= pages || ek[i] == top_k);
+          same_v = same_v && (i >= pages || ev[i] == top_v);
+        }
+        // 2^(e - top) of the 16 keys of step i; what is 2^24 below is lost, what lies past the end is anything finite
+        auto factor = [&](const int(&e)[8], int top, int i) {
+          int x = 0;
+          const int page = (16 * i) >> lg;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k == page) x = e[k] - top;
+          x = x > 0 ? 0 : x < -126 ? -126 : x;
+          return __float2half2_rn(kv_pow2(x));
+        };
+        const uint8_t* raw = sR + s * KT_RAW;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          kt_expand(raw, sK + s * CP_TILE, row0 + 16 * i, chunk, same_k ? __half2() : factor(ek, top_k, i), !same_k);
+        fence_proxy_async_smem();
+        arrive(&ctl.k_full[s]);
+        if (g >= KT_RING) ok = wait_all(&ctl.v_empty[s], par ^ 1u, 0xA39);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          kt_expand(raw + KT_BN * KV_D, sV + s * CP_TILE, row0 + 16 * i, chunk, same_v ? __half2() : factor(ev, top_v, i),
+                    !same_v);
+        fence_proxy_async_smem();
+        arrive(&ctl.v_full[s]);
+        arrive(&ctl.raw_empty[s]);
+      }
+    }
+  } else {
+    cp_reg_inc<184>();
+    // ----------------------------------------------------------------- softmax
+    const int t = warp >= 12 ? 1 : 0;
+    const uint32_t q = warp & 3u;
+    const int r = static_cast<int>(q * 32u + lane);        // tile row of this thread
+    const uint32_t lane_addr = (q * 32u) << 16;
+    const uint32_t tS = tmem + 256u * t + lane_addr;
+    const uint32_t tO = tS + 128u;
+    const int q_in_tile = r / p.group;
+    KtWalk w;
+    bool ok = q < active;
+    uint32_t count = 0;                                    // blocks this stream has seen
+    uint32_t seg = 0, g0 = 0;
+    for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
+      const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, tok = qt * p.qrows + q_in_tile;
+      const bool query = r < tile_rows && tok < w.span.count;
+      const bool padded = __any_sync(0xffffffffu, !query);   // the loads of tensor memory below want a converged warp
+      const int tile_first = w.span.q_first, q_pos = w.span.start + tok;
+      const int tile_last = tile_first + p.qrows - 1;
+      float m_ref = -INFINITY, l = 0.f, row_scale = 0.f;
+      for (int j = t; ok && j < w.n; j += 2) {
+        const uint32_t g = g0 + j;
+        ok = mbar_wait(&ctl.sc_full[g & 3u], (g >> 2) & 1u, &ctl.abort_flag, p.status, 0xA3A) &&
+             mbar_wait(&ctl.s_full[t], count & 1u, &ctl.abort_flag, p.status, 0xA3B);
+        if (!ok) break;
+        ++count;
+        tc_fence_after_sync();
+        const float2 sc = ctl.sc[g & 3u];
+        if (j == t) row_scale = p.scale_log2 * kv_pow2(ctl.row_exp[seg & 1u][r]);
+        const float scale = fmaxf(row_scale * sc.x, 1.2e-38f);
+        uint32_t s[128];
+        tmem_ld_32x32_at(tS, &s[0]);
+        tmem_ld_32x32_at(tS + 32u, &s[32]);
+        tmem_ld_32x32_at(tS + 64u, &s[64]);
+        tmem_ld_32x32_at(tS + 96u, &s[96]);
+        tmem_wait_ld();
+        const int key0 = w.key0(j);
+        if (key0 + KT_BN - 1 > tile_first || padded) cp_mask_tail(s, query ? q_pos - key0 + 1 : 0);
+        if (p.window > 0 && key0 <= tile_last - p.window && key0 + KT_BN > p.sinks)
+          cp_mask_range(s, max(p.sinks - key0, 0), min(q_pos - p.window + 1 - key0, KT_BN));
+        float mx8[8];
+        cp_row_max(s, mx8);
+        const float mx_all = cp_max3(fmaxf(cp_max3(mx8[0], mx8[1], mx8[2]), cp_max3(mx8[3], mx8[4], mx8[5])), mx8[6], mx8[7]);
+        const float mx = fmaf(mx_all, scale, sc.y);
+        // The running maximum, raised when a score passes it by 2^8, for all rows of the warp (see cp_update_max).
+        const bool grow = query && (mx > m_ref + CP_RESCALE_THRESHOLD || (m_ref == -INFINITY && mx > -INFINITY));
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = query ? fmaxf(m_ref, mx) : m_ref;
+          const float alpha = m_ref == -INFINITY ? 0.f : cp_ex2(m_ref - m_new);
+          m_ref = m_new;
+          l *= alpha;
+          if (j > 1) {   // these scores being complete implies that the previous product is: O is stable
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32(tO + c * 32u, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32(tO + c * 32u, o);
+            }
+          }
+        }
+        const float plus = sc.y - (m_ref == -INFINITY ? 0.f : m_ref);
+        uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull};
+        kt_probabilities<0, 64>(s, scale, plus, sum4);
+        tmem_st_32x32_at(tS, &s[0]);
+        tmem_wait_st();
+        // Both streams' O of the segment before must have been read before this hand-over.
+        if (j < 2 && seg > 0 && !mbar_wait(&ctl.seg_done, (seg - 1) & 1u, &ctl.abort_flag, p.status, 0xA3C)) {
+          ok = false;
+          break;
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.p_first[t]);
+        kt_probabilities<64, 128>(s, scale, plus, sum4);
+        tmem_st_32x32_at(tS + 32u, &s[32]);
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.p_rest[t]);
+        float sum = 0.f;
+        cp_add_sums(sum4, sum);
+        l = fmaf(sum, kv_pow2(-static_cast<int>(sc.y)), l);
+      }
+      if (!ok) break;
+      // -------------------------------------------- end of the segment: merge the streams
+      if (t < w.n) {
+        ok = mbar_wait(&ctl.pv_done[t], (count - 1u) & 1u, &ctl.abort_flag, p.status, 0xA3D);
+      } else if (seg > 0) {   // no block, so no wait for the last segment's readers yet
+        ok = mbar_wait(&ctl.seg_done, (seg - 1) & 1u, &ctl.abort_flag, p.status, 0xA3E);
+      }
+      if (!ok) break;
+      ctl.ml[t][r] = make_float2(m_ref, l);
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.seg_full);
+      if (!mbar_wait(&ctl.seg_full, seg & 1u, &ctl.abort_flag, p.status, 0xA40)) break;
+      tc_fence_after_sync();
+      const float2 ml0 = ctl.ml[0][r], ml1 = ctl.ml[1][r];
+      const float m = fmaxf(ml0.x, ml1.x);
+      // A stream without a visible key has no O: its columns may hold anything.  (A NaN sum counts as visible.)
+      const bool use0 = ml0.y != 0.f, use1 = ml1.y != 0.f;
+      const float a0 = use0 ? (ml0.x == m ? 1.f : exp2f(ml0.x - m)) : 0.f;
+      const float a1 = use1 ? (ml1.x == m ? 1.f : exp2f(ml1.x - m)) : 0.f;
+      const float lsum = (use0 ? a0 * ml0.y : 0.f) + (use1 ? a1 * ml1.y : 0.f);
+      const int h = w.head * p.group + (r - q_in_tile * p.group);
+      const bool row_ok = r < tile_rows && tok < p.batch.S;
+      const bool whole = w.n == w.span.n;
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      const size_t part = (static_cast<size_t>(2u * blockIdx.x) + (w.k0 == 0 ? 1u : 0u)) * tile_rows + r;
+#pragma unroll 1
+      for (int c = 2 * t; c < 2 * t + 2; ++c) {
+        uint32_t o0[32], o1[32];
+        tmem_ld_32x32(tmem + lane_addr + 128u + c * 32u, o0);
+        tmem_ld_32x32(tmem + lane_addr + 384u + c * 32u, o1);
+        tmem_wait_ld();
+        float o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          o[i] = (use0 ? a0 * __uint_as_float(o0[i]) : 0.f) + (use1 ? a1 * __uint_as_float(o1[i]) : 0.f);
+        if (!row_ok) continue;
+        if (whole) {
+          __nv_bfloat16* dst =
+              p.o + ((static_cast<size_t>(b) * p.batch.S + tok) * p.Hq + h) * KV_D + c * 32;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 v;
+            __nv_bfloat162* hh = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) hh[k] = __floats2bfloat162_rn(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+            *reinterpret_cast<uint4*>(dst + i) = v;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) kt_store8(p.part_o + part * KV_D + c * 32 + i, o + i);
+        }
+      }
+      if (t == 0 && row_ok) {
+        if (!whole)
+          p.part_ml[part] = make_float2(m, lsum);
+        else
+          p.lse[(static_cast<size_t>(b) * p.Hq + h) * p.batch.S + tok] =
+              lsum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(lsum);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.seg_done);
+      g0 += w.n;
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*reinterpret_cast<volatile int*>(&ctl.abort_flag) != 0) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Rows of items that were cut, in the order of the keys.  A warp takes a row.
+__global__ void __launch_bounds__(KT_MERGE_THREADS) kv_tiles_merge_kernel(const __grid_constant__ KvTilesParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const long long row = (blockIdx.x * static_cast<long long>(KT_MERGE_THREADS) + threadIdx.x) >> 5;
+  const int S = p.batch.S;
+  if (row >= static_cast<long long>(p.batch.B) * S * p.Hq) return;
+  const long long bs = row / p.Hq;
+  const int h = static_cast<int>(row - bs * p.Hq);
+  const int b = static_cast<int>(bs / S), tok = static_cast<int>(bs - static_cast<long long>(b) * S);
+  const int head = h / p.group, qt = tok / p.qrows, entry = b * p.nqt + qt;
+  const int r = (tok - qt * p.qrows) * p.group + (h - head * p.group), tile_rows = p.qrows * p.group;
+  const uint32_t base = p.plan[entry], per = p.plan[p.batch.B * p.nqt + 1];
+  const uint32_t n = (p.plan[entry + 1] - base) / static_cast<uint32_t>(p.cache.hkv);
+  const uint32_t start = base + static_cast<uint32_t>(head) * n;
+  const uint32_t cta0 = start / per, cta1 = (start + n - 1) / per;
+  if (cta0 == cta1) return;                                        // the row is final
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+  for (uint32_t i0 = cta0; i0 <= cta1; i0 += 8) {
+    float4 v[8];
+    float2 x[8];
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) {
+      x[u] = make_float2(-INFINITY, 0.f);
+      const uint32_t i = i0 + u;
+      if (i <= cta1) {
+        const long long at = static_cast<long long>(2u * i + (i * per <= start ? 1u : 0u)) * tile_rows + r;
+        x[u] = p.part_ml[at];
+        v[u] = reinterpret_cast<const float4*>(p.part_o + at * KV_D)[lane];
+      }
+    }
+    float m_new = m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m_new = fmaxf(m_new, x[u].x);
+    const float keep = m == -INFINITY ? 0.f : cp_ex2(m - m_new);
+    m = m_new;
+    l *= keep;
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (x[u].y == 0.f) continue;            // no visible key in the part
+      const float f = cp_ex2(x[u].x - m);
+      l += f * x[u].y;
+      acc.x += f * v[u].x, acc.y += f * v[u].y, acc.z += f * v[u].z, acc.w += f * v[u].w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const __nv_bfloat162 o2[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
+                                __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+  *reinterpret_cast<uint2*>(p.o + row * KV_D + 4 * lane) = *reinterpret_cast<const uint2*>(o2);
+  if (lane == 0)
+    p.lse[(static_cast<long long>(b) * p.Hq + h) * S + tok] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+}
+
+static int kt_sms() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
+    return 148;
+  return n;
+}
+
+struct KtLaunch {
+  int qrows, nqt, grid;
+  long long bytes, o_at, ml_at;
+};
+static bool kt_shape(KtLaunch* s, int B, int S, int Hq, int Hkv, long long max_len) {
+  const int group = Hq / Hkv;
+  if (group > CP_BM) return false;
+  s->qrows = CP_BM / group < S ? CP_BM / group : S;
+  s->nqt = (S + s->qrows - 1) / s->qrows;
+  const long long entries = static_cast<long long>(B) * s->nqt;
+  const long long blocks = entries * Hkv * ((max_len + KT_BN - 1) / KT_BN + 1);
+  if (entries > KT_MAX_ENTRIES || blocks > 0x3fffffffll || static_cast<long long>(B) * S * Hq > 0x3fffffffll) return false;
+  const long long want = (blocks + KT_MIN_BLOCKS - 1) / KT_MIN_BLOCKS;
+  const int sms = kt_sms();
+  s->grid = static_cast<int>(want < sms ? want : sms);
+  const long long rows = 2ll * s->grid * s->qrows * group;
+  s->o_at = ((entries + 2) * 4 + 127) / 128 * 128;
+  s->ml_at = s->o_at + rows * KV_D * 4;
+  s->bytes = s->ml_at + rows * 8;
+  return true;
+}
+
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" {
+
+// Bytes of workspace for cb_kv_tiles, or -1: not a call for it.
+long long cb_kv_tiles_bytes(int B, int S, int Hq, int Hkv, int max_len) {
+  KtLaunch s;
+  if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || max_len < 1 || !kt_shape(&s, B, S, Hq, Hkv, max_len)) {
+    set_last_error("key/value attention: bad shape, or more than 128 heads to a group or 96 query tiles");
+    return -1;
+  }
+  return s.bytes;
+}
+
+// Arguments as cb_kv_attend.
+int cb_kv_tiles(void* data, void* exps, int num_pages, int hkv, int page, const void* q, long long q_sb, long long q_ss,
+                long long q_sh, void* o, void* lse, const void* pages, int cols, const void* start, const void* count,
+                int B, int S, int Hq, int window, int sinks, int max_len, float scale, void* workspace,
+                long long workspace_bytes, void* status, void* stream) {
+  int lg = 0;
+  while ((1 << lg) < page) ++lg;
+  if (num_pages < 1 || page < 16 || page > 128 || (1 << lg) != page || cols < 1 || window < 0 || sinks < 0) {
+    set_last_error("key/value attention: bad cache, window or sinks");
+    return -1;
+  }
+  const long long need = cb_kv_tiles_bytes(B, S, Hq, hkv, max_len);
+  if (need < 0) return -1;
+  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31u) != 0) {
+    set_last_error("key/value attention: workspace missing, misaligned or too small");
+    return -1;
+  }
+  KtLaunch s;
+  kt_shape(&s, B, S, Hq, hkv, max_len);
+  KvTilesParams p;
+  p.cache = {static_cast<uint8_t*>(data), static_cast<int8_t*>(exps), num_pages, hkv, lg};
+  p.batch = {static_cast<const int*>(pages), static_cast<const int*>(start), static_cast<const int*>(count), B, S, cols};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sb = q_sb, p.q_ss = q_ss, p.q_sh = q_sh;
+  p.o = static_cast<__nv_bfloat16*>(o);
+  p.lse = static_cast<float*>(lse);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.plan = reinterpret_cast<uint32_t*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + s.o_at);
+  p.part_ml = reinterpret_cast<float2*>(ws + s.ml_at);
+  p.Hq = Hq;
+  p.group = Hq / hkv;
+  p.qrows = s.qrows;
+  p.nqt = s.nqt;
+  p.window = window;
+  p.sinks = window > 0 ? sinks : 0;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = static_cast<uint32_t*>(status);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  static std::atomic<uint64_t> smem_done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv_tiles_kernel), KT_SMEM, smem_done);
+  if (e == cudaSuccess)
+    e = launch_pdl(kv_tiles_kernel, dim3(static_cast<unsigned>(s.grid)), dim3(KT_THREADS), KT_SMEM, st, p);
+  if (e == cudaSuccess) {
+    const long long rows = static_cast<long long>(B) * S * Hq;
+    const int per = KT_MERGE_THREADS / 32;
+    e = launch_pdl(kv_tiles_merge_kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(KT_MERGE_THREADS), 0,
+                   st, p);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();   // reported here, not by the next call
+    set_last_error(std::string("key/value attention launch: ") + cudaGetErrorString(e));
+    return -1;
+  }
+  return 0;
+}
+
+}  // extern "C"

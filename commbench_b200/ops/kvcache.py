@@ -29,6 +29,7 @@ from ..utils.tracing import traced
 
 HEAD_DIM = 128
 _L9 = C.c_longlong * 9
+_FORMS = ("decode", "prefill", "tiles")
 
 
 def _tileable(q):
@@ -162,8 +163,9 @@ class KVCache8:
         cut of the work go by it, and later tokens are not seen.  A page id out of range leaves a status word, is
         not read, and makes the rows that should see it meaningless.
 
-        ``impl``: "decode" (few query rows, bound by the cache's bytes) or "prefill" (tcgen05 tiles over an expanded
-        copy); by default a model of both decides."""
+        ``impl``: "decode" (few query rows, bound by the cache's bytes), "tiles" (more of them: tcgen05 tiles,
+        expanded on their way) or "prefill" (many: tcgen05 tiles over an expanded copy); by default a model of the
+        three decides."""
         if stream is None and impl is None and isinstance(q, torch.Tensor) and q.dim() == 4 and pages.dim() == 2:
             room = pages.shape[1] * self.page
             r = N.fast().kv_attend(self.data, self.exps, self.num_pages, self.kv_heads, self.page, q, pages, start,
@@ -175,7 +177,7 @@ class KVCache8:
         B, S, Hq, _ = q.shape
         if Hq % self.kv_heads:
             raise CommError("query heads must be a multiple of the key/value heads")
-        if impl not in (None, "decode", "prefill"):
+        if impl is not None and impl not in _FORMS:
             raise CommError(f"unknown attention form {impl!r}")
         if window < 0 or sinks < 0:
             raise CommError("window and sinks must not be negative")
@@ -191,25 +193,26 @@ class KVCache8:
         max_len = room if max_len is None else max(1, min(int(max_len), room))
         sc = scale if scale is not None else 1.0 / math.sqrt(HEAD_DIM)
         lib = N.load()
-        long = bool(lib.cb_kv_attend_form(B, S, Hq, self.kv_heads, window, max_len)) if impl is None else \
-            impl == "prefill"
-        if long and not _tileable(q):
+        form = _FORMS.index(impl) if impl is not None else \
+            lib.cb_kv_attend_form(B, S, Hq, self.kv_heads, window, max_len)
+        size, run = ((lib.cb_kv_attend_bytes, lib.cb_kv_attend), (lib.cb_kv_prefill_bytes, lib.cb_kv_prefill),
+                     (lib.cb_kv_tiles_bytes, lib.cb_kv_tiles))[form]
+        if form == 1 and not _tileable(q):
             with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(q.device)):
                 q = q.contiguous()
         with torch.cuda.device(q.device):
-            n = (lib.cb_kv_prefill_bytes if long else lib.cb_kv_attend_bytes)(B, S, Hq, self.kv_heads, max_len)
+            n = size(B, S, Hq, self.kv_heads, max_len)
             if n < 0:
                 raise CommError(f"key/value attention failed: {N.last_error()}")
             ws = None
             if n > 0:
                 ws = q.new_empty((n,), dtype=torch.uint8) if stream is None else \
                     N.new_empty_on(stream, q, (n,), torch.uint8, handed_out=False)
-            strides = q.stride()[1:3] if long else q.stride()[:3]
-            rc = (lib.cb_kv_prefill if long else lib.cb_kv_attend)(
+            rc = run(
                 self.data.data_ptr(), self.exps.data_ptr(), self.num_pages, self.kv_heads, self.page, q.data_ptr(),
-                *strides, o.data_ptr(), lse.data_ptr(), pages.data_ptr(), pages.shape[1], start.data_ptr(),
-                count.data_ptr() if count is not None else 0, B, S, Hq, window, sinks, max_len, sc,
-                0 if ws is None else ws.data_ptr(), n, status_ptr, N.raw_stream(stream))
+                *q.stride()[1 if form == 1 else 0:3], o.data_ptr(), lse.data_ptr(), pages.data_ptr(),
+                pages.shape[1], start.data_ptr(), count.data_ptr() if count is not None else 0, B, S, Hq, window,
+                sinks, max_len, sc, 0 if ws is None else ws.data_ptr(), n, status_ptr, N.raw_stream(stream))
         if rc != 0:
             raise CommError(f"key/value attention failed: {N.last_error()}")
         return o, lse

@@ -213,6 +213,11 @@ def _check(o, lse, want):
     assert ((lse.double() - rl).abs()[~empty] <= 1e-4).all()
 
 
+def _tiles_take(B, S, group):
+    """The form of tiles takes at most 96 query tiles of 128 rows."""
+    return group <= 128 and B * -(-S // (128 // group)) <= 96
+
+
 def _case(lens, S, Hq, H, page, window=0, sinks=0, seed=20, max_len=None, count=None, scale=None, cache=None):
     """lens: tokens of each sequence with the new ones; the last S of them are queried."""
     B, T = len(lens), max(max(lens), 1)
@@ -222,7 +227,7 @@ def _case(lens, S, Hq, H, page, window=0, sinks=0, seed=20, max_len=None, count=
     cnt = count if count is not None else [S] * B
     start = [n - c for n, c in zip(lens, cnt)]
     want = _attend64(q, _quantised(k, page, lens), _quantised(v, page, lens), start, cnt, window, sinks, scale)
-    for impl in (None, "decode", "prefill"):
+    for impl in (None, "decode", "prefill") + (("tiles",) if _tiles_take(B, S, Hq // H) else ()):
         o, lse = cache.attend(q, pages, _ints(*start), count=None if count is None else _ints(*count), window=window,
                               sinks=sinks, max_len=max_len, scale=scale, impl=impl)
         _check(o, lse, want)
@@ -277,7 +282,7 @@ def test_attend_strides_and_scale(native_lib):
     q = big[:, :, 1:20:2, 4:].transpose(0, 0)[:, :, :8]
     q = q if q.data_ptr() % 8 == 0 else big[:, :, :8, :D]
     start = _ints(87, 87)
-    for impl in ("prefill", "decode"):
+    for impl in ("prefill", "tiles", "decode"):
         o, lse = cache.attend(q, pages, start, scale=0.03, impl=impl)
         o2, lse2 = cache.attend(q.contiguous(), pages, start, scale=0.03, impl=impl)
         assert torch.equal(o, o2) and torch.equal(lse, lse2)
@@ -346,7 +351,7 @@ def test_attend_repeats_its_bits_and_runs_on_another_stream(native_lib):
     cache, pages = _filled(k, v, 64, (1500, 700, 64), 71)
     q = torch.randn(3, 2, 8, D, device="cuda", generator=_gen(72)).bfloat16()
     start = _ints(1498, 698, 62)
-    for impl in ("decode", "prefill"):
+    for impl in ("decode", "prefill", "tiles"):
         o, lse = cache.attend(q, pages, start, impl=impl)
         s = torch.cuda.Stream()
         for i in range(4):
