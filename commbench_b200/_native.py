@@ -161,7 +161,7 @@ _FAST_ENTRIES = ("cb_gemm_bf16", "cb_gemm_fp8", "cb_gemm_fp8_blockscaled", "cb_g
                  "cb_quant_blockscaled", "cb_quant_blockscaled_pow2", "cb_attn_fwd4",
                  "cb_attn_split_bytes", "cb_attn_split", "cb_rms_norm", "cb_rms_norm_backward_floats",
                  "cb_rms_norm_backward", "cb_rope", "cb_kv_append", "cb_kv_read", "cb_kv_attend_bytes",
-                 "cb_kv_prefill_bytes", "cb_kv_attend_form", "cb_kv_attend", "cb_kv_prefill")
+                 "cb_kv_prefill_bytes", "cb_kv_tiles_bytes", "cb_kv_tiles", "cb_kv_attend_form", "cb_kv_attend", "cb_kv_prefill")
 
 
 class _NoFast:

@@ -770,6 +770,37 @@ static int ka_sms() {
   return n;
 }
 
+// Clusters of c CTAs that the current device runs at once, asked for once per device: a GPC's SMs are no multiple of 8,
+// so that clusters of 8 fill fewer SMs than there are.  16 of them took two turns (2 x 1 queries, 32 / 8 heads, over 4000 /
+// 16000 keys: 16.7 / 32.6 us; as 16 clusters of 4 11.3 / 22.4).
+template <class Cfg>
+static int ka_clusters(int c) {
+  static std::atomic<int> known[64][4];
+  const int at = c == 8 ? 3 : c == 4 ? 2 : c == 2 ? 1 : 0;
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148 / c;
+  if (dev < 64 && (n = known[dev][at].load(std::memory_order_relaxed)) > 0) return n;
+  auto kernel = kv_attend_kernel<Cfg, true>;
+  constexpr int kSmem = ka_smem_bytes<Cfg>();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(c));
+  cfg.blockDim = dim3(Cfg::kWarps * 32);
+  cfg.dynamicSmemBytes = kSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(c);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return 148 / c;
+  }
+  if (dev < 64) known[dev][at].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 struct KaLaunch {
   int tile_rows, row_tiles, grid, cluster;   // cluster 0: the flat list
   long long bytes, o_at, ml_at;
@@ -792,7 +823,8 @@ static bool ka_shape(KaLaunch* s, int B, int S, int Hq, int Hkv, long long max_l
   s->row_tiles = static_cast<int>(tiles);
   const int sms = ka_sms();
   int c = 1;
-  while (2 * c <= KA_MAX_CLUSTER && 2 * c * items <= sms && c * streams < per_item) c *= 2;
+  auto fit = [&](int n) { return rows <= 16 ? ka_clusters<KaCfg<1>>(n) : ka_clusters<KaCfg<2>>(n); };
+  while (2 * c <= KA_MAX_CLUSTER && 2 * c * items <= sms && items <= fit(2 * c) && c * streams < per_item) c *= 2;
   const float chain = static_cast<float>((per_item + c * streams - 1) / (c * streams));
   const float rounds = static_cast<float>(items * per_item) / static_cast<float>(sms * streams);
   s->cluster = 0;

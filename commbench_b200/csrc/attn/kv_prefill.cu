@@ -96,23 +96,38 @@ using namespace cb;
 
 extern "C" {
 
-// Which form takes a call: 1 this one, 0 cb_kv_attend, from a model of both in microseconds.
+// Which form takes a call: 0 cb_kv_attend (few rows), 1 this one (many), 2 cb_kv_tiles, from a model of the three in
+// microseconds, for calls in a graph.
 //   Few rows: a key of a head costs 37 ps of the whole chip with a tile of 16 rows and 73 with two (16 sequences of
 // 24000 keys, 64 / 8 heads: 129 us with one tile, 222 with two), however the rows are spread over sequences.
-//   Many: a key of a head is expanded in 150 ps, and a pair of 128-row tiles of one query head visits 128 keys in 1.3 us on one SM.
-// 4 x 16 queries over 6000 keys, 64 / 8 heads, take 196 us here (256 items, 16 of 256 rows each) and 74 there.
+//   Many: a key of a head is expanded in 150 ps, and a pair of 128-row tiles of one query head visits 128 keys in 1.3 us on
+// one SM; a call has 10 beside.
+//   Tiles: 128 keys of a head and tile of 128 rows take an SM 1.65 us, evenly cut, and a call 17 us.
+// Measured, few / tiles / many (sequences x queries, keys, heads): 1 x 64, 4160, 8 / 2: 18 / 22 / 64; 4 x 16, 6000, 64 / 8: 68 /
+// 40 / 196; 1 x 128, 4224, 32 / 8: 53 / 35 / 69; 1 x 256, 4352, 8 / 2: 30 / 28 / 68; 1 x 1000, 5096, 4 / 1: 62 / 34 / 78;
+// 2 x 256, 256, 32 / 8: 46 / 25 / 16; 1 x 1000, 7000, 32 / 8: 536 / 190 / 121; 16 x 4, 6000, 64 / 8: 72 / 85 / 700.
 int cb_kv_attend_form(int B, int S, int Hq, int Hkv, int window, int max_len) {
   if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || max_len < 1) return 0;
   const float group = static_cast<float>(Hq / Hkv), rows = static_cast<float>(S) * group;
   float keys = static_cast<float>(max_len);
   if (window > 0 && static_cast<float>(window) + S < keys) keys = static_cast<float>(window) + S;
   const float heads = static_cast<float>(B) * Hkv;
-  const float few = 14.f + heads * keys * (rows <= 16.f ? 37e-6f : 73e-6f * ceilf(rows / 32.f));
+  const float few = 8.f + heads * keys * (rows <= 16.f ? 37e-6f : 73e-6f * ceilf(rows / 32.f));
   const float waves = ceilf(ceilf(static_cast<float>(S) / (2 * CP_BM)) * B * Hq / 148.f);
   // a query in the middle of a chunk sees the chunk's first half
   const float seen = window > 0 ? keys : keys - 0.5f * S;
-  const float many = 14.f + heads * keys * 150e-6f + waves * 1.3f * seen / CP_BN;
-  return many < few ? 1 : 0;
+  const float many = 10.f + heads * keys * 150e-6f + waves * 1.3f * seen / CP_BN;
+  float best = few;
+  int form = 0;
+  if (many < best) best = many, form = 1;
+  if (rows > 32.f && group <= CP_BM) {
+    const float qrows = floorf(CP_BM / group), tiles = ceilf(static_cast<float>(S) / (qrows < S ? qrows : S));
+    const float of_tile = window > 0 ? static_cast<float>(window) + qrows < keys ? window + qrows : keys : seen;
+    const float blocks = heads * tiles * ceilf(of_tile / CP_BN + 0.5f);
+    const float cut = 17.f + 1.65f * ceilf(blocks / 148.f);
+    if (cut < best && tiles * B <= 96.f) form = 2;
+  }
+  return form;
 }
 
 // Bytes of workspace for cb_kv_prefill, or -1.

@@ -26,6 +26,7 @@ namespace cb {
 void set_last_error(const std::string& s);
 
 static constexpr int KT_THREADS = 512;    // producer, MMA and two idle warps; 4 that expand; 2 x 4 of softmax
+static constexpr int KT_EXPANDERS = 4;
 static constexpr int KT_BN = 128;         // keys of a block
 static constexpr int KT_RING = 2;         // raw blocks, and tiles of keys and of values
 static constexpr int KT_RAW = 2 * KT_BN * KV_D;
@@ -55,7 +56,8 @@ struct KtCtl {
   uint64_t sc_full[4];
   uint64_t s_full[2], p_first[2], p_rest[2], pv_done[2], seg_full, seg_done;
   float2 sc[4];                    // of a block: factor of the scores, exponent of the values
-  alignas(16) uint16_t exps[KT_RING][8];   // of a raw block's pages: key, value << 8
+  int4 blk[KT_RING];               // of a raw block: largest key and value exponent, whether all pages have it
+  uint16_t exps[KT_RING][8];       // of a raw block's pages: key, value << 8
   int8_t row_exp[2][CP_BM];        // rows were multiplied by 2^-e; of a segment and the next
   float2 ml[2][CP_BM];             // (max, sum) of the segment per stream and row
   uint32_t tmem_base;
@@ -121,8 +123,7 @@ struct KtWalk {
 };
 
 // 16 e4m3 numbers of a row, times a power of two, as fp16 into a swizzled tile: its row, its chunk of 16 columns.
-__device__ __forceinline__ void kt_expand(const uint8_t* raw, uint8_t* tile, int row, int chunk, __half2 f, bool scaled) {
-  const uint4 x = *reinterpret_cast<const uint4*>(raw + row * KV_D + ((chunk ^ (row & 7)) << 4));
+__device__ __forceinline__ void kt_expand(uint4 x, uint8_t* tile, int row, int chunk, __half2 f, bool scaled) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   uint32_t h[8];
 #pragma unroll
@@ -142,6 +143,34 @@ __device__ __forceinline__ void kt_expand(const uint8_t* raw, uint8_t* tile, int
   const int c0 = 2 * (chunk & 3);
   *reinterpret_cast<uint4*>(dst + ((c0 ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
   *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// A raw tile of 128 rows: a thread takes one chunk of 16 columns of every 16th row, so that eight lanes write eight
+// rows; four rows are read before the first is written.  e: the exponents of the block's pages (2^(e - top) is the
+// factor); a value 2^24 below is lost, rows past the end are anything finite.  Kept small: the roles share an
+// instruction cache, and with this unrolled for keys and values apart every warp of the CTA ran at half its pace (16 x 4
+// queries over 24000 keys, 64 / 8 heads, 366 us; 278 so).
+__device__ __forceinline__ void kt_expand_tile(const uint8_t* raw, uint8_t* tile, int tid, const uint16_t* exps, int shift,
+                                               int lg, int top, bool same) {
+  const int r = (tid & 7) + 8 * (tid >> 6), chunk = (tid >> 3) & 7;
+#pragma unroll 1
+  for (int i0 = 0; i0 < 8; i0 += 4) {
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = *reinterpret_cast<const uint4*>(raw + (r + 16 * (i0 + i)) * KV_D + ((chunk ^ (r & 7)) << 4));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = r + 16 * (i0 + i);
+      __half2 f = __half2();
+      if (!same) {
+        int e = static_cast<int8_t>(exps[row >> lg] >> shift) - top;
+        e = e > 0 ? 0 : e < -126 ? -126 : e;
+        f = __float2half2_rn(kv_pow2(e));
+      }
+      kt_expand(x[i], tile, row, chunk, f, !same);
+    }
+  }
 }
 
 __device__ __forceinline__ void kt_store8(float* dst, const float* v) {   // a whole sector
@@ -165,6 +194,93 @@ __device__ __forceinline__ void kt_probabilities(uint32_t (&s)[128], float scale
   }
 }
 
+// The role of warps 4 to 7: queries, keys and values to fp16 tiles.
+__device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, uint8_t* sQ, uint32_t per, uint32_t total) {
+  uint8_t* sK = sQ + CP_TILE;
+  uint8_t* sV = sK + KT_RING * CP_TILE;
+  uint8_t* sR = sV + KT_RING * CP_TILE;
+  const uint32_t lane = threadIdx.x & 31u;
+  const int tile_rows = p.qrows * p.group;
+  const int tid = static_cast<int>(threadIdx.x) - 128;
+  const int lg = p.cache.page_log2;
+  auto arrive = [&](uint64_t* bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  auto wait_all = [&](uint64_t* bar, uint32_t parity, uint32_t detail) -> bool {
+    return mbar_wait_warp(bar, parity, &ctl.abort_flag, p.status, detail);
+  };
+  KtWalk w;
+  bool ok = true;
+  uint32_t seg = 0, g = 0;
+  for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
+    if (seg > 0) ok = wait_all(&ctl.q_empty, (seg - 1) & 1u, 0xA36);
+    if (!ok) break;
+    // Queries: eight lanes take a row, brought to [1, 2) by a power of two so that fp16 holds it.
+    {
+      const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, chunk = tid & 7;
+#pragma unroll 1
+      for (int r0 = 0; r0 < CP_BM; r0 += 4 * KT_EXPANDERS) {
+        const int r = r0 + (tid >> 3);         // whole warps go on together: the shuffles below
+        const int in = r / p.group, tok = qt * p.qrows + in;
+        const bool there = r < tile_rows && tok < w.span.count;
+        const __nv_bfloat16* src = p.q + b * p.q_sb + tok * p.q_ss +
+                                   static_cast<long long>(w.head * p.group + r - in * p.group) * p.q_sh + 16 * chunk;
+        float x[16];
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint2 raw = there ? *reinterpret_cast<const uint2*>(src + 4 * i) : make_uint2(0u, 0u);
+          const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
+          const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+          x[4 * i] = f0.x, x[4 * i + 1] = f0.y, x[4 * i + 2] = f1.x, x[4 * i + 3] = f1.y;
+          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))));
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+        e = e < -60 ? -60 : e > 100 ? 100 : e;
+        const float down = kv_pow2(-e);
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const __half2 y = __floats2half2_rn(x[2 * i] * down, x[2 * i + 1] * down);
+          h[i] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        if (r >= CP_BM) continue;
+        uint8_t* dst = sQ + (chunk >> 2) * CP_SUB + r * 128;
+        const int c0 = 2 * (chunk & 3);
+        *reinterpret_cast<uint4*>(dst + ((c0 ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        if (chunk == 0) ctl.row_exp[seg & 1u][r] = static_cast<int8_t>(e);
+      }
+    }
+    fence_proxy_async_smem();
+    arrive(&ctl.q_full);
+    // A block's keys, then its values.  (Keys a block ahead hold the raw ring longer: 450 us instead of 278.)
+    for (int j = 0; ok && j < w.n; ++j, ++g) {
+      const uint32_t s = g % KT_RING, par = (g / KT_RING) & 1u;
+      ok = wait_all(&ctl.raw_full[s], par, 0xA37);
+      if (ok && g >= KT_RING) ok = wait_all(&ctl.k_empty[s], par ^ 1u, 0xA38);
+      if (!ok) break;
+      const int4 blk = ctl.blk[s];
+      if (tid == 0) ctl.sc[g & 3u] = make_float2(kv_pow2(blk.x), static_cast<float>(blk.y));
+      arrive(&ctl.sc_full[g & 3u]);
+#pragma unroll 1
+      for (int side = 0; ok && side < 2; ++side) {
+        if (side == 1 && g >= KT_RING) ok = wait_all(&ctl.v_empty[s], par ^ 1u, 0xA39);
+        if (!ok) break;
+        kt_expand_tile(sR + s * KT_RAW + side * (KT_BN * KV_D), (side ? sV : sK) + s * CP_TILE, tid, ctl.exps[s], 8 * side,
+                       lg, side ? blk.y : blk.x, (side ? blk.w : blk.z) != 0);
+        fence_proxy_async_smem();
+        arrive(side ? &ctl.v_full[s] : &ctl.k_full[s]);
+      }
+      if (!ok) break;
+      arrive(&ctl.raw_empty[s]);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_constant__ KvTilesParams p) {
   extern __shared__ __align__(1024) uint8_t kt_smem[];
   uint8_t* sQ = kt_smem;
@@ -184,15 +300,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
   if (threadIdx.x == 0) {
     for (int i = 0; i < KT_RING; ++i) {
       mbar_init(&ctl.raw_full[i], 1);
-      mbar_init(&ctl.raw_empty[i], 4);
-      mbar_init(&ctl.k_full[i], 4);
+      mbar_init(&ctl.raw_empty[i], KT_EXPANDERS);
+      mbar_init(&ctl.k_full[i], KT_EXPANDERS);
       mbar_init(&ctl.k_empty[i], 1);
-      mbar_init(&ctl.v_full[i], 4);
+      mbar_init(&ctl.v_full[i], KT_EXPANDERS);
       mbar_init(&ctl.v_empty[i], 1);
     }
-    mbar_init(&ctl.q_full, 4);
+    mbar_init(&ctl.q_full, KT_EXPANDERS);
     mbar_init(&ctl.q_empty, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&ctl.sc_full[i], 4);
+    for (int i = 0; i < 4; ++i) mbar_init(&ctl.sc_full[i], KT_EXPANDERS);
     mbar_init(&ctl.seg_full, 2 * active);
     mbar_init(&ctl.seg_done, 2 * active);
     for (int i = 0; i < 2; ++i) {
@@ -238,9 +354,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
   // stream t: S (fp32, 128 columns; the first 64 hold P as fp16 pairs after the softmax) at column 256 t, O at column
   // 256 t + 128.
 
-  // 128 x (64 + 80 + 184 + 184) registers = 65,536, what 512 threads x 128 were launched with.
+  // 128 x (72 + 72 + 184 + 184) registers = 65,536, what 512 threads x 128 were launched with.
   if (warp < 4) {
-    cp_reg_dec<64>();
+    cp_reg_dec<72>();
     if (warp == 0) {
       // ---------------------------------------------------------------- producer: raw blocks
       const int lg = p.cache.page_log2, pages = KT_BN >> lg;
@@ -273,7 +389,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
           if (g >= KT_RING)
             ok = mbar_wait_warp(&ctl.raw_empty[s], (g / KT_RING - 1) & 1u, &ctl.abort_flag, p.status, 0xA30);
           if (!ok) break;
+          const bool there = static_cast<int>(lane) < pages && w.key0(j) + (static_cast<int>(lane) << lg) < end;
+          const int ek = static_cast<int8_t>(ex), ev = static_cast<int8_t>(ex >> 8);
+          int top_k = __reduce_max_sync(0xffffffffu, there ? ek : KV_EXP_MIN);
+          int top_v = __reduce_max_sync(0xffffffffu, there ? ev : KV_EXP_MIN);
+          if (top_k == KV_EXP_MIN) top_k = 0;   // all zero
+          if (top_v == KV_EXP_MIN) top_v = 0;
+          const bool same_k = __all_sync(0xffffffffu, !there || ek == top_k);
+          const bool same_v = __all_sync(0xffffffffu, !there || ev == top_v);
           if (lane < 8) ctl.exps[s][lane] = static_cast<uint16_t>(ex);   // pages that are not there: 0
+          if (lane == 0) ctl.blk[s] = make_int4(top_k, top_v, same_k, same_v);
           __syncwarp();
           if (lane == 0) mbar_arrive_expect_tx(&ctl.raw_full[s], KT_RAW);
           __syncwarp();
@@ -360,121 +485,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
       }
     }
   } else if (warp < 8) {
-    cp_reg_dec<80>();
-    // ------------------------------------------------------------------- expansion
-    const int tid = static_cast<int>(threadIdx.x) - 128;
-    const int lg = p.cache.page_log2;
-    auto arrive = [&](uint64_t* bar) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
-    auto wait_all = [&](uint64_t* bar, uint32_t parity, uint32_t detail) -> bool {
-      return mbar_wait_warp(bar, parity, &ctl.abort_flag, p.status, detail);
-    };
-    KtWalk w;
-    bool ok = true;
-    uint32_t seg = 0, g = 0;
-    for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
-      if (seg > 0) ok = wait_all(&ctl.q_empty, (seg - 1) & 1u, 0xA36);
-      if (!ok) break;
-      // Queries: eight lanes take a row, brought to [1, 2) by a power of two so that fp16 holds it.
-      {
-        const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, chunk = tid & 7;
-#pragma unroll 1
-        for (int r = tid >> 3; r < CP_BM; r += 16) {
-          const int in = r / p.group, tok = qt * p.qrows + in;
-          const bool there = r < tile_rows && tok < w.span.count;
-          const __nv_bfloat16* src = p.q + b * p.q_sb + tok * p.q_ss +
-                                     static_cast<long long>(w.head * p.group + r - in * p.group) * p.q_sh + 16 * chunk;
-          float x[16];
-          float amax = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint2 raw = there ? *reinterpret_cast<const uint2*>(src + 4 * i) : make_uint2(0u, 0u);
-            const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-            const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-            x[4 * i] = f0.x, x[4 * i + 1] = f0.y, x[4 * i + 2] = f1.x, x[4 * i + 3] = f1.y;
-            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))));
-          }
-#pragma unroll
-          for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-          e = e < -60 ? -60 : e > 100 ? 100 : e;
-          const float down = kv_pow2(-e);
-          uint32_t h[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __half2 y = __floats2half2_rn(x[2 * i] * down, x[2 * i + 1] * down);
-            h[i] = *reinterpret_cast<const uint32_t*>(&y);
-          }
-          uint8_t* dst = sQ + (chunk >> 2) * CP_SUB + r * 128;
-          const int c0 = 2 * (chunk & 3);
-          *reinterpret_cast<uint4*>(dst + ((c0 ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-          if (chunk == 0) ctl.row_exp[seg & 1u][r] = static_cast<int8_t>(e);
-        }
-      }
-      fence_proxy_async_smem();
-      arrive(&ctl.q_full);
-      // A thread: rows (tid & 7) + 8 (tid >> 6) + 16 i, one chunk of 16 columns; eight lanes write eight rows.
-      const int row0 = (tid & 7) + 8 * (tid >> 6), chunk = (tid >> 3) & 7;
-      for (int j = 0; ok && j < w.n; ++j, ++g) {
-        const uint32_t s = g % KT_RING, par = (g / KT_RING) & 1u;
-        ok = wait_all(&ctl.raw_full[s], par, 0xA37);
-        if (ok && g >= KT_RING) ok = wait_all(&ctl.k_empty[s], par ^ 1u, 0xA38);
-        if (!ok) break;
-        const uint4 e4 = *reinterpret_cast<const uint4*>(ctl.exps[s]);
-        const uint32_t ew[4] = {e4.x, e4.y, e4.z, e4.w};
-        int ek[8], ev[8], top_k = KV_EXP_MIN, top_v = KV_EXP_MIN;
-        const int pages = KT_BN >> lg;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t x = ew[i >> 1] >> (16 * (i & 1));
-          ek[i] = static_cast<int8_t>(x);
-          ev[i] = static_cast<int8_t>(x >> 8);
-          // only pages with keys that exist
-          if (i < pages && w.key0(j) + (i << lg) < w.span.start + w.span.count) {
-            top_k = max(top_k, ek[i]);
-            top_v = max(top_v, ev[i]);
-          }
-        }
-        if (top_k == KV_EXP_MIN) top_k = 0;   // all zero
-        if (top_v == KV_EXP_MIN) top_v = 0;
-        if (tid == 0) ctl.sc[g & 3u] = make_float2(kv_pow2(top_k), static_cast<float>(top_v));
-        arrive(&ctl.sc_full[g & 3u]);
-        bool same_k = true, same_v = true;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          same_k = same_k && (i >= pages || ek[i] == top_k);
-          same_v = same_v && (i >= pages || ev[i] == top_v);
-        }
-        // 2^(e - top) of the 16 keys of step i; what is 2^24 below is lost, what lies past the end is anything finite
-        auto factor = [&](const int(&e)[8], int top, int i) {
-          int x = 0;
-          const int page = (16 * i) >> lg;
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k == page) x = e[k] - top;
-          x = x > 0 ? 0 : x < -126 ? -126 : x;
-          return __float2half2_rn(kv_pow2(x));
-        };
-        const uint8_t* raw = sR + s * KT_RAW;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          kt_expand(raw, sK + s * CP_TILE, row0 + 16 * i, chunk, same_k ? __half2() : factor(ek, top_k, i), !same_k);
-        fence_proxy_async_smem();
-        arrive(&ctl.k_full[s]);
-        if (g >= KT_RING) ok = wait_all(&ctl.v_empty[s], par ^ 1u, 0xA39);
-        if (!ok) break;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          kt_expand(raw + KT_BN * KV_D, sV + s * CP_TILE, row0 + 16 * i, chunk, same_v ? __half2() : factor(ev, top_v, i),
-                    !same_v);
-        fence_proxy_async_smem();
-        arrive(&ctl.v_full[s]);
-        arrive(&ctl.raw_empty[s]);
-      }
-    }
+    cp_reg_dec<72>();
+    kt_expander(p, ctl, sQ, per, total);
   } else {
     cp_reg_inc<184>();
     // ----------------------------------------------------------------- softmax

@@ -62,9 +62,9 @@ NormBwdFn g_norm_bwd;
 RopeFn g_rope;
 KvAppendFn g_kv_append;
 KvReadFn g_kv_read;
-KvBytesFn g_kv_attend_bytes, g_kv_prefill_bytes;
+KvBytesFn g_kv_attend_bytes, g_kv_prefill_bytes, g_kv_tiles_bytes;
 KvFormFn g_kv_form;
-KvAttendFn g_kv_attend;
+KvAttendFn g_kv_attend, g_kv_tiles;
 KvPrefillFn g_kv_prefill;
 GemmFn g_gemm_bf16, g_gemm_fp8;
 ScaledGemmFn g_gemm_bs;
@@ -610,7 +610,8 @@ PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (q == nullptr || pages == nullptr || pages->size(0) != q->size(0) || q->size(2) % c.hkv != 0) Py_RETURN_NONE;
   const int64_t B = q->size(0), S = q->size(1), Hq = q->size(2);
   if (!vector_of(v[7], B, false, &start) || !vector_of(v[8], B, true, &count)) Py_RETURN_NONE;
-  const bool tall = g_kv_form(static_cast<int>(B), static_cast<int>(S), static_cast<int>(Hq), c.hkv, window, max_len) != 0;
+  const int form = g_kv_form(static_cast<int>(B), static_cast<int>(S), static_cast<int>(Hq), c.hkv, window, max_len);
+  const bool tall = form == 1;
   if (tall && ((reinterpret_cast<uintptr_t>(q->const_data_ptr()) & 15u) != 0 || q->stride(1) % 8 != 0 ||
                q->stride(2) % 8 != 0 || q->stride(1) <= 0 || q->stride(2) <= 0 ||
                (B > 1 && q->stride(0) != S * q->stride(1))))
@@ -621,7 +622,8 @@ PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
   int rc = -1;
   {
     NoGil g;
-    const long long bytes = (tall ? g_kv_prefill_bytes : g_kv_attend_bytes)(b, s, hq, c.hkv, max_len);
+    const long long bytes =
+        (tall ? g_kv_prefill_bytes : form == 2 ? g_kv_tiles_bytes : g_kv_attend_bytes)(b, s, hq, c.hkv, max_len);
     if (bytes >= 0) {
       o = empty(*q, q->sizes(), at::kBFloat16);
       lse = empty(*q, {B, Hq, S}, at::kFloat);
@@ -634,7 +636,7 @@ PyObject* fast_kv_attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
                           lse.mutable_data_ptr(), pages->const_data_ptr(), cols, start, count, b, s, hq, window, sinks,
                           max_len, scale, work, bytes, status, current_stream());
       else
-        rc = g_kv_attend(c.data->mutable_data_ptr(), c.exps->mutable_data_ptr(), c.num_pages, c.hkv, c.page,
+        rc = (form == 2 ? g_kv_tiles : g_kv_attend)(c.data->mutable_data_ptr(), c.exps->mutable_data_ptr(), c.num_pages, c.hkv, c.page,
                          q->const_data_ptr(), q->stride(0), q->stride(1), q->stride(2), o.mutable_data_ptr(),
                          lse.mutable_data_ptr(), pages->const_data_ptr(), cols, start, count, b, s, hq, window, sinks,
                          max_len, scale, work, bytes, status, current_stream());
@@ -668,11 +670,13 @@ PyObject* fast_bind(PyObject*, PyObject* d) {
   g_kv_attend_bytes = reinterpret_cast<KvBytesFn>(get("cb_kv_attend_bytes"));
   g_kv_prefill_bytes = reinterpret_cast<KvBytesFn>(get("cb_kv_prefill_bytes"));
   g_kv_form = reinterpret_cast<KvFormFn>(get("cb_kv_attend_form"));
+  g_kv_tiles_bytes = reinterpret_cast<KvBytesFn>(get("cb_kv_tiles_bytes"));
+  g_kv_tiles = reinterpret_cast<KvAttendFn>(get("cb_kv_tiles"));
   g_kv_attend = reinterpret_cast<KvAttendFn>(get("cb_kv_attend"));
   g_kv_prefill = reinterpret_cast<KvPrefillFn>(get("cb_kv_prefill"));
   if (PyErr_Occurred()) return nullptr;
   if (!g_norm || !g_norm_bwd_floats || !g_norm_bwd || !g_rope || !g_kv_append || !g_kv_read || !g_kv_attend_bytes ||
-      !g_kv_prefill_bytes || !g_kv_form || !g_kv_attend || !g_kv_prefill || !g_gemm_bf16 || !g_gemm_fp8 || !g_gemm_bs || !g_gemm_mx || !g_quant || !g_quant_pow2 || !g_attn ||
+      !g_kv_prefill_bytes || !g_kv_form || !g_kv_tiles_bytes || !g_kv_tiles || !g_kv_attend || !g_kv_prefill || !g_gemm_bf16 || !g_gemm_fp8 || !g_gemm_bs || !g_gemm_mx || !g_quant || !g_quant_pow2 || !g_attn ||
       !g_split_bytes || !g_split) {
     PyErr_SetString(PyExc_RuntimeError, "fast_ops.bind: an entry point is missing");
     return nullptr;
