@@ -79,7 +79,8 @@ __device__ __forceinline__ void store_quantised(const NormParams& p, long long r
   for (int i = 0; i < VPT; ++i) {
     float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) amax = fmaxf(amax, fabsf(y[i][j]));
+    for (int j = 0; j < V; j += 2)
+      asm("max.f32 %0, %1, %2, %3;" : "=f"(amax) : "f"(amax), "f"(fabsf(y[i][j])), "f"(fabsf(y[i][j + 1])));
 #pragma unroll
     for (int o = 64 / V; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if constexpr (kMode == NORM_POW2) {
@@ -119,11 +120,11 @@ __device__ __forceinline__ void store_quantised(const NormParams& p, long long r
     uint32_t q[V / 4];
 #pragma unroll
     for (int j = 0; j < V; j += 4) {
-      const float f = inv[i];
-      const uint32_t lo =
-          __nv_cvt_float2_to_fp8x2(make_float2(y[i][j] * f, y[i][j + 1] * f), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi =
-          __nv_cvt_float2_to_fp8x2(make_float2(y[i][j + 2] * f, y[i][j + 3] * f), __NV_SATFINITE, __NV_E4M3);
+      const uint64_t f2 = f2_pack(inv[i], inv[i]);
+      const float2 a = f2_parts(f2_mul(f2_pack(y[i][j], y[i][j + 1]), f2));
+      const float2 b = f2_parts(f2_mul(f2_pack(y[i][j + 2], y[i][j + 3]), f2));
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
       q[j / 4] = lo | (hi << 16);
     }
     uint8_t* dst = static_cast<uint8_t*>(p.y) + row * p.D + col;
@@ -132,6 +133,15 @@ __device__ __forceinline__ void store_quantised(const NormParams& p, long long r
     else
       *reinterpret_cast<uint32_t*>(dst) = q[0];
   }
+}
+
+// What the rounding of r = 1 / sqrt(m) left off, by a Newton step: r (1 - m r^2) / 2; 0 where that says nothing.
+// The 8-bit form adds h times it to h r, because a y beside the middle of two e4m3 numbers falls to the wrong one if it
+// is off in its last bit, and an error of r is off for a whole row.
+__device__ __forceinline__ float rstd_rest(float m, float r) {
+  const float mr = m * r;
+  const float e = fmaf(-mr, r, 1.f) - fmaf(m, r, -mr) * r;
+  return fabsf(e) < 1e-3f ? 0.5f * r * e : 0.f;
 }
 
 // VPT vectors of V columns per thread, `threads` threads a row (32 or the CTA).
@@ -180,7 +190,8 @@ __global__ void __launch_bounds__(VPT == 4 || VPT == 8 ? 512 : 1024) rms_norm_ke
 #pragma unroll
     for (int j = 0; j < V; ++j) ss += h[i][j] * h[i][j];
   ss = row_sum<kWarpRow>(ss, sh, 0);
-  const float rstd = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
+  const float mean = ss / static_cast<float>(p.D) + p.eps;
+  const float rstd = 1.f / sqrtf(mean), rest = kMode == NORM_PLAIN ? 0.f : rstd_rest(mean, rstd);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int col = (i * threads + t) * V;
@@ -189,7 +200,10 @@ __global__ void __launch_bounds__(VPT == 4 || VPT == 8 ? 512 : 1024) rms_norm_ke
     if (active) {
       load_weight<T, V>(p.w, p.w_f32, col, w);
 #pragma unroll
-      for (int j = 0; j < V; ++j) h[i][j] = h[i][j] * rstd * w[j];
+      for (int j = 0; j < V; ++j) {
+        const float n = kMode == NORM_PLAIN ? h[i][j] * rstd : fmaf(h[i][j], rstd, h[i][j] * rest);
+        h[i][j] = n * w[j];
+      }
     }
     if (kMode == NORM_PLAIN && active) store_vec<T, V>(static_cast<T*>(p.y) + row * p.D + col, h[i]);
   }
@@ -286,8 +300,9 @@ __global__ void __launch_bounds__(512, 2)
       const long long next = row + static_cast<long long>(ring.slots) * gridDim.x;
       if (next < p.rows) issue(next, slot);
     }
-    const float rstd = 1.f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
-    const uint64_t r2 = f2_pack(rstd, rstd);
+    const float mean = ss / static_cast<float>(p.D) + p.eps;
+    const float rstd = 1.f / sqrtf(mean), rest = kMode == NORM_PLAIN ? 0.f : rstd_rest(mean, rstd);
+    const uint64_t r2 = f2_pack(rstd, rstd), rest2 = f2_pack(rest, rest);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int col = (i * threads + t) * V;
@@ -295,7 +310,9 @@ __global__ void __launch_bounds__(512, 2)
       if (active && two) store_vec<T, V>(static_cast<T*>(p.h) + row * p.D + col, h[i]);
 #pragma unroll
       for (int j = 0; j < V; j += 2) {
-        const float2 f = f2_parts(f2_mul(f2_mul(f2_pack(h[i][j], h[i][j + 1]), r2), f2_pack(w[i][j], w[i][j + 1])));
+        const uint64_t h2 = f2_pack(h[i][j], h[i][j + 1]);
+        const uint64_t n2 = kMode == NORM_PLAIN ? f2_mul(h2, r2) : f2_fma(h2, r2, f2_mul(h2, rest2));
+        const float2 f = f2_parts(f2_mul(n2, f2_pack(w[i][j], w[i][j + 1])));
         h[i][j] = f.x;
         h[i][j + 1] = f.y;
       }
