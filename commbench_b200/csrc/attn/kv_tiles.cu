@@ -5,14 +5,25 @@
 // bytes have arrived, and too few query tiles to pay for an expanded copy of the keys and to fill the chip with them.
 // Here the products are tcgen05's and the expansion happens on the way to them:
 //   * the rows of a 128-row tile are (query token, head of the group) couples of one key/value head;
-//   * bulk copies bring 128 keys and values, 32 KB, as they lie in their pages into a ring of two; four warps expand
-//     them to fp16, exactly, into the swizzled tiles that the tensor cores read (a copy through memory would cost 5
-//     bytes an element instead of 1).  The scales of a block's pages are brought to the largest of them, so that one
-//     factor for the scores and one exponent for the probabilities serve the whole block; a value 2^24 below the
-//     largest of its block is lost;
+//   * bulk copies bring 128 keys and values, 32 KB, as they lie in their pages into a ring of three;
+//   * the tensor cores read the keys from there: a page is laid out as an operand tile of 8-bit numbers is.  The queries
+//     become the sum of two e4m3 numbers each, which holds all of bf16's 8 bits (of a number 2^10 below the largest of
+//     its row 2^-18 of that one), and are multiplied by the keys in two rounds into the same scores;
+//   * four warps expand the values to fp16, exactly, into the swizzled tile of the second product (probabilities in
+//     two e4m3 numbers would reach down to 2^-17 only).  The scales of a block's values are brought to the largest of
+//     them, so that one exponent of the probabilities serves the whole block; a value 2^24 below the largest of its
+//     block is lost.  Where the pages of a block have other scales of the keys, the scores of each are multiplied;
+//   * up to 32 or 64 rows stand four times or twice in the tile, so that all softmax warps have a share of the keys;
 //   * two softmax streams take alternate blocks, each with its scores, probabilities (fp16) and results in tensor
 //     memory, as in fa_split.cu, and the flat list of (sequence, query tile, head, block) is cut evenly over the
 //     CTAs as there - by the lengths that the device holds.
+//
+// Measured, 64 / 8 heads, pages of 64: 16 sequences x 4 queries (32 rows) over 6000 / 24000 keys 60 / 194 us (the form of
+// few rows 72 / 223, 196 and 786 MB of cache), 16 x 8 over 6000 70 (134), 4 x 16 over 6000 37 (68).  A block of 128 keys
+// takes an SM 1.1 us, 1.3 with more than 64 rows: two products of 128 x 128 x 128, 0.54 us of the tensor cores, whose
+// operands and tiles move 176 KB through shared memory (0.72 us at 128 bytes a cycle), and the one warp that issues them
+// waits for nothing but its own barriers any more.  With keys expanded as well and one copy of a row it were
+// 1.65 us.
 // Every mbarrier wait is bounded (see mbarrier.cuh).
 #include <math.h>
 
@@ -28,10 +39,15 @@ void set_last_error(const std::string& s);
 static constexpr int KT_THREADS = 512;    // producer, MMA and two idle warps; 4 that expand; 2 x 4 of softmax
 static constexpr int KT_EXPANDERS = 4;
 static constexpr int KT_BN = 128;         // keys of a block
-static constexpr int KT_RING = 2;         // raw blocks, and tiles of keys and of values
+static constexpr int KT_RAWS = 3;         // raw blocks
+static constexpr int KT_VALS = 2;         // tiles of values
+static constexpr int KT_SCALES = 8;       // blocks whose scales are kept: see the producer
 static constexpr int KT_RAW = 2 * KT_BN * KV_D;
-static constexpr int KT_TILES = CP_TILE + KT_RING * (2 * CP_TILE + KT_RAW);
-static constexpr int KT_MAX_ENTRIES = 96;
+static constexpr int KT_Q8 = CP_BM * KV_D;    // one of the two terms of the queries
+static constexpr int KT_TILES = 2 * KT_Q8 + KT_VALS * CP_TILE + KT_RAWS * KT_RAW;
+static constexpr int KT_PIECE = 16;       // columns of a result that the copies of a row add up at a time
+static constexpr int KT_STAGE = 2 * 2 * CP_BM * KT_PIECE * 4;   // two of each stream
+static constexpr int KT_MAX_ENTRIES = 128;
 static constexpr int KT_MIN_BLOCKS = 2;   // of a CTA
 static constexpr int KT_MERGE_THREADS = 128;
 
@@ -51,21 +67,25 @@ struct KvTilesParams {
 };
 
 struct KtCtl {
-  uint64_t raw_full[KT_RING], raw_empty[KT_RING], q_full, q_empty;
-  uint64_t k_full[KT_RING], k_empty[KT_RING], v_full[KT_RING], v_empty[KT_RING];
-  uint64_t sc_full[4];
-  uint64_t s_full[2], p_first[2], p_rest[2], pv_done[2], seg_full, seg_done;
-  float2 sc[4];                    // of a block: factor of the scores, exponent of the values
-  int4 blk[KT_RING];               // of a raw block: largest key and value exponent, whether all pages have it
-  uint16_t exps[KT_RING][8];       // of a raw block's pages: key, value << 8
+  uint64_t raw_full[KT_RAWS], raw_empty[KT_RAWS], q_full, q_empty, v_full[KT_VALS], v_empty[KT_VALS];
+  uint64_t sc_full[KT_SCALES];
+  uint64_t s_full[2], p_first[2], p_rest[2], pv_done[2], seg_full, seg_done, piece_full[2];
+  // Of a block: the largest key and value exponent, whether all pages have it; its pages' exponents, key, value << 8.
+  int4 blk[KT_SCALES];
+  uint16_t exps[KT_SCALES][8];
   int8_t row_exp[2][CP_BM];        // rows were multiplied by 2^-e; of a segment and the next
   float2 ml[2][CP_BM];             // (max, sum) of the segment per stream and row
   uint32_t tmem_base;
   int abort_flag;
-  uint32_t base[KT_MAX_ENTRIES + 1];
+  uint32_t total, per;             // blocks in all, of a CTA
+  uint32_t base;                   // blocks before the entry that this CTA begins in
+  int entry;
 };
-static constexpr int KT_SMEM = KT_TILES + static_cast<int>(sizeof(KtCtl));
-static_assert(KT_SMEM <= 232448, "over the 227 KB shared-memory limit");
+// Copies of each row in the tile: see kv_tiles_kernel.
+static constexpr int kt_smem(int copies) {
+  return KT_TILES + (copies > 1 ? KT_STAGE : 0) + static_cast<int>(sizeof(KtCtl));
+}
+static_assert(kt_smem(4) <= 232448, "over the 227 KB shared-memory limit");
 
 // The blocks that the queries of a (sequence, query tile) see: the first `sink`, then `first` and on; n in all.
 struct KtSpan {
@@ -94,27 +114,34 @@ struct KtWalk {
   KtSpan span;
   uint32_t pos, end;
   int entry, head, k0, n;   // blocks k0 .. k0 + n - 1 of the item
-  __device__ __forceinline__ bool locate(const KvTilesParams& p, const KtCtl& ctl) {
+  uint32_t base;            // blocks before the entry
+  __device__ __forceinline__ bool locate(const KvTilesParams& p) {
     if (pos >= end) return false;
-    while (pos >= ctl.base[entry + 1]) ++entry;
-    span = kt_span(p, entry);
-    const uint32_t in = pos - ctl.base[entry];
+    for (;; ++entry) {
+      if (entry >= p.batch.B * p.nqt) return false;   // not with lengths that stay as they are
+      span = kt_span(p, entry);
+      const uint32_t of_entry = static_cast<uint32_t>(span.n) * p.cache.hkv;
+      if (pos - base < of_entry) break;
+      base += of_entry;
+    }
+    const uint32_t in = pos - base;
     head = static_cast<int>(in / span.n);
     k0 = static_cast<int>(in) - head * span.n;
     n = span.n - k0;
     if (static_cast<uint32_t>(n) > end - pos) n = static_cast<int>(end - pos);
     return true;
   }
-  __device__ __forceinline__ bool start(const KvTilesParams& p, const KtCtl& ctl, uint32_t per, uint32_t total) {
-    const unsigned long long e = static_cast<unsigned long long>(blockIdx.x + 1) * per;
-    pos = blockIdx.x * per;
-    end = e < total ? static_cast<uint32_t>(e) : total;
-    entry = 0;
-    return locate(p, ctl);
+  __device__ __forceinline__ bool start(const KvTilesParams& p, const KtCtl& ctl) {
+    const unsigned long long e = static_cast<unsigned long long>(blockIdx.x + 1) * ctl.per;
+    pos = blockIdx.x * ctl.per;
+    end = e < ctl.total ? static_cast<uint32_t>(e) : ctl.total;
+    entry = ctl.entry;
+    base = ctl.base;
+    return locate(p);
   }
-  __device__ __forceinline__ bool next(const KvTilesParams& p, const KtCtl& ctl) {
+  __device__ __forceinline__ bool next(const KvTilesParams& p) {
     pos += n;
-    return locate(p, ctl);
+    return locate(p);
   }
   __device__ __forceinline__ int key0(int j) const {   // first key of the segment's j-th block
     const int i = k0 + j;
@@ -148,8 +175,8 @@ __device__ __forceinline__ void kt_expand(uint4 x, uint8_t* tile, int row, int c
 // A raw tile of 128 rows: a thread takes one chunk of 16 columns of every 16th row, so that eight lanes write eight
 // rows; four rows are read before the first is written.  e: the exponents of the block's pages (2^(e - top) is the
 // factor); a value 2^24 below is lost, rows past the end are anything finite.  Kept small: the roles share an
-// instruction cache, and with this unrolled for keys and values apart every warp of the CTA ran at half its pace (16 x 4
-// queries over 24000 keys, 64 / 8 heads, 366 us; 278 so).
+// instruction cache, and with this unrolled for keys and values apart every warp of the CTA ran at half its pace (366 us
+// where this took 278).
 __device__ __forceinline__ void kt_expand_tile(const uint8_t* raw, uint8_t* tile, int tid, const uint16_t* exps, int shift,
                                                int lg, int top, bool same) {
   const int r = (tid & 7) + 8 * (tid >> 6), chunk = (tid >> 3) & 7;
@@ -179,9 +206,33 @@ __device__ __forceinline__ void kt_store8(float* dst, const float* v) {   // a w
                : "memory");
 }
 
+// Scores from the `to`-th on become -inf.
+template <int N>
+__device__ __forceinline__ void kt_mask(uint32_t (&s)[N], int to) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = i < to ? s[i] : 0xff800000u;
+}
+// Scores in [from, to) become -inf.
+template <int N>
+__device__ __forceinline__ void kt_mask_between(uint32_t (&s)[N], int from, int to) {
+  const uint32_t width = to > from ? static_cast<uint32_t>(to - from) : 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = static_cast<uint32_t>(i - from) < width ? 0xff800000u : s[i];
+}
+template <int N>
+__device__ __forceinline__ float kt_max(const uint32_t (&s)[N]) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+#pragma unroll
+  for (int i = 8; i < N; i += 2)
+    m[(i >> 1) & 3] = cp_max3(m[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+  return fmaxf(cp_max3(m[0], m[1], m[2]), m[3]);
+}
+
 // The scores FROM ... TO-1 become fp16 probabilities, two to a word, in s[FROM / 2 ...], their sums go to sum4.
-template <int FROM, int TO>
-__device__ __forceinline__ void kt_probabilities(uint32_t (&s)[128], float scale, float plus, uint64_t (&sum4)[4]) {
+template <int FROM, int TO, int N>
+__device__ __forceinline__ void kt_probabilities(uint32_t (&s)[N], float scale, float plus, uint64_t (&sum4)[4]) {
   const uint64_t scale2 = cp_pack(scale, scale), plus2 = cp_pack(plus, plus);
 #pragma unroll
   for (int i = FROM; i < TO; i += 2) {
@@ -194,11 +245,20 @@ __device__ __forceinline__ void kt_probabilities(uint32_t (&s)[128], float scale
   }
 }
 
-// The role of warps 4 to 7: queries, keys and values to fp16 tiles.
-__device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, uint8_t* sQ, uint32_t per, uint32_t total) {
-  uint8_t* sK = sQ + CP_TILE;
-  uint8_t* sV = sK + KT_RING * CP_TILE;
-  uint8_t* sR = sV + KT_RING * CP_TILE;
+__device__ __forceinline__ void kt_tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::
+          "r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// The role of warps 4 to 7: queries to two e4m3 tiles, values to fp16 tiles.
+template <int kCopies>
+__device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, uint8_t* sQ) {
+  uint8_t* sV = sQ + 2 * KT_Q8;
+  uint8_t* sR = sV + KT_VALS * CP_TILE;
   const uint32_t lane = threadIdx.x & 31u;
   const int tile_rows = p.qrows * p.group;
   const int tid = static_cast<int>(threadIdx.x) - 128;
@@ -213,19 +273,19 @@ __device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, 
   KtWalk w;
   bool ok = true;
   uint32_t seg = 0, g = 0;
-  for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
+  for (bool more = w.start(p, ctl); ok && more; more = w.next(p), ++seg) {
     if (seg > 0) ok = wait_all(&ctl.q_empty, (seg - 1) & 1u, 0xA36);
     if (!ok) break;
-    // Queries: eight lanes take a row, brought to [1, 2) by a power of two so that fp16 holds it.
+    // Queries: eight lanes take a row, brought to [128, 256) by a power of two; what is left of a number after its
+    // first term is below 1/16 of it and fits the second.
     {
       const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, chunk = tid & 7;
 #pragma unroll 1
-      for (int r0 = 0; r0 < CP_BM; r0 += 4 * KT_EXPANDERS) {
-        const int r = r0 + (tid >> 3);         // whole warps go on together: the shuffles below
-        const int in = r / p.group, tok = qt * p.qrows + in;
-        const bool there = r < tile_rows && tok < w.span.count;
+      for (int r = tid >> 3; r < CP_BM; r += 4 * KT_EXPANDERS) {
+        const int row = r & (CP_BM / kCopies - 1), in = row / p.group, tok = qt * p.qrows + in;
+        const bool there = row < tile_rows && tok < w.span.count;
         const __nv_bfloat16* src = p.q + b * p.q_sb + tok * p.q_ss +
-                                   static_cast<long long>(w.head * p.group + r - in * p.group) * p.q_sh + 16 * chunk;
+                                   static_cast<long long>(w.head * p.group + row - in * p.group) * p.q_sh + 16 * chunk;
         float x[16];
         float amax = 0.f;
 #pragma unroll
@@ -238,77 +298,83 @@ __device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, 
         }
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-        e = e < -60 ? -60 : e > 100 ? 100 : e;
-        const float down = kv_pow2(-e);
-        uint32_t h[8];
+        int e = static_cast<int>(__float_as_uint(amax) >> 23) - 134;
+        e = e < -100 ? -100 : e;
+        const float down = e > 120 ? NAN : kv_pow2(-e);   // an infinity: its scores are no numbers
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const __half2 y = __floats2half2_rn(x[2 * i] * down, x[2 * i + 1] * down);
-          h[i] = *reinterpret_cast<const uint32_t*>(&y);
+        for (int i = 0; i < 4; ++i) {
+          float rest[4];
+          hi[i] = lo[i] = 0;
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const float2 v = make_float2(x[4 * i + k] * down, x[4 * i + k + 1] * down);
+            const uint32_t two = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
+            const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+            const float2 f = __half22float2(__half2(back));
+            rest[k] = v.x - f.x, rest[k + 1] = v.y - f.y;
+            hi[i] |= two << (8 * k);
+          }
+          lo[i] = __nv_cvt_float2_to_fp8x2(make_float2(rest[0], rest[1]), __NV_SATFINITE, __NV_E4M3) |
+                  static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(rest[2], rest[3]), __NV_SATFINITE, __NV_E4M3))
+                      << 16;
         }
-        if (r >= CP_BM) continue;
-        uint8_t* dst = sQ + (chunk >> 2) * CP_SUB + r * 128;
-        const int c0 = 2 * (chunk & 3);
-        *reinterpret_cast<uint4*>(dst + ((c0 ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        uint8_t* dst = sQ + r * KV_D + ((chunk ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + KT_Q8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if (chunk == 0) ctl.row_exp[seg & 1u][r] = static_cast<int8_t>(e);
       }
     }
     fence_proxy_async_smem();
     arrive(&ctl.q_full);
-    // A block's keys, then its values.  (Keys a block ahead hold the raw ring longer: 450 us instead of 278.)
     for (int j = 0; ok && j < w.n; ++j, ++g) {
-      const uint32_t s = g % KT_RING, par = (g / KT_RING) & 1u;
-      ok = wait_all(&ctl.raw_full[s], par, 0xA37);
-      if (ok && g >= KT_RING) ok = wait_all(&ctl.k_empty[s], par ^ 1u, 0xA38);
+      const uint32_t s = g % KT_RAWS, v = g % KT_VALS;
+      ok = wait_all(&ctl.raw_full[s], (g / KT_RAWS) & 1u, 0xA37);
+      if (ok && g >= KT_VALS) ok = wait_all(&ctl.v_empty[v], (g / KT_VALS - 1) & 1u, 0xA39);
       if (!ok) break;
-      const int4 blk = ctl.blk[s];
-      if (tid == 0) ctl.sc[g & 3u] = make_float2(kv_pow2(blk.x), static_cast<float>(blk.y));
-      arrive(&ctl.sc_full[g & 3u]);
-#pragma unroll 1
-      for (int side = 0; ok && side < 2; ++side) {
-        if (side == 1 && g >= KT_RING) ok = wait_all(&ctl.v_empty[s], par ^ 1u, 0xA39);
-        if (!ok) break;
-        kt_expand_tile(sR + s * KT_RAW + side * (KT_BN * KV_D), (side ? sV : sK) + s * CP_TILE, tid, ctl.exps[s], 8 * side,
-                       lg, side ? blk.y : blk.x, (side ? blk.w : blk.z) != 0);
-        fence_proxy_async_smem();
-        arrive(side ? &ctl.v_full[s] : &ctl.k_full[s]);
-      }
-      if (!ok) break;
+      const int4 blk = ctl.blk[g % KT_SCALES];
+      kt_expand_tile(sR + s * KT_RAW + KT_BN * KV_D, sV + v * CP_TILE, tid, ctl.exps[g % KT_SCALES], 8, lg, blk.y, blk.w != 0);
+      fence_proxy_async_smem();
+      arrive(&ctl.v_full[v]);
       arrive(&ctl.raw_empty[s]);
     }
   }
 }
 
+// kCopies: of each row in the tile, in quadrants of their own.  Tensor memory gives a warp its quadrant's 32 lanes only, so
+// that up to 32 rows would be the work of one warp, 3000 cycles a block, while three idle.  With copies each quadrant
+// takes the probabilities of its share of a block's keys and leaves zeros for the others; the copies' results are
+// added at the end of a segment, as the streams' are.
+template <int kCopies>
 __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_constant__ KvTilesParams p) {
-  extern __shared__ __align__(1024) uint8_t kt_smem[];
-  uint8_t* sQ = kt_smem;
+  extern __shared__ __align__(1024) uint8_t kt_smem_raw[];
+  constexpr int kRows = CP_BM / kCopies, kKeys = KT_BN / kCopies;   // rows of the tile, keys of a quadrant
+  uint8_t* sQ = kt_smem_raw;
   if ((smem_u32(sQ) & 1023u) != 0u) {
     if (threadIdx.x == 0) report_status(p.status, CB_BAD_ARGUMENT, 0, 0xA3F);
     return;
   }
-  uint8_t* sK = sQ + CP_TILE;
-  uint8_t* sV = sK + KT_RING * CP_TILE;
-  uint8_t* sR = sV + KT_RING * CP_TILE;
-  KtCtl& ctl = *reinterpret_cast<KtCtl*>(kt_smem + KT_TILES);
+  uint8_t* sV = sQ + 2 * KT_Q8;
+  uint8_t* sR = sV + KT_VALS * CP_TILE;
+  float* sO = reinterpret_cast<float*>(kt_smem_raw + KT_TILES);
+  KtCtl& ctl = *reinterpret_cast<KtCtl*>(kt_smem_raw + kt_smem(kCopies) - sizeof(KtCtl));
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const int tile_rows = p.qrows * p.group;
-  const uint32_t active = static_cast<uint32_t>(tile_rows + 31) / 32;   // softmax warps per stream
+  const uint32_t active = kCopies > 1 ? 4u : static_cast<uint32_t>(tile_rows + 31) / 32;   // softmax warps per stream
   const int entries = p.batch.B * p.nqt;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < KT_RING; ++i) {
+    for (int i = 0; i < KT_RAWS; ++i) {
       mbar_init(&ctl.raw_full[i], 1);
-      mbar_init(&ctl.raw_empty[i], KT_EXPANDERS);
-      mbar_init(&ctl.k_full[i], KT_EXPANDERS);
-      mbar_init(&ctl.k_empty[i], 1);
+      mbar_init(&ctl.raw_empty[i], KT_EXPANDERS + 1);   // values expanded, scores computed
+    }
+    for (int i = 0; i < KT_VALS; ++i) {
       mbar_init(&ctl.v_full[i], KT_EXPANDERS);
       mbar_init(&ctl.v_empty[i], 1);
     }
     mbar_init(&ctl.q_full, KT_EXPANDERS);
     mbar_init(&ctl.q_empty, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&ctl.sc_full[i], KT_EXPANDERS);
+    for (int i = 0; i < KT_SCALES; ++i) mbar_init(&ctl.sc_full[i], 1);
     mbar_init(&ctl.seg_full, 2 * active);
     mbar_init(&ctl.seg_done, 2 * active);
     for (int i = 0; i < 2; ++i) {
@@ -316,6 +382,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
       mbar_init(&ctl.p_first[i], active);
       mbar_init(&ctl.p_rest[i], active);
       mbar_init(&ctl.pv_done[i], 1);
+      mbar_init(&ctl.piece_full[i], 4);
     }
     ctl.abort_flag = 0;
     fence_mbar_init();
@@ -326,30 +393,39 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
   }
   pdl_wait();
   pdl_launch_dependents();
-  if (warp == 0) {                                          // blocks before each entry
-    uint32_t before = 0;
-    for (int e0 = 0; e0 < entries; e0 += 32) {
-      const int e = e0 + static_cast<int>(lane);
-      const uint32_t mine = e < entries ? static_cast<uint32_t>(kt_span(p, e).n) * p.cache.hkv : 0u;
-      uint32_t x = mine;
+  if (warp == 0) {                                          // blocks before each entry, a CTA's first one
+    uint32_t first[KT_MAX_ENTRIES / 32], mine[KT_MAX_ENTRIES / 32], total = 0;
+#pragma unroll
+    for (int i = 0; i < KT_MAX_ENTRIES / 32; ++i) {
+      const int e = 32 * i + static_cast<int>(lane);
+      first[i] = total;
+      mine[i] = e < entries ? static_cast<uint32_t>(kt_span(p, e).n) * p.cache.hkv : 0u;
+      if (32 * i >= entries) continue;
+      uint32_t x = mine[i];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= static_cast<uint32_t>(o)) x += y;
       }
-      if (e < entries) ctl.base[e] = before + x - mine;
-      before += __shfl_sync(0xffffffffu, x, 31);
+      first[i] += x - mine[i];
+      total += __shfl_sync(0xffffffffu, x, 31);
     }
-    if (lane == 0) ctl.base[entries] = before;
+    const uint32_t even = (total + gridDim.x - 1) / gridDim.x, per = even < KT_MIN_BLOCKS ? KT_MIN_BLOCKS : even;
+    const uint32_t at = blockIdx.x * per;
+#pragma unroll
+    for (int i = 0; i < KT_MAX_ENTRIES / 32; ++i) {
+      const int e = 32 * i + static_cast<int>(lane);
+      if (at >= first[i] && at - first[i] < mine[i]) ctl.entry = e, ctl.base = first[i];
+      if (blockIdx.x == 0 && e < entries) p.plan[e] = first[i];
+    }
+    if (lane == 0) {
+      ctl.total = total, ctl.per = per;
+      if (blockIdx.x == 0) p.plan[entries] = total, p.plan[entries + 1] = per;
+    }
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t total = ctl.base[entries];
-  const uint32_t even = (total + gridDim.x - 1) / gridDim.x;
-  const uint32_t per = even < KT_MIN_BLOCKS ? KT_MIN_BLOCKS : even;
-  if (blockIdx.x == 0)
-    for (int e = threadIdx.x; e <= entries + 1; e += KT_THREADS) p.plan[e] = e <= entries ? ctl.base[e] : per;
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl.tmem_base);
   // stream t: S (fp32, 128 columns; the first 64 hold P as fp16 pairs after the softmax) at column 256 t, O at column
   // 256 t + 128.
@@ -364,7 +440,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
       KtWalk w;
       bool ok = true;
       uint32_t g = 0;
-      for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl)) {
+      for (bool more = w.start(p, ctl); ok && more; more = w.next(p)) {
         const int b = w.entry / p.nqt, end = w.span.start + w.span.count;
         const int* row = p.batch.pages + static_cast<long long>(b) * p.batch.cols;
         // lane l looks page l of a block up, a block ahead
@@ -385,9 +461,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
         };
         look_up(0);
         for (int j = 0; ok && j < w.n; ++j, ++g) {
-          const uint32_t s = g % KT_RING;
-          if (g >= KT_RING)
-            ok = mbar_wait_warp(&ctl.raw_empty[s], (g / KT_RING - 1) & 1u, &ctl.abort_flag, p.status, 0xA30);
+          const uint32_t s = g % KT_RAWS;
+          if (g >= KT_RAWS)
+            ok = mbar_wait_warp(&ctl.raw_empty[s], (g / KT_RAWS - 1) & 1u, &ctl.abort_flag, p.status, 0xA30);
           if (!ok) break;
           const bool there = static_cast<int>(lane) < pages && w.key0(j) + (static_cast<int>(lane) << lg) < end;
           const int ek = static_cast<int8_t>(ex), ev = static_cast<int8_t>(ex >> 8);
@@ -397,9 +473,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
           if (top_v == KV_EXP_MIN) top_v = 0;
           const bool same_k = __all_sync(0xffffffffu, !there || ek == top_k);
           const bool same_v = __all_sync(0xffffffffu, !there || ev == top_v);
-          if (lane < 8) ctl.exps[s][lane] = static_cast<uint16_t>(ex);   // pages that are not there: 0
-          if (lane == 0) ctl.blk[s] = make_int4(top_k, top_v, same_k, same_v);
+          // The scores of block g - 3 are complete: those are issued after the probabilities of g - 5 have come, so
+          // that no softmax reads the scales of g - 8 any more.
+          if (lane < 8) ctl.exps[g % KT_SCALES][lane] = static_cast<uint16_t>(ex);   // pages that are not there: 0
+          if (lane == 0) ctl.blk[g % KT_SCALES] = make_int4(top_k, top_v, same_k, same_v);
           __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.sc_full[g % KT_SCALES]);
           if (lane == 0) mbar_arrive_expect_tx(&ctl.raw_full[s], KT_RAW);
           __syncwarp();
           const int src = __shfl_sync(0xffffffffu, pid, lane >> 1);
@@ -412,41 +491,39 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
     } else if (warp == 1) {
       // ------------------------------------------------------------------- MMA
       // The whole warp walks the schedule and waits; one elected lane issues.
-      constexpr uint32_t idesc_s = make_idesc(128, 128, 0u);
-      constexpr uint32_t idesc_pv = make_idesc(128, 128, 0u) | (1u << 16);  // V is MN-major
+      constexpr uint32_t idesc_s = make_idesc(128, 128, 0u);                // e4m3
+      constexpr uint32_t idesc_pv = make_idesc(128, 128, 0u) | (1u << 16);  // fp16, V is MN-major
       const uint64_t q_desc = make_sw128_kmajor_desc(smem_u32(sQ));
-      const uint64_t k_desc0 = make_sw128_kmajor_desc(smem_u32(sK));
+      const uint64_t k_desc0 = make_sw128_kmajor_desc(smem_u32(sR));
       const uint64_t v_desc0 = cp_mnmajor_desc(smem_u32(sV));
-      constexpr uint64_t kTileStep = static_cast<uint64_t>(CP_TILE >> 4);
-      constexpr uint64_t kSubStep = static_cast<uint64_t>(CP_SUB >> 4);
+      constexpr uint64_t kTileStep = static_cast<uint64_t>(CP_TILE >> 4), kRawStep = static_cast<uint64_t>(KT_RAW >> 4);
       auto wait_all = [&](uint64_t* bar, uint32_t parity, uint32_t detail) -> bool {
         return mbar_wait_warp(bar, parity, &ctl.abort_flag, p.status, detail);
       };
       uint32_t g0 = 0;                 // blocks before this segment
       uint32_t pv_count[2] = {0u, 0u};
       auto issue_qk = [&](int j, bool last) -> bool {
-        const uint32_t g = g0 + j, s = g % KT_RING, t = j & 1;
-        if (!wait_all(&ctl.k_full[s], (g / KT_RING) & 1u, 0xA31)) return false;
+        const uint32_t g = g0 + j, s = g % KT_RAWS, t = j & 1;
+        if (!wait_all(&ctl.raw_full[s], (g / KT_RAWS) & 1u, 0xA31)) return false;
         tc_fence_after_sync();
         if (elect_one()) {
-          const uint64_t ka = k_desc0 + s * kTileStep;
+          const uint64_t ka = k_desc0 + s * kRawStep;
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t off = (kk >> 2) * kSubStep + 2u * (kk & 3);
-            mma_bf16_ss(tmem + 256u * t, q_desc + off, ka + off, idesc_s, kk > 0 ? 1u : 0u);
-          }
+          for (int kk = 0; kk < 8; ++kk)   // 32 columns: first terms, second terms
+            mma_fp8_ss(tmem + 256u * t, q_desc + (kk >> 2) * static_cast<uint64_t>(KT_Q8 >> 4) + 2u * (kk & 3),
+                       ka + 2u * (kk & 3), idesc_s, kk > 0 ? 1u : 0u);
           mma_commit(&ctl.s_full[t]);
-          mma_commit(&ctl.k_empty[s]);
+          mma_commit(&ctl.raw_empty[s]);
           if (last) mma_commit(&ctl.q_empty);
         }
         __syncwarp();
         return true;
       };
       auto issue_pv = [&](int j) -> bool {
-        const uint32_t g = g0 + j, s = g % KT_RING, t = j & 1;
+        const uint32_t g = g0 + j, s = g % KT_VALS, t = j & 1;
         const uint32_t par = pv_count[t] & 1u;
-        if (!wait_all(&ctl.p_first[t], par, 0xA32)) return false;
-        if (!wait_all(&ctl.v_full[s], (g / KT_RING) & 1u, 0xA33)) return false;
+        if (!mbar_wait_both(&ctl.v_full[s], (g / KT_VALS) & 1u, 0xA33, &ctl.p_first[t], par, 0xA32, &ctl.abort_flag, p.status))
+          return false;
         ++pv_count[t];
         tc_fence_after_sync();
         const uint64_t va = v_desc0 + s * kTileStep;
@@ -457,8 +534,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
             mma_bf16_ts(d, tmem + 256u * t + 8u * kk, va + kk * (2048u >> 4), idesc_pv, (j > 1 || kk > 0) ? 1u : 0u);
         }
         __syncwarp();
-        if (!wait_all(&ctl.p_rest[t], par, 0xA34)) return false;
-        tc_fence_after_sync();
+        if (kCopies == 1) {
+          if (!wait_all(&ctl.p_rest[t], par, 0xA34)) return false;
+          tc_fence_after_sync();
+        }
         if (elect_one()) {
 #pragma unroll
           for (int kk = 4; kk < 8; ++kk)
@@ -472,7 +551,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
       KtWalk w;
       bool ok = true;
       uint32_t seg = 0;
-      for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
+      for (bool more = w.start(p, ctl); ok && more; more = w.next(p), ++seg) {
         ok = wait_all(&ctl.q_full, seg & 1u, 0xA35);
         for (int j = 0; ok && j < 2 && j < w.n; ++j) ok = issue_qk(j, j + 1 == w.n);
         for (int j = 0; ok && j < w.n; ++j) {
@@ -486,7 +565,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
     }
   } else if (warp < 8) {
     cp_reg_dec<72>();
-    kt_expander(p, ctl, sQ, per, total);
+    kt_expander<kCopies>(p, ctl, sQ);
   } else {
     cp_reg_inc<184>();
     // ----------------------------------------------------------------- softmax
@@ -496,42 +575,50 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
     const uint32_t lane_addr = (q * 32u) << 16;
     const uint32_t tS = tmem + 256u * t + lane_addr;
     const uint32_t tO = tS + 128u;
-    const int q_in_tile = r / p.group;
+    const int row = r & (kRows - 1), part = r / kRows;     // the keys kKeys part ... of a block are this warp's
+    const int q_in_tile = row / p.group;
+    uint32_t pieces = 0;
     KtWalk w;
     bool ok = q < active;
     uint32_t count = 0;                                    // blocks this stream has seen
     uint32_t seg = 0, g0 = 0;
-    for (bool more = w.start(p, ctl, per, total); ok && more; more = w.next(p, ctl), ++seg) {
+    for (bool more = w.start(p, ctl); ok && more; more = w.next(p), ++seg) {
       const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, tok = qt * p.qrows + q_in_tile;
-      const bool query = r < tile_rows && tok < w.span.count;
+      const bool query = row < tile_rows && tok < w.span.count;
       const bool padded = __any_sync(0xffffffffu, !query);   // the loads of tensor memory below want a converged warp
       const int tile_first = w.span.q_first, q_pos = w.span.start + tok;
       const int tile_last = tile_first + p.qrows - 1;
       float m_ref = -INFINITY, l = 0.f, row_scale = 0.f;
       for (int j = t; ok && j < w.n; j += 2) {
         const uint32_t g = g0 + j;
-        ok = mbar_wait(&ctl.sc_full[g & 3u], (g >> 2) & 1u, &ctl.abort_flag, p.status, 0xA3A) &&
+        ok = mbar_wait(&ctl.sc_full[g % KT_SCALES], (g / KT_SCALES) & 1u, &ctl.abort_flag, p.status, 0xA3A) &&
              mbar_wait(&ctl.s_full[t], count & 1u, &ctl.abort_flag, p.status, 0xA3B);
         if (!ok) break;
         ++count;
         tc_fence_after_sync();
-        const float2 sc = ctl.sc[g & 3u];
+        const int4 blk = ctl.blk[g % KT_SCALES];
+        const float2 sc = make_float2(kv_pow2(blk.x), static_cast<float>(blk.y));
         if (j == t) row_scale = p.scale_log2 * kv_pow2(ctl.row_exp[seg & 1u][r]);
         const float scale = fmaxf(row_scale * sc.x, 1.2e-38f);
-        uint32_t s[128];
-        tmem_ld_32x32_at(tS, &s[0]);
-        tmem_ld_32x32_at(tS + 32u, &s[32]);
-        tmem_ld_32x32_at(tS + 64u, &s[64]);
-        tmem_ld_32x32_at(tS + 96u, &s[96]);
+        uint32_t s[kKeys];
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 32) tmem_ld_32x32_at(tS + part * kKeys + i, &s[i]);
         tmem_wait_ld();
-        const int key0 = w.key0(j);
-        if (key0 + KT_BN - 1 > tile_first || padded) cp_mask_tail(s, query ? q_pos - key0 + 1 : 0);
-        if (p.window > 0 && key0 <= tile_last - p.window && key0 + KT_BN > p.sinks)
-          cp_mask_range(s, max(p.sinks - key0, 0), min(q_pos - p.window + 1 - key0, KT_BN));
-        float mx8[8];
-        cp_row_max(s, mx8);
-        const float mx_all = cp_max3(fmaxf(cp_max3(mx8[0], mx8[1], mx8[2]), cp_max3(mx8[3], mx8[4], mx8[5])), mx8[6], mx8[7]);
-        const float mx = fmaf(mx_all, scale, sc.y);
+        if (blk.z == 0) {   // other exponents of keys in the block
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i) {
+            int e = static_cast<int8_t>(ctl.exps[g % KT_SCALES][(kKeys * part + 16 * i) >> p.cache.page_log2]) - blk.x;
+            e = e > 0 ? 0 : e < -126 ? -126 : e;
+            const float f = kv_pow2(e);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) s[16 * i + k] = __float_as_uint(__uint_as_float(s[16 * i + k]) * f);
+          }
+        }
+        const int key0 = w.key0(j) + kKeys * part;
+        if (key0 + kKeys - 1 > tile_first || padded) kt_mask(s, query ? q_pos - key0 + 1 : 0);
+        if (p.window > 0 && key0 <= tile_last - p.window && key0 + kKeys > p.sinks)
+          kt_mask_between(s, max(p.sinks - key0, 0), min(q_pos - p.window + 1 - key0, kKeys));
+        const float mx = fmaf(kt_max(s), scale, sc.y);
         // The running maximum, raised when a score passes it by 2^8, for all rows of the warp (see cp_update_max).
         const bool grow = query && (mx > m_ref + CP_RESCALE_THRESHOLD || (m_ref == -INFINITY && mx > -INFINITY));
         if (__any_sync(0xffffffffu, grow)) {
@@ -553,8 +640,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
         }
         const float plus = sc.y - (m_ref == -INFINITY ? 0.f : m_ref);
         uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull};
-        kt_probabilities<0, 64>(s, scale, plus, sum4);
-        tmem_st_32x32_at(tS, &s[0]);
+        kt_probabilities<0, (kCopies > 1 ? kKeys : 64)>(s, scale, plus, sum4);
+        if (kCopies == 1) {
+          tmem_st_32x32_at(tS, &s[0]);
+        } else {
+          const uint32_t none[16] = {};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {   // 16 words each: this quadrant's, then the others' zeros
+            const uint32_t at = tS + 16u * ((part * (4 / kCopies) + i) & 3);
+            kt_tmem_st16(at, i < 4 / kCopies ? &s[16 * (i < 4 / kCopies ? i : 0)] : none);
+          }
+        }
         tmem_wait_st();
         // Both streams' O of the segment before must have been read before this hand-over.
         if (j < 2 && seg > 0 && !mbar_wait(&ctl.seg_done, (seg - 1) & 1u, &ctl.abort_flag, p.status, 0xA3C)) {
@@ -564,12 +660,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.p_first[t]);
-        kt_probabilities<64, 128>(s, scale, plus, sum4);
-        tmem_st_32x32_at(tS + 32u, &s[32]);
-        tmem_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.p_rest[t]);
+        if constexpr (kCopies == 1) {
+          kt_probabilities<64, 128>(s, scale, plus, sum4);
+          tmem_st_32x32_at(tS + 32u, &s[32]);
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.p_rest[t]);
+        }
         float sum = 0.f;
         cp_add_sums(sum4, sum);
         l = fmaf(sum, kv_pow2(-static_cast<int>(sc.y)), l);
@@ -588,48 +686,102 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
       if (lane == 0) mbar_arrive(&ctl.seg_full);
       if (!mbar_wait(&ctl.seg_full, seg & 1u, &ctl.abort_flag, p.status, 0xA40)) break;
       tc_fence_after_sync();
+      // Over the streams and the copies.  One without a visible key has no O: its columns may hold anything.  (A NaN
+      // sum counts as visible.)
+      float m = -INFINITY, lsum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * kCopies; ++i) m = fmaxf(m, ctl.ml[i & 1][row + (i >> 1) * kRows].x);
+      auto weight = [&](float2 ml) { return ml.y == 0.f ? 0.f : ml.x == m ? 1.f : exp2f(ml.x - m); };
+#pragma unroll
+      for (int i = 0; i < 2 * kCopies; ++i) {
+        const float2 ml = ctl.ml[i & 1][row + (i >> 1) * kRows];
+        lsum += ml.y == 0.f ? 0.f : weight(ml) * ml.y;
+      }
       const float2 ml0 = ctl.ml[0][r], ml1 = ctl.ml[1][r];
-      const float m = fmaxf(ml0.x, ml1.x);
-      // A stream without a visible key has no O: its columns may hold anything.  (A NaN sum counts as visible.)
       const bool use0 = ml0.y != 0.f, use1 = ml1.y != 0.f;
-      const float a0 = use0 ? (ml0.x == m ? 1.f : exp2f(ml0.x - m)) : 0.f;
-      const float a1 = use1 ? (ml1.x == m ? 1.f : exp2f(ml1.x - m)) : 0.f;
-      const float lsum = (use0 ? a0 * ml0.y : 0.f) + (use1 ? a1 * ml1.y : 0.f);
-      const int h = w.head * p.group + (r - q_in_tile * p.group);
-      const bool row_ok = r < tile_rows && tok < p.batch.S;
+      const float a0 = weight(ml0), a1 = weight(ml1);
+      const int h = w.head * p.group + (row - q_in_tile * p.group);
+      const bool row_ok = row < tile_rows && tok < p.batch.S;
       const bool whole = w.n == w.span.n;
       const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-      const size_t part = (static_cast<size_t>(2u * blockIdx.x) + (w.k0 == 0 ? 1u : 0u)) * tile_rows + r;
+      const size_t part_at = (static_cast<size_t>(2u * blockIdx.x) + (w.k0 == 0 ? 1u : 0u)) * tile_rows + row;
+      __nv_bfloat16* dst = p.o + ((static_cast<size_t>(b) * p.batch.S + tok) * p.Hq + h) * KV_D;
+      if constexpr (kCopies == 1) {
 #pragma unroll 1
-      for (int c = 2 * t; c < 2 * t + 2; ++c) {
-        uint32_t o0[32], o1[32];
-        tmem_ld_32x32(tmem + lane_addr + 128u + c * 32u, o0);
-        tmem_ld_32x32(tmem + lane_addr + 384u + c * 32u, o1);
-        tmem_wait_ld();
-        float o[32];
+        for (int c = 2 * t; c < 2 * t + 2; ++c) {
+          uint32_t o0[32], o1[32];
+          tmem_ld_32x32(tmem + lane_addr + 128u + c * 32u, o0);
+          tmem_ld_32x32(tmem + lane_addr + 384u + c * 32u, o1);
+          tmem_wait_ld();
+          float o[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          o[i] = (use0 ? a0 * __uint_as_float(o0[i]) : 0.f) + (use1 ? a1 * __uint_as_float(o1[i]) : 0.f);
-        if (!row_ok) continue;
-        if (whole) {
-          __nv_bfloat16* dst =
-              p.o + ((static_cast<size_t>(b) * p.batch.S + tok) * p.Hq + h) * KV_D + c * 32;
+          for (int i = 0; i < 32; ++i)
+            o[i] = (use0 ? a0 * __uint_as_float(o0[i]) : 0.f) + (use1 ? a1 * __uint_as_float(o1[i]) : 0.f);
+          if (!row_ok) continue;
+          if (whole) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 v;
-            __nv_bfloat162* hh = reinterpret_cast<__nv_bfloat162*>(&v);
+            for (int i = 0; i < 32; i += 8) {
+              uint4 v;
+              __nv_bfloat162* hh = reinterpret_cast<__nv_bfloat162*>(&v);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) hh[k] = __floats2bfloat162_rn(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
-            *reinterpret_cast<uint4*>(dst + i) = v;
+              for (int k = 0; k < 4; ++k) hh[k] = __floats2bfloat162_rn(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+              *reinterpret_cast<uint4*>(dst + c * 32 + i) = v;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) kt_store8(p.part_o + part_at * KV_D + c * 32 + i, o + i);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) kt_store8(p.part_o + part * KV_D + c * 32 + i, o + i);
         }
+      } else {
+        // Through shared memory: every thread writes 16 columns of its copy, and then adds up its share of them.  Two
+        // pieces: what a warp overwrites was read by all before they came to the barrier in between.
+        float* stage = sO + t * (2 * CP_BM * KT_PIECE);
+        constexpr int kWords = 4 / kCopies;                 // four columns each
+#pragma unroll 1
+        for (int c = 64 * t; ok && c < 64 * t + 64; c += KT_PIECE, ++pieces) {
+          uint32_t o0[16], o1[16];
+          tmem_ld_32x16(tmem + lane_addr + 128u + c, o0);
+          tmem_ld_32x16(tmem + lane_addr + 384u + c, o1);
+          tmem_wait_ld();
+          float4* piece = reinterpret_cast<float4*>(stage + (pieces & 1u) * (CP_BM * KT_PIECE));
+          float o[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            o[i] = (use0 ? a0 * __uint_as_float(o0[i]) : 0.f) + (use1 ? a1 * __uint_as_float(o1[i]) : 0.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)                       // eight rows of 64 bytes in different banks
+            piece[4 * r + (i ^ ((r >> 1) & 3))] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.piece_full[t]);
+          ok = mbar_wait_warp(&ctl.piece_full[t], pieces & 1u, &ctl.abort_flag, p.status, 0xA41);
+          if (ok && row_ok) {
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) {
+              const int word = part * kWords + k;
+              float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < kCopies; ++i) {
+                const int from = row + i * kRows;
+                const float4 x = piece[4 * from + (word ^ ((from >> 1) & 3))];
+                sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+              }
+              const int col = c + 4 * word;
+              if (whole) {
+                const __nv_bfloat162 o2[2] = {__floats2bfloat162_rn(sum.x * inv, sum.y * inv),
+                                              __floats2bfloat162_rn(sum.z * inv, sum.w * inv)};
+                *reinterpret_cast<uint2*>(dst + col) = *reinterpret_cast<const uint2*>(o2);
+              } else {
+                *reinterpret_cast<float4*>(p.part_o + part_at * KV_D + col) = sum;
+              }
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
       }
-      if (t == 0 && row_ok) {
+      if (t == 0 && part == 0 && row_ok) {
         if (!whole)
-          p.part_ml[part] = make_float2(m, lsum);
+          p.part_ml[part_at] = make_float2(m, lsum);
         else
           p.lse[(static_cast<size_t>(b) * p.Hq + h) * p.batch.S + tok] =
               lsum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(lsum);
@@ -719,6 +871,15 @@ static int kt_sms() {
   return n;
 }
 
+template <int kCopies>
+static cudaError_t kt_launch(const KvTilesParams& p, int grid, cudaStream_t st) {
+  static std::atomic<uint64_t> smem_done{0};
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv_tiles_kernel<kCopies>), kt_smem(kCopies), smem_done);
+  return e != cudaSuccess ? e
+                          : launch_pdl(kv_tiles_kernel<kCopies>, dim3(static_cast<unsigned>(grid)), dim3(KT_THREADS),
+                                       kt_smem(kCopies), st, p);
+}
+
 struct KtLaunch {
   int qrows, nqt, grid;
   long long bytes, o_at, ml_at;
@@ -751,7 +912,7 @@ extern "C" {
 long long cb_kv_tiles_bytes(int B, int S, int Hq, int Hkv, int max_len) {
   KtLaunch s;
   if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || max_len < 1 || !kt_shape(&s, B, S, Hq, Hkv, max_len)) {
-    set_last_error("key/value attention: bad shape, or more than 128 heads to a group or 96 query tiles");
+    set_last_error("key/value attention: bad shape, or more than 128 heads to a group or 128 query tiles");
     return -1;
   }
   return s.bytes;
@@ -796,10 +957,9 @@ int cb_kv_tiles(void* data, void* exps, int num_pages, int hkv, int page, const 
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = static_cast<uint32_t*>(status);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  static std::atomic<uint64_t> smem_done{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv_tiles_kernel), KT_SMEM, smem_done);
-  if (e == cudaSuccess)
-    e = launch_pdl(kv_tiles_kernel, dim3(static_cast<unsigned>(s.grid)), dim3(KT_THREADS), KT_SMEM, st, p);
+  const int tile_rows = s.qrows * p.group;
+  cudaError_t e = tile_rows <= 32 ? kt_launch<4>(p, s.grid, st) : tile_rows <= 64 ? kt_launch<2>(p, s.grid, st)
+                                                                                  : kt_launch<1>(p, s.grid, st);
   if (e == cudaSuccess) {
     const long long rows = static_cast<long long>(B) * S * Hq;
     const int per = KT_MERGE_THREADS / 32;

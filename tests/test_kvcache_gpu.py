@@ -214,8 +214,8 @@ def _check(o, lse, want):
 
 
 def _tiles_take(B, S, group):
-    """The form of tiles takes at most 96 query tiles of 128 rows."""
-    return group <= 128 and B * -(-S // (128 // group)) <= 96
+    """The form of tiles takes at most 128 query tiles of 128 rows."""
+    return group <= 128 and B * -(-S // (128 // group)) <= 128
 
 
 def _case(lens, S, Hq, H, page, window=0, sinks=0, seed=20, max_len=None, count=None, scale=None, cache=None):
@@ -344,6 +344,51 @@ def test_attend_of_large_scores(native_lib):
     # |s| up to 2^9: a score is off by 2^9 * 2^-24 * a few, the weights by as much relative to each other
     tol = 2.0 ** -8 * (ro.abs() + mag) * 1.1 + 2.0 ** -11 * mag
     assert ((o.double() - ro).abs() <= tol).all() and ((lse.double() - rl).abs() <= 2.0 ** -11).all()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("S,Hq", [(4, 16), (5, 18), (12, 8), (30, 8), (33, 14)])
+def test_attend_tiles_of_pages_with_different_scales(native_lib, page, S, Hq):
+    """32, 64 and 128 rows to a tile, keys and values whose size changes by 2^8 within a block."""
+    lens = (900, 700)
+    k, v = _kv(2, 900, 2, 100)
+    size = torch.exp2((torch.arange(900, device="cuda") // 13 % 9).float()).bfloat16()[None, :, None, None]
+    k, v = k * size / 32, v * size.flip(1)
+    cache, pages = _filled(k, v, page, lens, 101)
+    q = torch.randn(2, S, Hq, D, device="cuda", generator=_gen(102)).bfloat16()
+    start = [n - S for n in lens]
+    ro, rl, mag = _attend64(q, _quantised(k, page, lens), _quantised(v, page, lens), start, [S] * 2, 0, 0)
+    # sums of |q k| up to 2^7, held to 2^-18 of that; the weights are off by as much relative to each other
+    tol = 2.0 ** -8 * (ro.abs() + mag) * 1.1 + 2.0 ** -11 * mag + 2.0 ** -24
+    for impl in ("tiles", "decode", "prefill"):
+        o, lse = cache.attend(q, pages, _ints(*start), impl=impl)
+        assert ((o.double() - ro).abs() <= tol).all(), impl
+        assert ((lse.double() - rl).abs() <= 2.0 ** -11).all(), impl
+
+
+@pytest.mark.parametrize("S", [3, 12, 40])
+def test_attend_tiles_of_small_large_and_infinite_queries(native_lib, S):
+    """A row's own power of two carries it from 2^-60 to 2^60; an infinity makes its row no numbers, and no other."""
+    k, v = _kv(1, 600, 1, 110)
+    cache, pages = _filled(k * 2.0 ** -8, v, 32, (600,), 111)
+    q = torch.randn(1, S, 8, D, device="cuda", generator=_gen(112)).bfloat16()
+    q[:, :, 1] *= 2.0 ** -60
+    q[:, :, 2] = 0
+    q[:, :, 4, 5] *= 2.0 ** -30
+    start = [600 - S]
+    want = _attend64(q, _quantised(k * 2.0 ** -8, 32, (600,)), _quantised(v, 32, (600,)), start, [S], 0, 0)
+    _check(*cache.attend(q, pages, _ints(*start), impl="tiles"), want)
+    q2 = q.clone()
+    q2[:, 1, 3, 7] = math.inf
+    o, lse = cache.attend(q2, pages, _ints(*start), impl="tiles")
+    assert not torch.isfinite(o[0, 1, 3]).any() and not torch.isfinite(lse[0, 3, 1])
+    o[0, 1, 3], lse[0, 3, 1] = want[0][0, 1, 3].to(o.dtype), want[1][0, 3, 1].float()
+    _check(o, lse, want)
+
+
+@pytest.mark.parametrize("B", [33, 100, 128])
+def test_attend_tiles_of_many_sequences(native_lib, B):
+    _case([8 + (i * 7919) % 500 for i in range(B)], 4, 8, 1, 32, max_len=520, seed=120)
 
 
 def test_attend_repeats_its_bits_and_runs_on_another_stream(native_lib):
