@@ -10,9 +10,9 @@
 //     become the sum of two e4m3 numbers each, which holds all of bf16's 8 bits (of a number 2^10 below the largest of
 //     its row 2^-18 of that one), and are multiplied by the keys in two rounds into the same scores;
 //   * four warps expand the values to fp16, exactly, into the swizzled tile of the second product (probabilities in
-//     two e4m3 numbers would reach down to 2^-17 only).  The scales of a block's values are brought to the largest of
-//     them, so that one exponent of the probabilities serves the whole block; a value 2^24 below the largest of its
-//     block is lost.  Where the pages of a block have other scales of the keys, the scores of each are multiplied;
+//     two e4m3 numbers would reach down to 2^-17 only);
+//   * a page's scales come in with the softmax: the keys' as a factor of its scores, the values' as a power of two on
+//     its probabilities, which the sum leaves out again.  A contribution 2^24 below the largest of its row is lost;
 //   * up to 32 or 64 rows stand four times or twice in the tile, so that all softmax warps have a share of the keys;
 //   * two softmax streams take alternate blocks, each with its scores, probabilities (fp16) and results in tensor
 //     memory, as in fa_split.cu, and the flat list of (sequence, query tile, head, block) is cut evenly over the
@@ -28,6 +28,7 @@
 #include <math.h>
 
 #include <string>
+#include <utility>
 
 #include "../gemm/launch.h"
 #include "fa_cp.cuh"
@@ -36,7 +37,7 @@
 namespace cb {
 void set_last_error(const std::string& s);
 
-static constexpr int KT_THREADS = 512;    // producer, MMA and two idle warps; 4 that expand; 2 x 4 of softmax
+static constexpr int KT_THREADS = 512;    // keys, MMA, values, an idle warp; 4 that expand; 2 x 4 of softmax
 static constexpr int KT_EXPANDERS = 4;
 static constexpr int KT_BN = 128;         // keys of a block
 static constexpr int KT_RAWS = 3;         // raw blocks
@@ -70,9 +71,8 @@ struct KtCtl {
   uint64_t raw_full[KT_RAWS], raw_empty[KT_RAWS], q_full, q_empty, v_full[KT_VALS], v_empty[KT_VALS];
   uint64_t sc_full[KT_SCALES];
   uint64_t s_full[2], p_first[2], p_rest[2], pv_done[2], seg_full, seg_done, piece_full[2];
-  // Of a block: the largest key and value exponent, whether all pages have it; its pages' exponents, key, value << 8.
-  int4 blk[KT_SCALES];
-  uint16_t exps[KT_SCALES][8];
+  // Of 16 keys of a block: the keys' exponent + 127 in the top bits, the values' + 128 in the lowest.
+  uint32_t scale[KT_SCALES][KT_BN / 16];
   int8_t row_exp[2][CP_BM];        // rows were multiplied by 2^-e; of a segment and the next
   float2 ml[2][CP_BM];             // (max, sum) of the segment per stream and row
   uint32_t tmem_base;
@@ -115,7 +115,7 @@ struct KtWalk {
   uint32_t pos, end;
   int entry, head, k0, n;   // blocks k0 .. k0 + n - 1 of the item
   uint32_t base;            // blocks before the entry
-  __device__ __forceinline__ bool locate(const KvTilesParams& p) {
+  __device__ __forceinline__ bool locate(const KvTilesParams& p) {   // the segment at pos
     if (pos >= end) return false;
     for (;; ++entry) {
       if (entry >= p.batch.B * p.nqt) return false;   // not with lengths that stay as they are
@@ -131,17 +131,12 @@ struct KtWalk {
     if (static_cast<uint32_t>(n) > end - pos) n = static_cast<int>(end - pos);
     return true;
   }
-  __device__ __forceinline__ bool start(const KvTilesParams& p, const KtCtl& ctl) {
+  __device__ __forceinline__ void start(const KtCtl& ctl) {
     const unsigned long long e = static_cast<unsigned long long>(blockIdx.x + 1) * ctl.per;
     pos = blockIdx.x * ctl.per;
     end = e < ctl.total ? static_cast<uint32_t>(e) : ctl.total;
     entry = ctl.entry;
     base = ctl.base;
-    return locate(p);
-  }
-  __device__ __forceinline__ bool next(const KvTilesParams& p) {
-    pos += n;
-    return locate(p);
   }
   __device__ __forceinline__ int key0(int j) const {   // first key of the segment's j-th block
     const int i = k0 + j;
@@ -149,37 +144,12 @@ struct KtWalk {
   }
 };
 
-// 16 e4m3 numbers of a row, times a power of two, as fp16 into a swizzled tile: its row, its chunk of 16 columns.
-__device__ __forceinline__ void kt_expand(uint4 x, uint8_t* tile, int row, int chunk, __half2 f, bool scaled) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t h[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(h[2 * i]), "=r"(h[2 * i + 1])
-        : "r"(w[i]));
-  }
-  if (scaled) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), f);
-      h[i] = *reinterpret_cast<const uint32_t*>(&y);
-    }
-  }
-  uint8_t* dst = tile + (chunk >> 2) * CP_SUB + row * 128;
-  const int c0 = 2 * (chunk & 3);
-  *reinterpret_cast<uint4*>(dst + ((c0 ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-  *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-}
-
-// A raw tile of 128 rows: a thread takes one chunk of 16 columns of every 16th row, so that eight lanes write eight
-// rows; four rows are read before the first is written.  e: the exponents of the block's pages (2^(e - top) is the
-// factor); a value 2^24 below is lost, rows past the end are anything finite.  Kept small: the roles share an
-// instruction cache, and with this unrolled for keys and values apart every warp of the CTA ran at half its pace (366 us
-// where this took 278).
-__device__ __forceinline__ void kt_expand_tile(const uint8_t* raw, uint8_t* tile, int tid, const uint16_t* exps, int shift,
-                                               int lg, int top, bool same) {
-  const int r = (tid & 7) + 8 * (tid >> 6), chunk = (tid >> 3) & 7;
+// A raw tile of 128 rows to fp16: a thread takes one chunk of 16 columns of every 16th row, so that eight lanes write
+// eight rows; four rows are read before the first is written.  Kept small: the roles share an instruction cache,
+// and with this unrolled for keys and values apart every warp of the CTA ran at half its pace (366 us where this took
+// 278).
+__device__ __forceinline__ void kt_expand_tile(const uint8_t* raw, uint8_t* tile, int tid) {
+  const int r = (tid & 7) + 8 * (tid >> 6), chunk = (tid >> 3) & 7, c0 = 2 * (chunk & 3);
 #pragma unroll 1
   for (int i0 = 0; i0 < 8; i0 += 4) {
     uint4 x[4];
@@ -188,14 +158,16 @@ __device__ __forceinline__ void kt_expand_tile(const uint8_t* raw, uint8_t* tile
       x[i] = *reinterpret_cast<const uint4*>(raw + (r + 16 * (i0 + i)) * KV_D + ((chunk ^ (r & 7)) << 4));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = r + 16 * (i0 + i);
-      __half2 f = __half2();
-      if (!same) {
-        int e = static_cast<int8_t>(exps[row >> lg] >> shift) - top;
-        e = e > 0 ? 0 : e < -126 ? -126 : e;
-        f = __float2half2_rn(kv_pow2(e));
-      }
-      kt_expand(x[i], tile, row, chunk, f, !same);
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint32_t h[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(h[2 * k]), "=r"(h[2 * k + 1])
+            : "r"(w[k]));
+      uint8_t* dst = tile + (chunk >> 2) * CP_SUB + (r + 16 * (i0 + i)) * 128;
+      *reinterpret_cast<uint4*>(dst + ((c0 ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
     }
   }
 }
@@ -219,30 +191,68 @@ __device__ __forceinline__ void kt_mask_between(uint32_t (&s)[N], int from, int 
 #pragma unroll
   for (int i = 0; i < N; ++i) s[i] = static_cast<uint32_t>(i - from) < width ? 0xff800000u : s[i];
 }
-template <int N>
-__device__ __forceinline__ float kt_max(const uint32_t (&s)[N]) {
-  float m[4];
+template <int FROM, int N>
+__device__ __forceinline__ float kt_max16(const uint32_t (&s)[N]) {
+  float m0 = fmaxf(__uint_as_float(s[FROM]), __uint_as_float(s[FROM + 1]));
+  float m1 = fmaxf(__uint_as_float(s[FROM + 2]), __uint_as_float(s[FROM + 3]));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-#pragma unroll
-  for (int i = 8; i < N; i += 2)
-    m[(i >> 1) & 3] = cp_max3(m[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-  return fmaxf(cp_max3(m[0], m[1], m[2]), m[3]);
+  for (int i = FROM + 4; i < FROM + 16; i += 4) {
+    m0 = cp_max3(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+    m1 = cp_max3(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+  }
+  return fmaxf(m0, m1);
 }
 
-// The scores FROM ... TO-1 become fp16 probabilities, two to a word, in s[FROM / 2 ...], their sums go to sum4.
+// Scales of 16 keys: the factor of their scores (kept off 0, which would make a NaN of -inf), the exponent of their values,
+// 2^-exponent.  Read where they are used, twice: in registers they would not fit beside 128 scores.
+struct KtScale {
+  float score, exponent, back;
+};
+__device__ __forceinline__ KtScale kt_scale(const uint32_t* from, float row_scale) {
+  uint32_t x;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(smem_u32(from)));
+  KtScale s;
+  s.score = fmaxf(row_scale * __uint_as_float(x & 0xff800000u), 1.2e-38f);
+  s.exponent = __uint_as_float(0x4b000000u | (x & 0xffu)) - 8388736.f;   // 2^23 + 128
+  s.back = __uint_as_float((255u - (x & 0xffu)) << 23);
+  return s;
+}
+
+template <int N, int... I>
+__device__ __forceinline__ float kt_row_max(const uint32_t (&s)[N], const uint32_t* scales, float row_scale,
+                                            std::integer_sequence<int, I...>) {
+  float mx = -INFINITY;
+  ([&] {
+    const KtScale f = kt_scale(scales + I, row_scale);
+    mx = fmaxf(mx, fmaf(kt_max16<16 * I>(s), f.score, f.exponent));
+  }(), ...);
+  return mx;
+}
+
+// The scores FROM ... TO-1 become fp16 probabilities, two to a word, in s[FROM / 2 ...]; returns their sum without
+// the values' exponents.
 template <int FROM, int TO, int N>
-__device__ __forceinline__ void kt_probabilities(uint32_t (&s)[N], float scale, float plus, uint64_t (&sum4)[4]) {
-  const uint64_t scale2 = cp_pack(scale, scale), plus2 = cp_pack(plus, plus);
+__device__ __forceinline__ float kt_probabilities(uint32_t (&s)[N], const uint32_t* scales, float row_scale, float m) {
+  float all = 0.f;
 #pragma unroll
-  for (int i = FROM; i < TO; i += 2) {
-    const uint64_t y = cp_fma2(cp_pack_u(s[i], s[i + 1]), scale2, plus2);
-    const float p0 = cp_ex2(__uint_as_float(static_cast<uint32_t>(y)));
-    const float p1 = cp_ex2(__uint_as_float(static_cast<uint32_t>(y >> 32)));
-    sum4[(i >> 1) & 3] = cp_add2(sum4[(i >> 1) & 3], cp_pack(p0, p1));
-    const __half2 h = __floats2half2_rn(p0, p1);
-    s[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+  for (int i0 = FROM; i0 < TO; i0 += 16) {
+    const KtScale f = kt_scale(scales + i0 / 16, row_scale);
+    const float plus = f.exponent - m;
+    const uint64_t scale2 = cp_pack(f.score, f.score), plus2 = cp_pack(plus, plus);
+    uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+    for (int i = i0; i < i0 + 16; i += 2) {
+      const uint64_t y = cp_fma2(cp_pack_u(s[i], s[i + 1]), scale2, plus2);
+      const float p0 = cp_ex2(__uint_as_float(static_cast<uint32_t>(y)));
+      const float p1 = cp_ex2(__uint_as_float(static_cast<uint32_t>(y >> 32)));
+      sum2[(i >> 1) & 1] = cp_add2(sum2[(i >> 1) & 1], cp_pack(p0, p1));
+      const __half2 h = __floats2half2_rn(p0, p1);
+      s[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const uint64_t sum = cp_add2(sum2[0], sum2[1]);
+    all = fmaf(__uint_as_float(static_cast<uint32_t>(sum)) + __uint_as_float(static_cast<uint32_t>(sum >> 32)), f.back, all);
   }
+  return all;
 }
 
 __device__ __forceinline__ void kt_tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -262,7 +272,6 @@ __device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, 
   const uint32_t lane = threadIdx.x & 31u;
   const int tile_rows = p.qrows * p.group;
   const int tid = static_cast<int>(threadIdx.x) - 128;
-  const int lg = p.cache.page_log2;
   auto arrive = [&](uint64_t* bar) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar);
@@ -273,7 +282,7 @@ __device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, 
   KtWalk w;
   bool ok = true;
   uint32_t seg = 0, g = 0;
-  for (bool more = w.start(p, ctl); ok && more; more = w.next(p), ++seg) {
+  for (w.start(ctl); ok && w.locate(p); w.pos += w.n, ++seg) {
     if (seg > 0) ok = wait_all(&ctl.q_empty, (seg - 1) & 1u, 0xA36);
     if (!ok) break;
     // Queries: eight lanes take a row, brought to [128, 256) by a power of two; what is left of a number after its
@@ -332,8 +341,7 @@ __device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, 
       ok = wait_all(&ctl.raw_full[s], (g / KT_RAWS) & 1u, 0xA37);
       if (ok && g >= KT_VALS) ok = wait_all(&ctl.v_empty[v], (g / KT_VALS - 1) & 1u, 0xA39);
       if (!ok) break;
-      const int4 blk = ctl.blk[g % KT_SCALES];
-      kt_expand_tile(sR + s * KT_RAW + KT_BN * KV_D, sV + v * CP_TILE, tid, ctl.exps[g % KT_SCALES], 8, lg, blk.y, blk.w != 0);
+      kt_expand_tile(sR + s * KT_RAW + KT_BN * KV_D, sV + v * CP_TILE, tid);
       fence_proxy_async_smem();
       arrive(&ctl.v_full[v]);
       arrive(&ctl.raw_empty[s]);
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < KT_RAWS; ++i) {
-      mbar_init(&ctl.raw_full[i], 1);
+      mbar_init(&ctl.raw_full[i], 2);
       mbar_init(&ctl.raw_empty[i], KT_EXPANDERS + 1);   // values expanded, scores computed
     }
     for (int i = 0; i < KT_VALS; ++i) {
@@ -433,59 +441,66 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
   // 128 x (72 + 72 + 184 + 184) registers = 65,536, what 512 threads x 128 were launched with.
   if (warp < 4) {
     cp_reg_dec<72>();
-    if (warp == 0) {
-      // ---------------------------------------------------------------- producer: raw blocks
+    if (warp == 0 || warp == 2) {
+      // ------------------------------------------- producers: raw keys and the scales; raw values
+      const int side = static_cast<int>(warp >> 1);
       const int lg = p.cache.page_log2, pages = KT_BN >> lg;
       const uint32_t bytes = static_cast<uint32_t>(KV_D) << lg;
       KtWalk w;
       bool ok = true;
       uint32_t g = 0;
-      for (bool more = w.start(p, ctl); ok && more; more = w.next(p)) {
+      for (w.start(ctl); ok && w.locate(p); w.pos += w.n) {
         const int b = w.entry / p.nqt, end = w.span.start + w.span.count;
         const int* row = p.batch.pages + static_cast<long long>(b) * p.batch.cols;
-        // lane l looks page l of a block up, a block ahead
-        int pid = 0;
-        uint32_t ex = 0;
-        auto look_up = [&](int j) {
-          pid = 0;
-          ex = 0;
-          const int at = w.key0(j) + (static_cast<int>(lane) << lg);
-          if (j >= w.n || static_cast<int>(lane) >= pages || at >= end) return;
-          const int col = at >> lg;
-          pid = col < p.batch.cols ? row[col] : -1;
+        // Lane l looks page l of a block up: its number three blocks ahead, its exponents two, because each is a load that
+        // may go to memory (pages of 16, 32 x 4 queries over 4096 keys, 64 / 8 heads: WAS us with both a block ahead, one
+        // warp for keys and values, NOW so).
+        auto there = [&](int j) {
+          return j < w.n && static_cast<int>(lane) < pages && w.key0(j) + (static_cast<int>(lane) << lg) < end;
+        };
+        auto number = [&](int j) -> int {
+          const int col = (w.key0(j) >> lg) + static_cast<int>(lane);
+          return !there(j) ? 0 : col < p.batch.cols ? row[col] : -1;
+        };
+        auto exponents = [&](int j, int& pid) -> uint32_t {   // of pages that are not there: 0
+          if (!there(j)) return 0u;   // number 0
           if (pid < 0 || pid >= p.cache.num_pages) {
             report_status(p.status, CB_BAD_ARGUMENT, 2, 0xA04);
             pid = 0;
           }
-          ex = *reinterpret_cast<const uint16_t*>(p.cache.exp_of(pid, w.head, 0));
+          return *reinterpret_cast<const uint16_t*>(p.cache.exp_of(pid, w.head, 0));
         };
-        look_up(0);
+        int pid = number(0), pid1 = number(1), pid2 = number(2);
+        uint32_t ex = exponents(0, pid), ex1 = exponents(1, pid1);
         for (int j = 0; ok && j < w.n; ++j, ++g) {
+          const int pid3 = number(j + 3);
+          const uint32_t ex2 = exponents(j + 2, pid2);
           const uint32_t s = g % KT_RAWS;
           if (g >= KT_RAWS)
             ok = mbar_wait_warp(&ctl.raw_empty[s], (g / KT_RAWS - 1) & 1u, &ctl.abort_flag, p.status, 0xA30);
           if (!ok) break;
-          const bool there = static_cast<int>(lane) < pages && w.key0(j) + (static_cast<int>(lane) << lg) < end;
-          const int ek = static_cast<int8_t>(ex), ev = static_cast<int8_t>(ex >> 8);
-          int top_k = __reduce_max_sync(0xffffffffu, there ? ek : KV_EXP_MIN);
-          int top_v = __reduce_max_sync(0xffffffffu, there ? ev : KV_EXP_MIN);
-          if (top_k == KV_EXP_MIN) top_k = 0;   // all zero
-          if (top_v == KV_EXP_MIN) top_v = 0;
-          const bool same_k = __all_sync(0xffffffffu, !there || ek == top_k);
-          const bool same_v = __all_sync(0xffffffffu, !there || ev == top_v);
-          // The scores of block g - 3 are complete: those are issued after the probabilities of g - 5 have come, so
-          // that no softmax reads the scales of g - 8 any more.
-          if (lane < 8) ctl.exps[g % KT_SCALES][lane] = static_cast<uint16_t>(ex);   // pages that are not there: 0
-          if (lane == 0) ctl.blk[g % KT_SCALES] = make_int4(top_k, top_v, same_k, same_v);
+          if (side == 0) {
+            const int top = __reduce_max_sync(0xffffffffu, there(j) ? static_cast<int8_t>(ex >> 8) : KV_EXP_MIN);
+            const uint32_t mine = __shfl_sync(0xffffffffu, ex, (16 * (lane & 7u)) >> lg);
+            const int ek = static_cast<int8_t>(mine);
+            int ev = static_cast<int8_t>(mine >> 8);
+            // Values that are all zero do not matter but their probabilities do, in the sum; as do those of values too small
+            // to be seen beside the block's largest.
+            ev = ev == KV_EXP_MIN ? (top == KV_EXP_MIN ? 0 : top) : max(ev, top - 60);
+            // The scores of block g - 3 are complete: those are issued after the probabilities of g - 5 have come, so
+            // that no softmax reads the scales of g - 8 any more.
+            if (lane < 8)   // of pages that are not there: 0 and 0
+              ctl.scale[g % KT_SCALES][lane] = static_cast<uint32_t>(ek + 127) << 23 | static_cast<uint32_t>(ev + 128);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.sc_full[g % KT_SCALES]);
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&ctl.raw_full[s], KT_RAW / 2);
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.sc_full[g % KT_SCALES]);
-          if (lane == 0) mbar_arrive_expect_tx(&ctl.raw_full[s], KT_RAW);
-          __syncwarp();
-          const int src = __shfl_sync(0xffffffffu, pid, lane >> 1);
-          if (static_cast<int>(lane) < 2 * pages)
-            bulk_load_1d(sR + s * KT_RAW + (lane & 1u) * (KT_BN * KV_D) + (lane >> 1) * bytes,
-                         p.cache.tile(src, w.head, lane & 1u), bytes, &ctl.raw_full[s]);
-          look_up(j + 1);
+          if (static_cast<int>(lane) < pages)
+            bulk_load_1d(sR + s * KT_RAW + side * (KT_RAW / 2) + lane * bytes, p.cache.tile(pid, w.head, side), bytes,
+                         &ctl.raw_full[s]);
+          pid = pid1, pid1 = pid2, pid2 = pid3;
+          ex = ex1, ex1 = ex2;
         }
       }
     } else if (warp == 1) {
@@ -551,7 +566,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
       KtWalk w;
       bool ok = true;
       uint32_t seg = 0;
-      for (bool more = w.start(p, ctl); ok && more; more = w.next(p), ++seg) {
+      for (w.start(ctl); ok && w.locate(p); w.pos += w.n, ++seg) {
         ok = wait_all(&ctl.q_full, seg & 1u, 0xA35);
         for (int j = 0; ok && j < 2 && j < w.n; ++j) ok = issue_qk(j, j + 1 == w.n);
         for (int j = 0; ok && j < w.n; ++j) {
@@ -582,7 +597,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
     bool ok = q < active;
     uint32_t count = 0;                                    // blocks this stream has seen
     uint32_t seg = 0, g0 = 0;
-    for (bool more = w.start(p, ctl); ok && more; more = w.next(p), ++seg) {
+    for (w.start(ctl); ok && w.locate(p); w.pos += w.n, ++seg) {
       const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, tok = qt * p.qrows + q_in_tile;
       const bool query = row < tile_rows && tok < w.span.count;
       const bool padded = __any_sync(0xffffffffu, !query);   // the loads of tensor memory below want a converged warp
@@ -596,29 +611,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
         if (!ok) break;
         ++count;
         tc_fence_after_sync();
-        const int4 blk = ctl.blk[g % KT_SCALES];
-        const float2 sc = make_float2(kv_pow2(blk.x), static_cast<float>(blk.y));
+        const uint32_t* scales = ctl.scale[g % KT_SCALES] + part * (kKeys / 16);
         if (j == t) row_scale = p.scale_log2 * kv_pow2(ctl.row_exp[seg & 1u][r]);
-        const float scale = fmaxf(row_scale * sc.x, 1.2e-38f);
         uint32_t s[kKeys];
 #pragma unroll
         for (int i = 0; i < kKeys; i += 32) tmem_ld_32x32_at(tS + part * kKeys + i, &s[i]);
         tmem_wait_ld();
-        if (blk.z == 0) {   // other exponents of keys in the block
-#pragma unroll
-          for (int i = 0; i < kKeys / 16; ++i) {
-            int e = static_cast<int8_t>(ctl.exps[g % KT_SCALES][(kKeys * part + 16 * i) >> p.cache.page_log2]) - blk.x;
-            e = e > 0 ? 0 : e < -126 ? -126 : e;
-            const float f = kv_pow2(e);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) s[16 * i + k] = __float_as_uint(__uint_as_float(s[16 * i + k]) * f);
-          }
-        }
         const int key0 = w.key0(j) + kKeys * part;
         if (key0 + kKeys - 1 > tile_first || padded) kt_mask(s, query ? q_pos - key0 + 1 : 0);
         if (p.window > 0 && key0 <= tile_last - p.window && key0 + kKeys > p.sinks)
           kt_mask_between(s, max(p.sinks - key0, 0), min(q_pos - p.window + 1 - key0, kKeys));
-        const float mx = fmaf(kt_max(s), scale, sc.y);
+        const float mx = kt_row_max(s, scales, row_scale, std::make_integer_sequence<int, kKeys / 16>());
         // The running maximum, raised when a score passes it by 2^8, for all rows of the warp (see cp_update_max).
         const bool grow = query && (mx > m_ref + CP_RESCALE_THRESHOLD || (m_ref == -INFINITY && mx > -INFINITY));
         if (__any_sync(0xffffffffu, grow)) {
@@ -638,9 +641,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
             }
           }
         }
-        const float plus = sc.y - (m_ref == -INFINITY ? 0.f : m_ref);
-        uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull};
-        kt_probabilities<0, (kCopies > 1 ? kKeys : 64)>(s, scale, plus, sum4);
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        l += kt_probabilities<0, (kCopies > 1 ? kKeys : 64)>(s, scales, row_scale, m_use);
         if (kCopies == 1) {
           tmem_st_32x32_at(tS, &s[0]);
         } else {
@@ -661,16 +663,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.p_first[t]);
         if constexpr (kCopies == 1) {
-          kt_probabilities<64, 128>(s, scale, plus, sum4);
+          l += kt_probabilities<64, 128>(s, scales, row_scale, m_use);
           tmem_st_32x32_at(tS + 32u, &s[32]);
           tmem_wait_st();
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctl.p_rest[t]);
         }
-        float sum = 0.f;
-        cp_add_sums(sum4, sum);
-        l = fmaf(sum, kv_pow2(-static_cast<int>(sc.y)), l);
       }
       if (!ok) break;
       // -------------------------------------------- end of the segment: merge the streams
