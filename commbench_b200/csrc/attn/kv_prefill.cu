@@ -102,11 +102,12 @@ extern "C" {
 // 24000 keys, 64 / 8 heads: 129 us with one tile, 222 with two), however the rows are spread over sequences.
 //   Many: a key of a head is expanded in 150 ps, and a pair of 128-row tiles of one query head visits 128 keys in 1.3 us on
 // one SM; a call has 10 beside.
-//   Tiles: 128 keys of a head and tile of 128 rows take an SM 1.3 us, of up to 64 rows 1.1, evenly cut, and a call 17 us.
-// Measured, few / tiles / many (sequences x queries, keys, heads): 1 x 64, 4160, 8 / 2: 18 / 23 / 64; 4 x 16, 6000, 64 / 8: 68 /
-// 37 / 196; 1 x 128, 4224, 32 / 8: 53 / 34 / 69; 1 x 256, 4352, 8 / 2: 30 / 28 / 68; 1 x 1000, 5096, 4 / 1: 62 / 33 / 77;
-// 2 x 256, 256, 32 / 8: 46 / 25 / 16; 1 x 1000, 7000, 32 / 8: 535 / 164 / 122; 16 x 4, 6000, 64 / 8: 72 / 60 / 700;
-// 16 x 1, 6001, 32 / 8: 39 / 58 / 446.
+//   Tiles: 128 keys of a head and tile of 128 rows take an SM 1.7 us, of up to 64 rows 1.0, evenly cut; a call has 19 and 17
+// beside.
+// Measured, few / tiles / many (sequences x queries, keys, heads): 1 x 64, 4160, 8 / 2: 18 / 22 / 64; 4 x 16, 6000, 64 / 8: 68 /
+// 36 / 196; 1 x 128, 4224, 32 / 8: 53 / 32 / 69; 1 x 256, 4352, 8 / 2: 30 / 27 / 68; 1 x 1000, 5096, 4 / 1: 62 / 32 / 78;
+// 2 x 256, 256, 32 / 8: 46 / 24 / 16; 1 x 1000, 7000, 32 / 8: 535 / 174 / 121; 16 x 4, 6000, 64 / 8: 72 / 53 / 700;
+// 16 x 1, 6001, 32 / 8: 39 / 50 / 446.
 int cb_kv_attend_form(int B, int S, int Hq, int Hkv, int window, int max_len) {
   if (B < 1 || S < 1 || Hkv < 1 || Hq < 1 || max_len < 1) return 0;
   const float group = static_cast<float>(Hq / Hkv), rows = static_cast<float>(S) * group;
@@ -114,10 +115,10 @@ int cb_kv_attend_form(int B, int S, int Hq, int Hkv, int window, int max_len) {
   if (window > 0 && static_cast<float>(window) + S < keys) keys = static_cast<float>(window) + S;
   const float heads = static_cast<float>(B) * Hkv;
   const float few = 8.f + heads * keys * (rows <= 16.f ? 37e-6f : 73e-6f * ceilf(rows / 32.f));
-  const float waves = ceilf(ceilf(static_cast<float>(S) / (2 * CP_BM)) * B * Hq / 148.f);
+  const float rounds = ceilf(ceilf(static_cast<float>(S) / (2 * CP_BM)) * B * Hq / 148.f);
   // a query in the middle of a chunk sees the chunk's first half
   const float seen = window > 0 ? keys : keys - 0.5f * S;
-  const float many = 10.f + heads * keys * 150e-6f + waves * 1.3f * seen / CP_BN;
+  const float many = 10.f + heads * keys * 150e-6f + rounds * 1.3f * seen / CP_BN;
   float best = few;
   int form = 0;
   if (many < best) best = many, form = 1;
@@ -126,7 +127,7 @@ int cb_kv_attend_form(int B, int S, int Hq, int Hkv, int window, int max_len) {
     const float tiles = ceilf(static_cast<float>(S) / qrows);
     const float of_tile = window > 0 ? static_cast<float>(window) + qrows < keys ? window + qrows : keys : seen;
     const float blocks = heads * tiles * ceilf(of_tile / CP_BN + 0.5f);
-    const float cut = 17.f + (tile_rows <= 64.f ? 1.1f : 1.3f) * ceilf(blocks / 148.f);
+    const float waves = ceilf(blocks / 148.f), cut = tile_rows <= 64.f ? 17.f + 1.f * waves : 19.f + 1.7f * waves;
     if (cut < best && tiles * B <= 128.f) form = 2;
   }
   return form;

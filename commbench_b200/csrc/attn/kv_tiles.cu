@@ -18,12 +18,13 @@
 //     memory, as in fa_split.cu, and the flat list of (sequence, query tile, head, block) is cut evenly over the
 //     CTAs as there - by the lengths that the device holds.
 //
-// Measured, 64 / 8 heads, pages of 64: 16 sequences x 4 queries (32 rows) over 6000 / 24000 keys 60 / 194 us (the form of
-// few rows 72 / 223, 196 and 786 MB of cache), 16 x 8 over 6000 70 (134), 4 x 16 over 6000 37 (68).  A block of 128 keys
-// takes an SM 1.1 us, 1.3 with more than 64 rows: two products of 128 x 128 x 128, 0.54 us of the tensor cores, whose
-// operands and tiles move 176 KB through shared memory (0.72 us at 128 bytes a cycle), and the one warp that issues them
-// waits for nothing but its own barriers any more.  With keys expanded as well and one copy of a row it were
-// 1.65 us.
+// Measured, 64 / 8 heads, pages of 64: 16 sequences x 4 queries (32 rows) over 6000 / 24000 keys 53 / 182 us (the form of
+// few rows 72 / 224; 196 and 786 MB of cache), 16 x 8 over 6000 60 (132), 4 x 16 over 6000 36 (68).  A block of 128 keys
+// takes an SM 1.0 us, 1.7 with more than 64 rows.  Of that two products of 128 x 128 x 128 are 0.54 us of the tensor cores,
+// and 176 KB go through shared memory (0.72 us at 128 bytes a cycle): with up to 64 rows the warp that issues the products
+// waits for little else, with more for the softmax of the block, 2600 cycles.  With the keys expanded as well and one copy of
+// each row it was 1.65 us.  A call has 17 us beside its blocks: 5 until the first block is known and its query
+// tile made, 3 for the end of a segment, the merge of what was cut.
 // Every mbarrier wait is bounded (see mbarrier.cuh).
 #include <math.h>
 
@@ -290,21 +291,20 @@ __device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, 
     {
       const int b = w.entry / p.nqt, qt = w.entry - b * p.nqt, chunk = tid & 7;
 #pragma unroll 1
-      for (int r = tid >> 3; r < CP_BM; r += 4 * KT_EXPANDERS) {
-        const int row = r & (CP_BM / kCopies - 1), in = row / p.group, tok = qt * p.qrows + in;
+      for (int row = tid >> 3; row < CP_BM / kCopies; row += 4 * KT_EXPANDERS) {
+        const int in = row / p.group, tok = qt * p.qrows + in;
         const bool there = row < tile_rows && tok < w.span.count;
         const __nv_bfloat16* src = p.q + b * p.q_sb + tok * p.q_ss +
                                    static_cast<long long>(w.head * p.group + row - in * p.group) * p.q_sh + 16 * chunk;
-        float x[16];
-        float amax = 0.f;
+        uint2 raw[4];
+        __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint2 raw = there ? *reinterpret_cast<const uint2*>(src + 4 * i) : make_uint2(0u, 0u);
-          const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-          const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-          x[4 * i] = f0.x, x[4 * i + 1] = f0.y, x[4 * i + 2] = f1.x, x[4 * i + 3] = f1.y;
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y))));
+          raw[i] = there ? *reinterpret_cast<const uint2*>(src + 4 * i) : make_uint2(0u, 0u);
+          top = __hmax2(top, __hmax2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].x)),
+                                     __habs2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].y))));
         }
+        float amax = fmaxf(__low2float(top), __high2float(top));
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         int e = static_cast<int>(__float_as_uint(amax) >> 23) - 134;
@@ -313,25 +313,27 @@ __device__ __forceinline__ void kt_expander(const KvTilesParams& p, KtCtl& ctl, 
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float rest[4];
           hi[i] = lo[i] = 0;
 #pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            const float2 v = make_float2(x[4 * i + k] * down, x[4 * i + k + 1] * down);
-            const uint32_t two = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
-            const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-            const float2 f = __half22float2(__half2(back));
-            rest[k] = v.x - f.x, rest[k + 1] = v.y - f.y;
-            hi[i] |= two << (8 * k);
+          for (int k = 0; k < 2; ++k) {   // fp16 holds the scaled number and its difference from the first term
+            const uint32_t two = k ? raw[i].y : raw[i].x;
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two));
+            const __half2 v = __floats2half2_rn(f.x * down, f.y * down);
+            const uint32_t first = __nv_cvt_halfraw2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
+            const __half2 back =
+                __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(first), __NV_E4M3));
+            hi[i] |= first << (16 * k);
+            lo[i] |= static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(__hsub2(v, back), __NV_SATFINITE, __NV_E4M3)) << (16 * k);
           }
-          lo[i] = __nv_cvt_float2_to_fp8x2(make_float2(rest[0], rest[1]), __NV_SATFINITE, __NV_E4M3) |
-                  static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(rest[2], rest[3]), __NV_SATFINITE, __NV_E4M3))
-                      << 16;
         }
-        uint8_t* dst = sQ + r * KV_D + ((chunk ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(dst + KT_Q8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (chunk == 0) ctl.row_exp[seg & 1u][r] = static_cast<int8_t>(e);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int r = row + i * (CP_BM / kCopies);
+          uint8_t* dst = sQ + r * KV_D + ((chunk ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(dst + KT_Q8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          if (chunk == 0) ctl.row_exp[seg & 1u][r] = static_cast<int8_t>(e);
+        }
       }
     }
     fence_proxy_async_smem();
@@ -453,8 +455,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) kv_tiles_kernel(const __grid_co
         const int b = w.entry / p.nqt, end = w.span.start + w.span.count;
         const int* row = p.batch.pages + static_cast<long long>(b) * p.batch.cols;
         // Lane l looks page l of a block up: its number three blocks ahead, its exponents two, because each is a load that
-        // may go to memory (pages of 16, 32 x 4 queries over 4096 keys, 64 / 8 heads: WAS us with both a block ahead, one
-        // warp for keys and values, NOW so).
+        // may go to memory (pages of 16, 32 x 4 queries over 4096 keys, 64 / 8 heads: 94 us with both a block ahead and one
+        // warp for keys and values, 78 so).
         auto there = [&](int j) {
           return j < w.n && static_cast<int>(lane) < pages && w.key0(j) + (static_cast<int>(lane) << lg) < end;
         };
