@@ -117,7 +117,7 @@ int cb_kv_attend_form(int B, int S, int Hq, int Hkv, int window, int max_len) {
   const float few = 8.f + heads * keys * (rows <= 16.f ? 37e-6f : 73e-6f * ceilf(rows / 32.f));
   const float rounds = ceilf(ceilf(static_cast<float>(S) / (2 * CP_BM)) * B * Hq / 148.f);
   // a query in the middle of a chunk sees the chunk's first half
-  const float seen = window > 0 ? keys : keys - 0.5f * S;
+  const float seen = window > 0 ? fminf(keys, static_cast<float>(window + 2 * CP_BM)) : keys - 0.5f * S;
   const float many = 10.f + heads * keys * 150e-6f + rounds * 1.3f * seen / CP_BN;
   float best = few;
   int form = 0;
@@ -125,7 +125,7 @@ int cb_kv_attend_form(int B, int S, int Hq, int Hkv, int window, int max_len) {
   if (rows > 16.f && group <= CP_BM) {
     const float qrows = fminf(floorf(CP_BM / group), static_cast<float>(S)), tile_rows = qrows * group;
     const float tiles = ceilf(static_cast<float>(S) / qrows);
-    const float of_tile = window > 0 ? static_cast<float>(window) + qrows < keys ? window + qrows : keys : seen;
+    const float of_tile = window > 0 ? fminf(keys, window + qrows) : seen;
     const float blocks = heads * tiles * ceilf(of_tile / CP_BN + 0.5f);
     const float waves = ceilf(blocks / 148.f), cut = tile_rows <= 64.f ? 17.f + 1.f * waves : 19.f + 1.7f * waves;
     if (cut < best && tiles * B <= 128.f) form = 2;

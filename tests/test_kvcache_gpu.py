@@ -391,6 +391,25 @@ def test_attend_tiles_of_many_sequences(native_lib, B):
     _case([8 + (i * 7919) % 500 for i in range(B)], 4, 8, 1, 32, max_len=520, seed=120)
 
 
+def test_pages_past_32_bits(native_lib):
+    """A cache of more than 4 GB whose last pages are used, beside its first."""
+    from commbench_b200.ops.kvcache import KVCache8
+
+    page, H, lens = 64, 8, (700, 300)
+    n = 2 ** 32 // (H * 2 * page * D) + 40
+    cache = KVCache8(n, H, page=page)
+    k, v = _kv(2, 700, H, 130)
+    pages = torch.stack([torch.arange(n - 11, n, device="cuda"), torch.arange(11, device="cuda")]).int()
+    cache.append(k, v, pages, _ints(0, 0), count=_ints(*lens))
+    rk, rv = cache.read(pages, None, 700, length=_ints(*lens))
+    kc, vc = _quantised(k, page, lens), _quantised(v, page, lens)
+    assert torch.equal(rk.double(), kc) and torch.equal(rv.double(), vc)
+    q = torch.randn(2, 5, 16, D, device="cuda", generator=_gen(131)).bfloat16()
+    want = _attend64(q, kc, vc, (695, 295), (5, 5), 0, 0)
+    for impl in ("decode", "prefill", "tiles"):
+        _check(*cache.attend(q, pages, _ints(695, 295), impl=impl), want)
+
+
 def test_attend_repeats_its_bits_and_runs_on_another_stream(native_lib):
     k, v = _kv(3, 1500, 2, 70)
     cache, pages = _filled(k, v, 64, (1500, 700, 64), 71)
