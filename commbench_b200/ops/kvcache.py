@@ -160,7 +160,7 @@ class KVCache8:
         ``window`` > 0: a query at p sees the keys j > p - window, and the first ``sinks`` tokens of the sequence.
         Rows that see no key, and the rows from ``count[b]`` on, are zeros with lse -inf.  ``max_len``: an upper
         bound of ``start + count`` that the host knows (default: what the table has room for); workspaces and the
-        cut of the work go by it, and later tokens are not seen.  A page id out of range leaves a status word, is
+        cut of the work go by it; whether later tokens are seen is not said.  A page id out of range leaves a status word, is
         not read, and makes the rows that should see it meaningless.
 
         ``impl``: "decode" (few query rows, bound by the cache's bytes), "tiles" (more of them: tcgen05 tiles,
